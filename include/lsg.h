@@ -573,6 +573,93 @@ LSG_API size_t lsg_nvfp4_sf_buffer_bytes(int rows, int K);
 LSG_API int lsg_nvfp4_reformat_scales(const float* src, void* dst, int rows, int K, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* 8-bit integers: one scale per token and per output channel                */
+/* No counterpart in the reference (its 8-bit family is FP8); the entries    */
+/* stand beside lsg_dynamic_fp8_quant / lsg_weight_fp8_quant / lsg_fp8_gemm. */
+/* ------------------------------------------------------------------------ */
+
+/* Per-row quantizer: a = max |x[r,:]|, scales[r] = a / 127 in fp32, codes[r,k] = 127 x[r,k] / a
+ * rounded to the nearest integer, half-way cases to the even one (exactly: the code is the one of
+ * the unrounded quotient).  An all-zero row gets scale 0 and codes 0, a row with an infinity or a
+ * NaN scale NaN and codes 0.  x: bf16 or fp16 (lsg_dtype), row stride ldx values; codes: int8, row
+ * stride ldq bytes, a multiple of 16, rows on 16-byte boundaries (bytes from K to ldq are left as
+ * they are); scales: fp32 [rows].  Rows may be tokens of an activation or output channels of a
+ * weight.  Rows that are whole 16-byte pieces of at most 16384 values are read once. */
+LSG_API int lsg_dynamic_int8_quant(const void* x, long long ldx, int dtype, void* codes, long long ldq, float* scales,
+                                   long long rows, int K, void* stream);
+/* The same of silu(gate) * up, formed in fp32 and not rounded in between; gate, up: bf16, fp16 or
+ * f32 with row strides ldg, ldu (the halves of one [rows, 2 K] matrix, say). */
+LSG_API int lsg_silu_mul_int8_quant(const void* gate, long long ldg, const void* up, long long ldu, int dtype,
+                                    void* codes, long long ldq, float* scales, long long rows, int K, void* stream);
+/* The same of a token matrix, written to the rows of its (token, slot) pairs: the codes and scale of
+ * hidden[t] go to rows inv_perm[t*top_k + s].  Each token is read and quantized once.  Pairs whose
+ * entry lies outside [0, num_tokens*top_k) are left out; rows no pair names are left as they are. */
+LSG_API int lsg_moe_permute_int8(const void* hidden, long long ld, int dtype, const int32_t* inv_perm, int num_tokens,
+                                 int top_k, int H, void* codes, long long ldq, float* scales, void* stream);
+
+/* D[m,n] = scale_A[m] * scale_B[n] * sum_k A[m,k] B[n,k], the sum exact in int32, the scales applied in
+ * fp32, one rounding to the output type.  1 <= K <= 131056; row strides lda, ldb are multiples of 16
+ * bytes, operand rows start on 16-byte boundaries and are readable up to K rounded up to 16 (what
+ * lies behind K does not matter).  Any M and N. */
+typedef struct lsg_int8_gemm_params {
+    int M, N, K;
+    const void* A;        /* int8 [M, K]                        */
+    long long lda;
+    const void* B;        /* int8 [N, K]                        */
+    long long ldb;
+    void* D;              /* [M, N] output_dtype, contiguous    */
+    const float* scale_A; /* [M]                                */
+    const float* scale_B; /* [N]                                */
+    int output_dtype;     /* LSG_DTYPE_BF16, _F16 or _F32       */
+} lsg_int8_gemm_params;
+LSG_API int lsg_int8_gemm(const lsg_int8_gemm_params* p, void* stream);
+/* lsg_dynamic_int8_quant and lsg_int8_gemm in one call: p->A is the bf16 or fp16 activation with row
+ * stride p->lda VALUES, p->scale_A is ignored.  The same bits as the two calls.  Workspace:
+ * lsg_int8_gemm_from_bf16_workspace_bytes(M, K), 256-byte aligned. */
+LSG_API size_t lsg_int8_gemm_from_bf16_workspace_bytes(int M, int K);
+LSG_API int lsg_int8_gemm_from_bf16(const lsg_int8_gemm_params* p, int input_dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* The product for rows grouped by expert: row r of expert e (expert_offsets[e] <= r <
+ * expert_offsets[e+1]) times matrix e.  Routed on the device, no host synchronisation; rows behind
+ * the last expert's are left as they are, offsets past total_tokens are taken as total_tokens.
+ * num_experts <= 1024; K and the strides as above. */
+typedef struct lsg_int8_grouped_gemm_params {
+    int num_experts, N, K;
+    const void* A_base;            /* int8 [total_tokens, K]                 */
+    long long lda;
+    const void* B_base;            /* int8 [num_experts, N, K], row stride ldb, experts N*ldb apart */
+    long long ldb;
+    void* D_base;                  /* [total_tokens, N] output_dtype         */
+    const float* scale_A_base;     /* [total_tokens]                         */
+    const float* scale_B_base;     /* [num_experts, N]                       */
+    const int32_t* expert_offsets; /* [num_experts + 1], device              */
+    int output_dtype;
+} lsg_int8_grouped_gemm_params;
+LSG_API int lsg_int8_grouped_gemm(const lsg_int8_grouped_gemm_params* p, int total_tokens, void* stream);
+
+/* Expert feed-forward block: row inv_perm[t*top_k + s] of D is
+ *   down_e( quant( silu(g) * u ) ),  (g | u) = gate_up_e( quant(hidden[t]) ),  e the row's expert,
+ * with lsg_moe_permute_int8 in front, gate, up and their product in fp32 up to the second quantizer.
+ * H and I multiples of 16.  Workspace: lsg_int8_moe_ffn_workspace_bytes, 256-byte aligned. */
+typedef struct lsg_int8_moe_ffn_params {
+    int num_tokens, top_k, num_experts, H, I;
+    const void* hidden;            /* bf16 or fp16 [num_tokens, H], row stride ld_hidden values */
+    long long ld_hidden;
+    int input_dtype;
+    const int32_t* expert_offsets; /* [num_experts + 1]                      */
+    const int32_t* inv_perm;       /* [num_tokens * top_k], pair -> row      */
+    const void* gate_up;           /* int8 [num_experts, 2 I, H]: gate rows, then up rows */
+    const float* gate_up_scales;   /* [num_experts, 2 I]                     */
+    const void* down;              /* int8 [num_experts, H, I]               */
+    const float* down_scales;      /* [num_experts, H]                       */
+    void* D;                       /* [num_tokens * top_k, H] output_dtype   */
+    int output_dtype;
+} lsg_int8_moe_ffn_params;
+LSG_API size_t lsg_int8_moe_ffn_workspace_bytes(int num_tokens, int top_k, int H, int I);
+LSG_API int lsg_int8_moe_ffn(const lsg_int8_moe_ffn_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* MoE routing, permutation, combine                                        */
 /* No counterpart in the reference: its grouped operators take rows that are */
 /* already grouped by expert (gguf_grouped_gemm.h:20-24).                   */
@@ -585,7 +672,8 @@ LSG_API int lsg_moe_route(const float* logits, int num_tokens, int num_experts, 
 
 /* Stable grouping of the T*k (token, slot) pairs by expert: expert_offsets int32 [E+1],
  * perm int32 [T*k] (row -> pair), inv_perm int32 [T*k] (pair -> row).
- * E <= 1024.  Pairs with an expert id outside [0, E) get no row.
+ * E <= 1024.  Pairs with an expert id outside [0, E) get no row: their entry of inv_perm is -1;
+ * perm is 0 in the rows behind the last expert's, which belong to no pair.
  * counts_scratch: int32 [lsg_moe_permutation_scratch_ints(T, k, E)] (per-chunk histograms
  * of a counting sort over chunks of 256 pairs). */
 LSG_API long long lsg_moe_permutation_scratch_ints(int num_tokens, int top_k, int num_experts);
@@ -667,9 +755,35 @@ LSG_API int lsg_moe_permute(const void* hidden_bf16, const int32_t* perm, int ro
                             void* out_bf16, void* stream);
 
 /* out[t,:] = sum over slots s (in order) of topk_weights[t,s] * y[inv_perm[t*k+s], :],
- * fp32 fused multiply-adds, rounded to bf16. */
+ * fp32 fused multiply-adds, rounded to bf16; pairs without a row (inv_perm < 0) add nothing. */
 LSG_API int lsg_moe_unpermute(const void* y_bf16, const int32_t* inv_perm, const float* topk_weights,
                               int num_tokens, int top_k, int H, void* out_bf16, void* stream);
+
+/* The same two in bf16, fp16 or f32 (lsg_dtype), for any H; rows outside [0, rows) are pairs without
+ * a row (unpermute: they add nothing), perm entries outside the pairs leave their row as it is. */
+LSG_API int lsg_moe_permute_dtype(const void* hidden, int dtype, const int32_t* perm, int rows, int num_tokens, int top_k,
+                                  int H, void* out, void* stream);
+LSG_API int lsg_moe_unpermute_dtype(const void* y, int dtype, const int32_t* inv_perm, const float* topk_weights, int rows,
+                                    int num_tokens, int top_k, int H, void* out, void* stream);
+
+/* Gradients of the three steps (dtype: bf16, fp16 or f32 for rows and tokens, fp32 for weights and
+ * logits; top_k <= 16; sums in fp32 in a fixed order, no atomics).
+ *   permute    grad_hidden[t,:] = sum over slots (in order) of grad_rows[inv_perm[t*k+s],:]
+ *   unpermute  grad_y[inv_perm[t*k+s],:] = topk_weights[t,s] * grad_out[t,:],
+ *              grad_weights[t,s] = sum_h y[inv_perm[t*k+s],h] * grad_out[t,h]
+ *   route      grad_logits[t,topk_idx[t,s]] = w[t,s] (grad_weights[t,s] - sum_r w[t,r] grad_weights[t,r]),
+ *              0 for the experts not chosen (w = topk_weights, the softmax over the chosen logits)
+ * A pair whose entry of inv_perm lies outside [0, rows) has no row: it adds nothing and its weight's
+ * gradient is 0.  Rows of grad_y that no pair names are left as they are, except that with
+ * expert_offsets (int32 [num_experts + 1], may be null) the rows from expert_offsets[num_experts] on
+ * are cleared; rows <= num_tokens * top_k.  No counterpart in the reference (it has no routing). */
+LSG_API int lsg_moe_permute_backward(const void* grad_rows, int dtype, const int32_t* inv_perm, int rows, int num_tokens,
+                                     int top_k, int H, void* grad_hidden, void* stream);
+LSG_API int lsg_moe_unpermute_backward(const void* grad_out, const void* y, int dtype, const int32_t* inv_perm,
+                                       const float* topk_weights, const int32_t* expert_offsets, int num_experts, int rows,
+                                       int num_tokens, int top_k, int H, void* grad_y, float* grad_weights, void* stream);
+LSG_API int lsg_moe_route_backward(const int32_t* topk_idx, const float* topk_weights, const float* grad_weights,
+                                   int num_tokens, int num_experts, int top_k, float* grad_logits, void* stream);
 
 #ifdef __cplusplus
 }

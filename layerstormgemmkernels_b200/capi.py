@@ -82,6 +82,30 @@ class Fp8GroupedGemmParams(ctypes.Structure):
                 ("output_dtype", ctypes.c_int), ("B_ptrs", ctypes.c_void_p), ("scale_B_ptrs", ctypes.c_void_p)]
 
 
+class Int8GemmParams(ctypes.Structure):
+    _fields_ = [("M", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int), ("A", ctypes.c_void_p),
+                ("lda", ctypes.c_longlong), ("B", ctypes.c_void_p), ("ldb", ctypes.c_longlong),
+                ("D", ctypes.c_void_p), ("scale_A", ctypes.c_void_p), ("scale_B", ctypes.c_void_p),
+                ("output_dtype", ctypes.c_int)]
+
+
+class Int8GroupedGemmParams(ctypes.Structure):
+    _fields_ = [("num_experts", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int),
+                ("A_base", ctypes.c_void_p), ("lda", ctypes.c_longlong), ("B_base", ctypes.c_void_p),
+                ("ldb", ctypes.c_longlong), ("D_base", ctypes.c_void_p), ("scale_A_base", ctypes.c_void_p),
+                ("scale_B_base", ctypes.c_void_p), ("expert_offsets", ctypes.c_void_p),
+                ("output_dtype", ctypes.c_int)]
+
+
+class Int8MoeFfnParams(ctypes.Structure):
+    _fields_ = [("num_tokens", ctypes.c_int), ("top_k", ctypes.c_int), ("num_experts", ctypes.c_int),
+                ("H", ctypes.c_int), ("I", ctypes.c_int), ("hidden", ctypes.c_void_p),
+                ("ld_hidden", ctypes.c_longlong), ("input_dtype", ctypes.c_int),
+                ("expert_offsets", ctypes.c_void_p), ("inv_perm", ctypes.c_void_p), ("gate_up", ctypes.c_void_p),
+                ("gate_up_scales", ctypes.c_void_p), ("down", ctypes.c_void_p), ("down_scales", ctypes.c_void_p),
+                ("D", ctypes.c_void_p), ("output_dtype", ctypes.c_int)]
+
+
 class Nvfp4GemmParams(ctypes.Structure):
     _fields_ = [("M", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int), ("A", ctypes.c_void_p),
                 ("B", ctypes.c_void_p), ("D", ctypes.c_void_p), ("scale_A", ctypes.c_void_p),
@@ -173,6 +197,20 @@ def _load():
         "lsg_moe_permutation": (ci, [vp, ci, ci, ci, vp, vp, vp, vp, vp]),
         "lsg_moe_permute": (ci, [vp, vp, ci, ci, ci, vp, vp]),
         "lsg_moe_unpermute": (ci, [vp, vp, vp, ci, ci, ci, vp, vp]),
+        "lsg_dynamic_int8_quant": (ci, [vp, ll, ci, vp, ll, vp, ll, ci, vp]),
+        "lsg_silu_mul_int8_quant": (ci, [vp, ll, vp, ll, ci, vp, ll, vp, ll, ci, vp]),
+        "lsg_moe_permute_int8": (ci, [vp, ll, ci, vp, ci, ci, ci, vp, ll, vp, vp]),
+        "lsg_int8_gemm": (ci, [ctypes.POINTER(Int8GemmParams), vp]),
+        "lsg_int8_gemm_from_bf16_workspace_bytes": (sz, [ci, ci]),
+        "lsg_int8_gemm_from_bf16": (ci, [ctypes.POINTER(Int8GemmParams), ci, vp, sz, vp]),
+        "lsg_int8_grouped_gemm": (ci, [ctypes.POINTER(Int8GroupedGemmParams), ci, vp]),
+        "lsg_int8_moe_ffn_workspace_bytes": (sz, [ci, ci, ci, ci]),
+        "lsg_int8_moe_ffn": (ci, [ctypes.POINTER(Int8MoeFfnParams), vp, sz, vp]),
+        "lsg_moe_permute_dtype": (ci, [vp, ci, vp, ci, ci, ci, ci, vp, vp]),
+        "lsg_moe_unpermute_dtype": (ci, [vp, ci, vp, vp, ci, ci, ci, ci, vp, vp]),
+        "lsg_moe_permute_backward": (ci, [vp, ci, vp, ci, ci, ci, ci, vp, vp]),
+        "lsg_moe_unpermute_backward": (ci, [vp, vp, ci, vp, vp, vp, ci, ci, ci, ci, ci, vp, vp, vp]),
+        "lsg_moe_route_backward": (ci, [vp, vp, vp, ci, ci, ci, vp, vp]),
         "lsg_gguf_dequant_gemm": (ci, [ctypes.POINTER(GgufMmvqParams), vp]),
         "lsg_gguf_dequant_blocks": (ci, [vp, vp, ci, ll, vp]),
     }

@@ -1,0 +1,232 @@
+// Products of 8-bit integers with a scale per token and per output channel:
+//
+//   D[m, n] = scale_A[m] * scale_B[n] * sum_k A[m, k] B[n, k]        A, B int8, the sum in int32
+//
+// dense, and for rows grouped by expert.  The sum is exact (128 * 128 * K stays below 2^31 for the K
+// accepted here), so results do not depend on how K is cut; it is converted to fp32, multiplied by
+// the two scales in fp32 and rounded once to the output type.
+#include "common.cuh"
+#include "host.h"
+#include "int8.cuh"
+
+namespace lsg {
+
+namespace {
+
+// One warp per output column and unit of up to eight token rows, lanes striding over 16-byte pieces
+// of the weight row.
+__global__ void __launch_bounds__(256)
+int8_dot_kernel(const Int8Gemm a) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    const int lane = threadIdx.x & 31;
+    const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
+    int expert = 0, r0 = blockIdx.y * 8, rows = min(8, a.M - r0);
+    if (a.expert_offsets && !find_unit(a.expert_offsets, a.E, a.M, 8, blockIdx.y, expert, r0, rows)) return;
+    if (n >= a.N || rows <= 0) return;
+    const int8_t* w = a.B + (static_cast<long long>(expert) * a.N + n) * a.ldb;
+    int acc[8];
+#pragma unroll
+    for (int m = 0; m < 8; ++m) acc[m] = 0;
+    for (int k = lane * 16; k < a.K; k += 512) {
+        const int4 wv = __ldg(reinterpret_cast<const int4*>(w + k));
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+            if (m < rows) {
+                int4 xv = *reinterpret_cast<const int4*>(a.A + (r0 + m) * a.lda + k);
+                if (k + 16 > a.K) xv = keep_bytes(xv, a.K - k);
+                acc[m] = dp4a_ss(wv.x, xv.x, dp4a_ss(wv.y, xv.y, dp4a_ss(wv.z, xv.z, dp4a_ss(wv.w, xv.w, acc[m]))));
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < 8; ++m) acc[m] = __reduce_add_sync(0xffffffffu, acc[m]);
+    if (lane < rows) {
+        int v = acc[0];
+#pragma unroll
+        for (int m = 1; m < 8; ++m) v = lane == m ? acc[m] : v;
+        const int row = r0 + lane;
+        store_out(a.D, a.out_dtype, static_cast<size_t>(row) * a.N + n,
+                  static_cast<float>(v) * a.scale_A[row] * a.scale_B[static_cast<long long>(expert) * a.N + n]);
+    }
+}
+
+int check(const char* op, int N, int K, const void* A, long long lda, const void* B, long long ldb, const void* D, int dt) {
+    if (dt != LSG_DTYPE_BF16 && dt != LSG_DTYPE_F16 && dt != LSG_DTYPE_F32)
+        return fail(LSG_ERR_UNSUPPORTED, "%s: output dtype must be bf16, fp16 or f32", op);
+    if (K < 1 || K > kInt8MaxK)
+        return fail(LSG_ERR_INVALID, "%s: need 1 <= K <= %d, where the int32 sums cannot overflow (K=%d)", op, kInt8MaxK, K);
+    if (lda < K || ldb < K) return fail(LSG_ERR_INVALID, "%s: a row stride is smaller than K", op);
+    if (!A || !B || !D) return fail(LSG_ERR_INVALID, "%s: null pointer", op);
+    if (((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) || lda % 16 || ldb % 16)
+        return fail(LSG_ERR_ALIGNMENT, "%s: operand rows must start on 16-byte boundaries", op);
+    if (reinterpret_cast<uintptr_t>(D) & (dt == LSG_DTYPE_F32 ? 3 : 1))
+        return fail(LSG_ERR_ALIGNMENT, "%s: the output is not aligned to its type", op);
+    return LSG_OK;
+}
+
+}  // namespace
+
+int int8_gemm(const Int8Gemm& a, cudaStream_t s) {
+    const long long units = a.expert_offsets ? a.M / 8 + static_cast<long long>(a.E) : (a.M + 7) / 8;
+    if (units > 65535) return fail(LSG_ERR_UNSUPPORTED, "int8 product: too many rows");
+    LSG_CUDA_TRY(launch_kernel(int8_dot_kernel, dim3((a.N + 7) / 8, static_cast<unsigned>(units)), dim3(256), 0, s, true, a));
+    return LSG_OK;
+}
+
+}  // namespace lsg
+
+using namespace lsg;
+
+namespace {
+size_t a256(size_t v) { return (v + 255) & ~size_t(255); }
+long long pad16(long long v) { return (v + 15) & ~15ll; }
+}  // namespace
+
+extern "C" int lsg_int8_gemm(const lsg_int8_gemm_params* p, void* stream) {
+    if (!p) return fail(LSG_ERR_INVALID, "int8_gemm: null params");
+    if (p->M < 0 || p->N < 0) return fail(LSG_ERR_INVALID, "int8_gemm: negative shape");
+    if (p->M == 0 || p->N == 0) return LSG_OK;
+    const int rc = check("int8_gemm", p->N, p->K, p->A, p->lda, p->B, p->ldb, p->D, p->output_dtype);
+    if (rc != LSG_OK) return rc;
+    if (!p->scale_A || !p->scale_B) return fail(LSG_ERR_INVALID, "int8_gemm: null pointer");
+    Int8Gemm a = {};
+    a.A = static_cast<const int8_t*>(p->A); a.lda = p->lda;
+    a.B = static_cast<const int8_t*>(p->B); a.ldb = p->ldb;
+    a.D = p->D; a.out_dtype = p->output_dtype;
+    a.scale_A = p->scale_A; a.scale_B = p->scale_B;
+    a.M = p->M; a.N = p->N; a.K = p->K; a.E = 1;
+    return int8_gemm(a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t lsg_int8_gemm_from_bf16_workspace_bytes(int M, int K) {
+    if (M <= 0 || K <= 0) return 0;
+    return a256(static_cast<size_t>(M) * pad16(K)) + a256(static_cast<size_t>(M) * 4);
+}
+
+extern "C" int lsg_int8_gemm_from_bf16(const lsg_int8_gemm_params* p, int input_dtype, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+    if (!p) return fail(LSG_ERR_INVALID, "int8_gemm_from_bf16: null params");
+    if (p->M < 0 || p->N < 0) return fail(LSG_ERR_INVALID, "int8_gemm_from_bf16: negative shape");
+    if (input_dtype != LSG_DTYPE_BF16 && input_dtype != LSG_DTYPE_F16)
+        return fail(LSG_ERR_UNSUPPORTED, "int8_gemm_from_bf16: input must be bf16 or fp16");
+    if (p->M == 0 || p->N == 0) return LSG_OK;
+    // the activations may lie anywhere: their codes, in the workspace, are what the product reads
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    const long long ldq = pad16(p->K);
+    const size_t need = lsg_int8_gemm_from_bf16_workspace_bytes(p->M, p->K);
+    if (p->K >= 1 && (!workspace || workspace_bytes < need))
+        return fail(LSG_ERR_WORKSPACE, "int8_gemm_from_bf16: workspace too small (have %zu, need %zu)",
+                    workspace ? workspace_bytes : size_t(0), need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255)
+        return fail(LSG_ERR_ALIGNMENT, "int8_gemm_from_bf16: workspace must be 256-byte aligned");
+    int rc = check("int8_gemm_from_bf16", p->N, p->K, codes, ldq, p->B, p->ldb, p->D, p->output_dtype);
+    if (rc != LSG_OK) return rc;
+    if (!p->A || !p->scale_B) return fail(LSG_ERR_INVALID, "int8_gemm_from_bf16: null pointer");
+    if (p->lda < p->K) return fail(LSG_ERR_INVALID, "int8_gemm_from_bf16: a row stride is smaller than K");
+    float* scales = reinterpret_cast<float*>(codes + a256(static_cast<size_t>(p->M) * ldq));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Int8Gemm a = {};
+    a.A = reinterpret_cast<const int8_t*>(codes); a.lda = ldq;
+    a.B = static_cast<const int8_t*>(p->B); a.ldb = p->ldb;
+    a.D = p->D; a.out_dtype = p->output_dtype;
+    a.scale_A = scales; a.scale_B = p->scale_B;
+    a.M = p->M; a.N = p->N; a.K = p->K; a.E = 1;
+    rc = int8_quant_rows(p->A, p->lda, input_dtype, reinterpret_cast<int8_t*>(codes), ldq, scales, p->M, p->K, nullptr, 1, 0, s);
+    if (rc != LSG_OK) return rc;
+    return int8_gemm(a, s);
+}
+
+extern "C" int lsg_int8_grouped_gemm(const lsg_int8_grouped_gemm_params* p, int total_tokens, void* stream) {
+    if (!p) return fail(LSG_ERR_INVALID, "int8_grouped_gemm: null params");
+    if (p->num_experts < 0 || total_tokens < 0 || p->N < 0) return fail(LSG_ERR_INVALID, "int8_grouped_gemm: negative shape");
+    if (p->num_experts > 1024) return fail(LSG_ERR_INVALID, "int8_grouped_gemm: at most 1024 experts (E=%d)", p->num_experts);
+    if (p->num_experts == 0 || total_tokens == 0 || p->N == 0) return LSG_OK;
+    const int rc = check("int8_grouped_gemm", p->N, p->K, p->A_base, p->lda, p->B_base, p->ldb, p->D_base, p->output_dtype);
+    if (rc != LSG_OK) return rc;
+    if (!p->scale_A_base || !p->scale_B_base || !p->expert_offsets)
+        return fail(LSG_ERR_INVALID, "int8_grouped_gemm: null pointer");
+    if (static_cast<long long>(p->num_experts) * p->N > 0x7fffffffll)
+        return fail(LSG_ERR_INVALID, "int8_grouped_gemm: more than 2^31 - 1 weight rows");
+    Int8Gemm a = {};
+    a.A = static_cast<const int8_t*>(p->A_base); a.lda = p->lda;
+    a.B = static_cast<const int8_t*>(p->B_base); a.ldb = p->ldb;
+    a.D = p->D_base; a.out_dtype = p->output_dtype;
+    a.scale_A = p->scale_A_base; a.scale_B = p->scale_B_base;
+    a.M = total_tokens; a.N = p->N; a.K = p->K; a.E = p->num_experts;
+    a.expert_offsets = p->expert_offsets;
+    return int8_gemm(a, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+struct FfnPlan {
+    size_t codes, scales, gate_up, act, act_scales, total;
+    long long ldh, ldi;
+};
+FfnPlan ffn_plan(long long rows, int H, int I) {
+    FfnPlan f;
+    f.ldh = pad16(H);
+    f.ldi = pad16(I);
+    f.codes = 0;
+    f.scales = f.codes + a256(static_cast<size_t>(rows) * f.ldh);
+    f.gate_up = f.scales + a256(static_cast<size_t>(rows) * 4);
+    f.act = f.gate_up + a256(static_cast<size_t>(rows) * 2 * I * 4);
+    f.act_scales = f.act + a256(static_cast<size_t>(rows) * f.ldi);
+    f.total = f.act_scales + a256(static_cast<size_t>(rows) * 4);
+    return f;
+}
+}  // namespace
+
+extern "C" size_t lsg_int8_moe_ffn_workspace_bytes(int num_tokens, int top_k, int H, int I) {
+    if (num_tokens <= 0 || top_k <= 0 || H <= 0 || I <= 0) return 0;
+    return ffn_plan(static_cast<long long>(num_tokens) * top_k, H, I).total;
+}
+
+extern "C" int lsg_int8_moe_ffn(const lsg_int8_moe_ffn_params* p, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!p) return fail(LSG_ERR_INVALID, "int8_moe_ffn: null params");
+    if (p->num_tokens < 0 || p->num_experts < 0 || p->H < 0 || p->I < 0) return fail(LSG_ERR_INVALID, "int8_moe_ffn: negative shape");
+    if (p->num_experts > 1024) return fail(LSG_ERR_INVALID, "int8_moe_ffn: at most 1024 experts (E=%d)", p->num_experts);
+    if (p->top_k < 1 || static_cast<long long>(p->num_tokens) * p->top_k > 0x7fffffffll)
+        return fail(LSG_ERR_INVALID, "int8_moe_ffn: need top_k >= 1 and at most 2^31 - 1 pairs");
+    if (p->input_dtype != LSG_DTYPE_BF16 && p->input_dtype != LSG_DTYPE_F16)
+        return fail(LSG_ERR_UNSUPPORTED, "int8_moe_ffn: hidden must be bf16 or fp16");
+    if (p->num_tokens == 0 || p->num_experts == 0) return LSG_OK;
+    if (p->H < 1 || p->I < 1 || p->H % 16 != 0 || p->I % 16 != 0 || p->H > kInt8MaxK || p->I > kInt8MaxK)
+        return fail(LSG_ERR_INVALID, "int8_moe_ffn: H and I must be positive multiples of 16 up to %d (H=%d, I=%d)", kInt8MaxK, p->H, p->I);
+    if (static_cast<long long>(p->num_experts) * 2 * p->I > 0x7fffffffll || static_cast<long long>(p->num_experts) * p->H > 0x7fffffffll)
+        return fail(LSG_ERR_INVALID, "int8_moe_ffn: more than 2^31 - 1 weight rows");
+    if (!p->hidden || !p->inv_perm || !p->expert_offsets || !p->gate_up_scales || !p->down_scales)
+        return fail(LSG_ERR_INVALID, "int8_moe_ffn: null pointer");
+    if (p->ld_hidden < p->H) return fail(LSG_ERR_INVALID, "int8_moe_ffn: a row stride is smaller than the row");
+    const int rows = p->num_tokens * p->top_k, H = p->H, I = p->I;
+    const FfnPlan f = ffn_plan(rows, H, I);
+    if (!workspace || workspace_bytes < f.total)
+        return fail(LSG_ERR_WORKSPACE, "int8_moe_ffn: workspace too small (have %zu, need %zu)",
+                    workspace ? workspace_bytes : size_t(0), f.total);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255)
+        return fail(LSG_ERR_ALIGNMENT, "int8_moe_ffn: workspace must be 256-byte aligned");
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    int rc = check("int8_moe_ffn", 2 * I, H, ws, f.ldh, p->gate_up, H, ws, LSG_DTYPE_F32);
+    if (rc == LSG_OK) rc = check("int8_moe_ffn", H, I, ws, f.ldi, p->down, I, p->D, p->output_dtype);
+    if (rc != LSG_OK) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int8_t* codes = reinterpret_cast<int8_t*>(ws + f.codes);
+    float* scales = reinterpret_cast<float*>(ws + f.scales);
+    float* gu = reinterpret_cast<float*>(ws + f.gate_up);
+    int8_t* act = reinterpret_cast<int8_t*>(ws + f.act);
+    float* act_scales = reinterpret_cast<float*>(ws + f.act_scales);
+    rc = int8_quant_rows(p->hidden, p->ld_hidden, p->input_dtype, codes, f.ldh, scales, p->num_tokens, H, p->inv_perm, p->top_k, rows, s);
+    if (rc != LSG_OK) return rc;
+    Int8Gemm a = {};
+    a.A = codes; a.lda = f.ldh; a.B = static_cast<const int8_t*>(p->gate_up); a.ldb = H;
+    a.D = gu; a.out_dtype = LSG_DTYPE_F32; a.scale_A = scales; a.scale_B = p->gate_up_scales;
+    a.M = rows; a.N = 2 * I; a.K = H; a.E = p->num_experts; a.expert_offsets = p->expert_offsets;
+    rc = int8_gemm(a, s);
+    if (rc != LSG_OK) return rc;
+    rc = int8_quant_silu_mul(gu, 2ll * I, gu + I, 2ll * I, LSG_DTYPE_F32, act, f.ldi, act_scales, rows, I, s);
+    if (rc != LSG_OK) return rc;
+    a.A = act; a.lda = f.ldi; a.B = static_cast<const int8_t*>(p->down); a.ldb = I;
+    a.D = p->D; a.out_dtype = p->output_dtype; a.scale_A = act_scales; a.scale_B = p->down_scales;
+    a.N = H; a.K = I;
+    return int8_gemm(a, s);
+}

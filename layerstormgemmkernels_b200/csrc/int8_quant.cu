@@ -1,0 +1,320 @@
+// Quantizers of the 8-bit integer family: one scale per row (per token of an activation, per output
+// channel of a weight).
+//
+//   a = max_k |x[k]|      scale = fl(a / 127)      q[k] = rne(127 x[k] / a)
+//
+// An all-zero row gets scale 0 and codes 0; a row with an infinity or a NaN gets scale NaN and
+// codes 0, so that whatever it is multiplied with is NaN and not a number that looks right.
+//
+// The code is the rounding of the exact quotient for bf16 and fp16 inputs: 127 x has at most 18
+// bits and is exact in fp32, fma(fma(-t, a, y), 1/a, t) is the correctly rounded quotient y / a,
+// and a quotient of two 11-bit numbers that is not half-way between two integers is at least 2^-20
+// (relative to the larger of the integers' spacing and itself, 2^-12 at 127) away from half-way,
+// more than fp32 moves it.  fl(x / scale) would not do: the scale is rounded, so quotients next to
+// a half-way point fall on either side of it.
+//
+// The activation silu(g) * u of silu_mul stays in fp32 up to its code (rounding it to bf16 first
+// moves one value in fifteen by a code).
+//
+// Memory bound: one CTA per row, the row held in registers between the maximum and the codes, so
+// that every input byte is read once.  Rows that are not whole 16-byte pieces, or longer than
+// 16384 values, are read twice, value by value.
+#include "common.cuh"
+#include "host.h"
+
+namespace lsg {
+
+namespace {
+
+constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer, in the low byte
+
+struct RowQuantArgs {
+    const void* x;        // [rows, K], row stride ldx values (gate of silu_mul)
+    const void* up;
+    long long ldx, ldu;
+    int8_t* codes;        // row stride ldq bytes
+    long long ldq;
+    float* scales;
+    int K;
+    const int32_t* inv;   // scatter: [rows * top_k] destination rows; null = row to row
+    int top_k;
+    int out_rows;
+};
+
+template <typename T> struct Elem;
+template <> struct Elem<__nv_bfloat16> {
+    static constexpr int kVecs = 1;   // 16-byte loads for eight values
+    static __device__ __forceinline__ float get(const void* p, size_t i) {
+        return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+    }
+    static __device__ __forceinline__ void unpack(const uint4* v, float (&f)[8]) {
+        const uint32_t w[4] = {v->x, v->y, v->z, v->w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+template <> struct Elem<__half> {
+    static constexpr int kVecs = 1;
+    static __device__ __forceinline__ float get(const void* p, size_t i) {
+        return __half2float(static_cast<const __half*>(p)[i]);
+    }
+    static __device__ __forceinline__ void unpack(const uint4* v, float (&f)[8]) {
+        const uint32_t w[4] = {v->x, v->y, v->z, v->w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = h.x;
+            f[2 * i + 1] = h.y;
+        }
+    }
+};
+template <> struct Elem<float> {
+    static constexpr int kVecs = 2;
+    static __device__ __forceinline__ float get(const void* p, size_t i) { return static_cast<const float*>(p)[i]; }
+    static __device__ __forceinline__ void unpack(const uint4* v, float (&f)[8]) {
+        const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+    }
+};
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// Bits of the largest magnitude of the CTA's values; magnitudes order like their bit patterns, with
+// infinity and NaN on top, so nothing that is not finite is lost.
+__device__ __forceinline__ uint32_t block_max_bits(uint32_t m) {
+    __shared__ uint32_t part[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (blockDim.x + 31) >> 5;
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (n == 1) return m;
+    if (lane == 0) part[warp] = m;
+    __syncthreads();
+    return __reduce_max_sync(0xffffffffu, lane < n ? part[lane] : 0u);
+}
+
+// The row's constants: y = x * mul is 127 x, moved by a power of two where 127 a or 1 / a would leave
+// the range of fp32; den = a moved alike.
+struct RowScale {
+    float scale, mul, den, rcp;
+    bool dead;   // all zero, or not finite: codes are 0
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
+    RowScale r;
+    const float a = __uint_as_float(amax_bits);
+    const bool finite = amax_bits < 0x7F800000u;
+    r.dead = !finite || amax_bits == 0;
+    r.scale = finite ? a / 127.0f : __uint_as_float(0x7FC00000u);
+    const float s = a > 0x1p100f ? 0x1p-64f : (a < 0x1p-100f ? 0x1p64f : 1.0f);
+    r.mul = 127.0f * s;
+    r.den = a * s;
+    r.rcp = r.dead ? 0.0f : 1.0f / r.den;
+    return r;
+}
+__device__ __forceinline__ uint32_t code_bits(float x, const RowScale& r) {
+    const float y = x * r.mul;
+    const float t = y * r.rcp;
+    return __float_as_uint(fmaf(fmaf(-t, r.den, y), r.rcp, t) + kMagic);
+}
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// V pieces of eight values per thread.
+template <typename T, bool SILU, int V>
+__global__ void __launch_bounds__(V == 4 ? 512 : 1024)
+quant_rows_kernel(const RowQuantArgs a) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    constexpr int L = Elem<T>::kVecs;
+    const long long row = blockIdx.x;
+    const int nvec = a.K >> 3;
+    const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ldx);
+    const uint4* up = SILU ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.up) + row * a.ldu) : nullptr;
+    uint4 raw[V][L];
+    float h[SILU ? V : 1][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int v = threadIdx.x + i * blockDim.x;
+#pragma unroll
+        for (int l = 0; l < L; ++l) raw[i][l] = v < nvec ? __ldg(x + v * L + l) : make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (SILU) {
+        uint4 ur[V][L];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int v = threadIdx.x + i * blockDim.x;
+#pragma unroll
+            for (int l = 0; l < L; ++l) ur[i][l] = v < nvec ? __ldg(up + v * L + l) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float g[8], u[8];
+            Elem<T>::unpack(raw[i], g);
+            Elem<T>::unpack(ur[i], u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                h[i][j] = silu_mul(g[j], u[j]);
+                m = max(m, __float_as_uint(fabsf(h[i][j])));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float f[8];
+            Elem<T>::unpack(raw[i], f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(f[j])));
+        }
+    }
+    const RowScale r = row_scale(block_max_bits(m));
+    uint2 out[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float f[8];
+        if constexpr (SILU) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = h[i][j];
+        } else {
+            Elem<T>::unpack(raw[i], f);
+        }
+        uint32_t q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = code_bits(f[j], r);
+        out[i] = r.dead ? make_uint2(0, 0) : make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+    }
+    const int copies = a.inv ? a.top_k : 1;
+    for (int s = 0; s < copies; ++s) {
+        const long long dst = a.inv ? __ldg(a.inv + row * a.top_k + s) : row;
+        if (a.inv && (dst < 0 || dst >= a.out_rows)) continue;
+        uint2* q = reinterpret_cast<uint2*>(a.codes + dst * a.ldq);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int v = threadIdx.x + i * blockDim.x;
+            if (v < nvec) q[v] = out[i];
+        }
+        if (threadIdx.x == 0) a.scales[dst] = r.scale;
+    }
+}
+
+template <typename T, bool SILU>
+__global__ void __launch_bounds__(256)
+quant_rows_any_kernel(const RowQuantArgs a) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    const long long row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* up = SILU ? static_cast<const T*>(a.up) + row * a.ldu : nullptr;
+    auto value = [&](int k) {
+        const float g = Elem<T>::get(x, k);
+        return SILU ? silu_mul(g, Elem<T>::get(up, k)) : g;
+    };
+    uint32_t m = 0;
+    for (int k = threadIdx.x; k < a.K; k += 256) m = max(m, __float_as_uint(fabsf(value(k))));
+    const RowScale r = row_scale(block_max_bits(m));
+    const int copies = a.inv ? a.top_k : 1;
+    for (int k = threadIdx.x; k < a.K; k += 256) {
+        const int8_t q = r.dead ? int8_t(0) : static_cast<int8_t>(code_bits(value(k), r) & 0xFFu);
+        for (int s = 0; s < copies; ++s) {
+            const long long dst = a.inv ? __ldg(a.inv + row * a.top_k + s) : row;
+            if (a.inv && (dst < 0 || dst >= a.out_rows)) continue;
+            a.codes[dst * a.ldq + k] = q;
+        }
+    }
+    if (threadIdx.x == 0)
+        for (int s = 0; s < copies; ++s) {
+            const long long dst = a.inv ? __ldg(a.inv + row * a.top_k + s) : row;
+            if (a.inv && (dst < 0 || dst >= a.out_rows)) continue;
+            a.scales[dst] = r.scale;
+        }
+}
+
+template <typename T, bool SILU>
+int launch_rows(const RowQuantArgs& a, long long rows, cudaStream_t s) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.x) | (SILU ? reinterpret_cast<uintptr_t>(a.up) : 0) |
+                         static_cast<uintptr_t>(a.ldx * static_cast<long long>(sizeof(T))) |
+                         (SILU ? static_cast<uintptr_t>(a.ldu * static_cast<long long>(sizeof(T))) : 0);
+    const int nvec = a.K / 8;
+    const dim3 grid(static_cast<unsigned>(rows));
+    if ((at & 15) != 0 || a.K % 8 != 0 || nvec == 0 || nvec > 2048) {
+        LSG_CUDA_TRY(launch_kernel(quant_rows_any_kernel<T, SILU>, grid, dim3(256), 0, s, true, a));
+        return LSG_OK;
+    }
+    const int v = nvec <= 256 ? 1 : (nvec <= 1024 ? 2 : 4);
+    const dim3 block(static_cast<unsigned>(((nvec + v - 1) / v + 31) / 32 * 32));
+    if (v == 1) LSG_CUDA_TRY(launch_kernel(quant_rows_kernel<T, SILU, 1>, grid, block, 0, s, true, a));
+    else if (v == 2) LSG_CUDA_TRY(launch_kernel(quant_rows_kernel<T, SILU, 2>, grid, block, 0, s, true, a));
+    else LSG_CUDA_TRY(launch_kernel(quant_rows_kernel<T, SILU, 4>, grid, block, 0, s, true, a));
+    return LSG_OK;
+}
+
+// Shape and pointer checks shared by the entries; `ld` in values, ldq in bytes.
+int check_rows(const char* op, int dtype, bool f32_ok, long long rows, int K, long long ld, const void* codes,
+               long long ldq) {
+    if (dtype != LSG_DTYPE_BF16 && dtype != LSG_DTYPE_F16 && !(f32_ok && dtype == LSG_DTYPE_F32))
+        return fail(LSG_ERR_UNSUPPORTED, "%s: input must be bf16 or fp16%s", op, f32_ok ? " or f32" : "");
+    if (rows < 0 || K < 0) return fail(LSG_ERR_INVALID, "%s: negative shape", op);
+    if (rows > 0x7fffffffll) return fail(LSG_ERR_INVALID, "%s: more than 2^31 - 1 rows", op);
+    if (ld < K || ldq < K) return fail(LSG_ERR_INVALID, "%s: a row stride is smaller than the row", op);
+    if (ldq % 16 != 0 || (reinterpret_cast<uintptr_t>(codes) & 15))
+        return fail(LSG_ERR_ALIGNMENT, "%s: code rows must start on 16-byte boundaries", op);
+    return LSG_OK;
+}
+
+}  // namespace
+
+int int8_quant_rows(const void* x, long long ldx, int dtype, int8_t* codes, long long ldq, float* scales, long long rows,
+                    int K, const int32_t* inv, int top_k, int out_rows, cudaStream_t s) {
+    RowQuantArgs a = {};
+    a.x = x; a.ldx = ldx; a.codes = codes; a.ldq = ldq; a.scales = scales; a.K = K;
+    a.inv = inv; a.top_k = top_k; a.out_rows = out_rows;
+    return dtype == LSG_DTYPE_F16 ? launch_rows<__half, false>(a, rows, s) : launch_rows<__nv_bfloat16, false>(a, rows, s);
+}
+
+int int8_quant_silu_mul(const void* gate, long long ldg, const void* up, long long ldu, int dtype, int8_t* codes,
+                        long long ldq, float* scales, long long rows, int K, cudaStream_t s) {
+    RowQuantArgs a = {};
+    a.x = gate; a.ldx = ldg; a.up = up; a.ldu = ldu; a.codes = codes; a.ldq = ldq; a.scales = scales; a.K = K;
+    if (dtype == LSG_DTYPE_F32) return launch_rows<float, true>(a, rows, s);
+    return dtype == LSG_DTYPE_F16 ? launch_rows<__half, true>(a, rows, s) : launch_rows<__nv_bfloat16, true>(a, rows, s);
+}
+
+}  // namespace lsg
+
+using namespace lsg;
+
+extern "C" int lsg_dynamic_int8_quant(const void* x, long long ldx, int dtype, void* codes, long long ldq, float* scales,
+                                      long long rows, int K, void* stream) {
+    const int rc = check_rows("dynamic_int8_quant", dtype, false, rows, K, ldx, codes, ldq);
+    if (rc != LSG_OK) return rc;
+    if (rows == 0) return LSG_OK;
+    if (!scales || (K > 0 && (!x || !codes))) return fail(LSG_ERR_INVALID, "dynamic_int8_quant: null pointer");
+    return int8_quant_rows(x, ldx, dtype, static_cast<int8_t*>(codes), ldq, scales, rows, K, nullptr, 1, 0,
+                           static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lsg_silu_mul_int8_quant(const void* gate, long long ldg, const void* up, long long ldu, int dtype,
+                                       void* codes, long long ldq, float* scales, long long rows, int K, void* stream) {
+    int rc = check_rows("silu_mul_int8_quant", dtype, true, rows, K, ldg < ldu ? ldg : ldu, codes, ldq);
+    if (rc != LSG_OK) return rc;
+    if (rows == 0) return LSG_OK;
+    if (!scales || (K > 0 && (!gate || !up || !codes))) return fail(LSG_ERR_INVALID, "silu_mul_int8_quant: null pointer");
+    return int8_quant_silu_mul(gate, ldg, up, ldu, dtype, static_cast<int8_t*>(codes), ldq, scales, rows, K,
+                               static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lsg_moe_permute_int8(const void* hidden, long long ld, int dtype, const int32_t* inv_perm, int num_tokens,
+                                    int top_k, int H, void* codes, long long ldq, float* scales, void* stream) {
+    int rc = check_rows("moe_permute_int8", dtype, false, num_tokens, H, ld, codes, ldq);
+    if (rc != LSG_OK) return rc;
+    if (top_k < 1 || static_cast<long long>(num_tokens) * top_k > 0x7fffffffll)
+        return fail(LSG_ERR_INVALID, "moe_permute_int8: need top_k >= 1 and at most 2^31 - 1 pairs");
+    if (num_tokens == 0) return LSG_OK;
+    if (!scales || !inv_perm || (H > 0 && (!hidden || !codes)))
+        return fail(LSG_ERR_INVALID, "moe_permute_int8: null pointer");
+    return int8_quant_rows(hidden, ld, dtype, static_cast<int8_t*>(codes), ldq, scales, num_tokens, H, inv_perm, top_k,
+                           num_tokens * top_k, static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,298 @@
+// The way of a token to its experts and back in fp16, bf16 and fp32, and its gradients.  With
+// inv[t, s] the row of pair (token t, slot s), w the routing weights and L the loss:
+//
+//   permute     x_e[inv[t,s]] = x[t]                    dL/dx[t]          = sum_s dL/dx_e[inv[t,s]]
+//   unpermute   out[t] = sum_s w[t,s] y[inv[t,s]]       dL/dy[inv[t,s]]   = w[t,s] dL/dout[t]
+//                                                       dL/dw[t,s]        = < y[inv[t,s]], dL/dout[t] >
+//   route       w[t,:] = softmax of the k chosen        dL/dl[t,idx[t,s]] = w[t,s] (dL/dw[t,s] - sum_r w[t,r] dL/dw[t,r])
+//               logits (renormalising the top k of a                         0 for the experts not chosen
+//               softmax leaves just that)
+//
+// A pair whose entry of inv lies outside [0, rows) has no row: it adds nothing, and its weight's
+// gradient is 0.  Every sum is taken in fp32 in the order of the slots or by one CTA in a fixed
+// order, without atomics: the same inputs give the same bits.
+#include "common.cuh"
+#include "host.h"
+
+namespace lsg {
+
+namespace {
+
+constexpr int kMaxSlots = 16;
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f(float v) { return v; }
+template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+
+// P values as one load or store: 16 bytes, or a single value where rows are not whole pieces.
+template <typename T, int P> struct alignas(sizeof(T) * P) Piece { T v[P]; };
+
+// out[t] = sum over slots, in order, of (w ? w[t,s] : 1) * y[inv[t,s]].
+template <typename T, int P>
+__global__ void __launch_bounds__(256)
+moe_sum_slots_kernel(const Piece<T, P>* __restrict__ y, const int32_t* __restrict__ inv, const float* __restrict__ w,
+                     int rows, int k, int per_row, Piece<T, P>* __restrict__ out) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    const size_t t = blockIdx.x;
+    for (int c = threadIdx.x; c < per_row; c += blockDim.x) {
+        float acc[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) acc[i] = 0.0f;
+        for (int s = 0; s < k; ++s) {
+            const int row = __ldg(inv + t * k + s);
+            if (row < 0 || row >= rows) continue;
+            const float ws = w ? __ldg(w + t * k + s) : 1.0f;
+            const Piece<T, P> p = y[static_cast<size_t>(row) * per_row + c];
+#pragma unroll
+            for (int i = 0; i < P; ++i) acc[i] = fmaf(ws, to_f(p.v[i]), acc[i]);
+        }
+        Piece<T, P> o;
+#pragma unroll
+        for (int i = 0; i < P; ++i) o.v[i] = from_f<T>(acc[i]);
+        out[t * per_row + c] = o;
+    }
+}
+
+// out[row] = x[perm[row] / k]
+template <typename T, int P>
+__global__ void __launch_bounds__(256)
+moe_copy_rows_kernel(const Piece<T, P>* __restrict__ x, const int32_t* __restrict__ perm, int tokens, int k, int per_row,
+                     Piece<T, P>* __restrict__ out) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    const size_t row = blockIdx.x;
+    const int pair = __ldg(perm + row);
+    if (pair < 0 || pair / k >= tokens) return;
+    const size_t src = static_cast<size_t>(pair / k) * per_row;
+    for (int c = threadIdx.x; c < per_row; c += blockDim.x) out[row * per_row + c] = x[src + c];
+}
+
+// One CTA per token: grad_out[t] is read once for all its slots.
+template <typename T, int P>
+__global__ void __launch_bounds__(256)
+moe_unpermute_backward_kernel(const Piece<T, P>* __restrict__ grad_out, const Piece<T, P>* __restrict__ y,
+                              const int32_t* __restrict__ inv, const float* __restrict__ w,
+                              const int32_t* __restrict__ rows_used, int rows, int k, int per_row,
+                              Piece<T, P>* __restrict__ grad_y, float* __restrict__ grad_w) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    __shared__ float part[8][kMaxSlots];
+    const size_t t = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float dot[kMaxSlots];
+#pragma unroll
+    for (int s = 0; s < kMaxSlots; ++s) dot[s] = 0.0f;
+    for (int c = threadIdx.x; c < per_row; c += blockDim.x) {
+        const Piece<T, P> g = grad_out[t * per_row + c];
+#pragma unroll
+        for (int s = 0; s < kMaxSlots; ++s) {
+            if (s < k) {
+                const int row = __ldg(inv + t * k + s);
+                if (row >= 0 && row < rows) {
+                    const float ws = __ldg(w + t * k + s);
+                    const size_t at = static_cast<size_t>(row) * per_row + c;
+                    const Piece<T, P> v = y[at];
+                    Piece<T, P> o;
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        const float gf = to_f(g.v[i]);
+                        dot[s] = fmaf(to_f(v.v[i]), gf, dot[s]);
+                        o.v[i] = from_f<T>(ws * gf);
+                    }
+                    grad_y[at] = o;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < kMaxSlots; ++s) {
+        if (s < k) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) dot[s] += __shfl_xor_sync(0xffffffffu, dot[s], o);
+            if (lane == 0) part[warp][s] = dot[s];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < k) {
+        float v = 0.0f;
+        for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) v += part[i][threadIdx.x];
+        grad_w[t * k + threadIdx.x] = v;
+    }
+    // rows behind the last expert's belong to no pair
+    if (rows_used) {
+        const int used = __ldg(rows_used);
+        for (int s = 0; s < k; ++s) {
+            const size_t row = t * k + s;
+            if (row >= static_cast<size_t>(max(used, 0)) && row < static_cast<size_t>(rows)) {
+                Piece<T, P> z;
+#pragma unroll
+                for (int i = 0; i < P; ++i) z.v[i] = from_f<T>(0.0f);
+                for (int c = threadIdx.x; c < per_row; c += blockDim.x) grad_y[row * per_row + c] = z;
+            }
+        }
+    }
+}
+
+// One warp per token.  The chosen experts' gradients are formed by lanes 0..k-1; every lane then
+// writes the experts lane, lane + 32, ..., summing the slots that name the expert (routing names an
+// expert once; a caller's own indices may name it twice).
+__global__ void __launch_bounds__(256)
+moe_route_backward_kernel(const int32_t* __restrict__ idx, const float* __restrict__ w, const float* __restrict__ grad_w,
+                          int T, int E, int k, float* __restrict__ grad_logits) {
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    const int lane = threadIdx.x & 31;
+    const long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (t >= T) return;
+    const float wl = lane < k ? w[t * k + lane] : 0.0f;
+    const float gl = lane < k ? grad_w[t * k + lane] : 0.0f;
+    const int el = lane < k ? idx[t * k + lane] : -1;
+    float dot = wl * gl;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    const float d = wl * (gl - dot);
+    for (int e = lane; e < ((E + 31) & ~31); e += 32) {
+        float v = 0.0f;
+        for (int s = 0; s < k; ++s) {
+            const int es = __shfl_sync(0xffffffffu, el, s);
+            const float ds = __shfl_sync(0xffffffffu, d, s);
+            if (es == e) v += ds;
+        }
+        if (e < E) grad_logits[t * E + e] = v;
+    }
+}
+
+int threads_for(int per_row) { return per_row >= 256 ? 256 : (per_row < 1 ? 32 : (per_row + 31) / 32 * 32); }
+
+bool whole_pieces(int H, size_t size, uintptr_t at) { return (static_cast<size_t>(H) * size) % 16 == 0 && (at & 15) == 0; }
+
+template <typename T>
+int sum_slots(const void* y, const int32_t* inv, const float* w, int rows, int tokens, int k, int H, void* out,
+              cudaStream_t s) {
+    constexpr int P = 16 / sizeof(T);
+    const dim3 grid(static_cast<unsigned>(tokens));
+    if (whole_pieces(H, sizeof(T), reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)))
+        LSG_CUDA_TRY(launch_kernel(moe_sum_slots_kernel<T, P>, grid, dim3(threads_for(H / P)), 0, s, true,
+                                   static_cast<const Piece<T, P>*>(y), inv, w, rows, k, H / P, static_cast<Piece<T, P>*>(out)));
+    else
+        LSG_CUDA_TRY(launch_kernel(moe_sum_slots_kernel<T, 1>, grid, dim3(threads_for(H)), 0, s, true,
+                                   static_cast<const Piece<T, 1>*>(y), inv, w, rows, k, H, static_cast<Piece<T, 1>*>(out)));
+    return LSG_OK;
+}
+
+template <typename T>
+int copy_rows(const void* x, const int32_t* perm, int rows, int tokens, int k, int H, void* out, cudaStream_t s) {
+    constexpr int P = 16 / sizeof(T);
+    const dim3 grid(static_cast<unsigned>(rows));
+    if (whole_pieces(H, sizeof(T), reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)))
+        LSG_CUDA_TRY(launch_kernel(moe_copy_rows_kernel<T, P>, grid, dim3(threads_for(H / P)), 0, s, true,
+                                   static_cast<const Piece<T, P>*>(x), perm, tokens, k, H / P, static_cast<Piece<T, P>*>(out)));
+    else
+        LSG_CUDA_TRY(launch_kernel(moe_copy_rows_kernel<T, 1>, grid, dim3(threads_for(H)), 0, s, true,
+                                   static_cast<const Piece<T, 1>*>(x), perm, tokens, k, H, static_cast<Piece<T, 1>*>(out)));
+    return LSG_OK;
+}
+
+template <typename T>
+int unpermute_backward(const void* grad_out, const void* y, const int32_t* inv, const float* w, const int32_t* used, int rows,
+                       int tokens, int k, int H, void* grad_y, float* grad_w, cudaStream_t s) {
+    constexpr int P = 16 / sizeof(T);
+    const dim3 grid(static_cast<unsigned>(tokens));
+    if (whole_pieces(H, sizeof(T), reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(grad_y)))
+        LSG_CUDA_TRY(launch_kernel(moe_unpermute_backward_kernel<T, P>, grid, dim3(threads_for(H / P)), 0, s, true,
+                                   static_cast<const Piece<T, P>*>(grad_out), static_cast<const Piece<T, P>*>(y), inv, w, used,
+                                   rows, k, H / P, static_cast<Piece<T, P>*>(grad_y), grad_w));
+    else
+        LSG_CUDA_TRY(launch_kernel(moe_unpermute_backward_kernel<T, 1>, grid, dim3(threads_for(H)), 0, s, true,
+                                   static_cast<const Piece<T, 1>*>(grad_out), static_cast<const Piece<T, 1>*>(y), inv, w, used,
+                                   rows, k, H, static_cast<Piece<T, 1>*>(grad_y), grad_w));
+    return LSG_OK;
+}
+
+int check_moe(const char* op, int dtype, int tokens, int k, int H) {
+    if (dtype != LSG_DTYPE_BF16 && dtype != LSG_DTYPE_F16 && dtype != LSG_DTYPE_F32)
+        return fail(LSG_ERR_UNSUPPORTED, "%s: dtype must be bf16, fp16 or f32", op);
+    if (tokens < 0 || H < 0) return fail(LSG_ERR_INVALID, "%s: negative shape", op);
+    if (k < 1 || k > kMaxSlots) return fail(LSG_ERR_INVALID, "%s: need 1 <= top_k <= %d (k=%d)", op, kMaxSlots, k);
+    if (static_cast<long long>(tokens) * k > 0x7fffffffll)
+        return fail(LSG_ERR_INVALID, "%s: more than 2^31 - 1 pairs", op);
+    return LSG_OK;
+}
+
+}  // namespace
+
+}  // namespace lsg
+
+using namespace lsg;
+
+#define LSG_BY_DTYPE(call)                                        \
+    (dtype == LSG_DTYPE_F32 ? call<float> : dtype == LSG_DTYPE_F16 ? call<__half> : call<__nv_bfloat16>)
+
+extern "C" int lsg_moe_permute_dtype(const void* hidden, int dtype, const int32_t* perm, int rows, int num_tokens,
+                                     int top_k, int H, void* out, void* stream) {
+    const int rc = check_moe("moe_permute", dtype, num_tokens, top_k, H);
+    if (rc != LSG_OK) return rc;
+    if (rows <= 0 || H == 0) return rows < 0 ? fail(LSG_ERR_INVALID, "moe_permute: negative shape") : LSG_OK;
+    if (!hidden || !perm || !out) return fail(LSG_ERR_INVALID, "moe_permute: null pointer");
+    return LSG_BY_DTYPE(copy_rows)(hidden, perm, rows, num_tokens, top_k, H, out, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lsg_moe_unpermute_dtype(const void* y, int dtype, const int32_t* inv_perm, const float* topk_weights, int rows,
+                                       int num_tokens, int top_k, int H, void* out, void* stream) {
+    const int rc = check_moe("moe_unpermute", dtype, num_tokens, top_k, H);
+    if (rc != LSG_OK) return rc;
+    if (rows < 0) return fail(LSG_ERR_INVALID, "moe_unpermute: negative shape");
+    if (num_tokens == 0 || H == 0) return LSG_OK;
+    if ((rows > 0 && !y) || !inv_perm || !topk_weights || !out) return fail(LSG_ERR_INVALID, "moe_unpermute: null pointer");
+    return LSG_BY_DTYPE(sum_slots)(y, inv_perm, topk_weights, rows, num_tokens, top_k, H, out, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lsg_moe_permute_backward(const void* grad_rows, int dtype, const int32_t* inv_perm, int rows, int num_tokens,
+                                        int top_k, int H, void* grad_hidden, void* stream) {
+    const int rc = check_moe("moe_permute_backward", dtype, num_tokens, top_k, H);
+    if (rc != LSG_OK) return rc;
+    if (rows < 0) return fail(LSG_ERR_INVALID, "moe_permute_backward: negative shape");
+    if (num_tokens == 0 || H == 0) return LSG_OK;
+    if ((rows > 0 && !grad_rows) || !inv_perm || !grad_hidden)
+        return fail(LSG_ERR_INVALID, "moe_permute_backward: null pointer");
+    return LSG_BY_DTYPE(sum_slots)(grad_rows, inv_perm, nullptr, rows, num_tokens, top_k, H, grad_hidden,
+                                   static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lsg_moe_unpermute_backward(const void* grad_out, const void* y, int dtype, const int32_t* inv_perm,
+                                          const float* topk_weights, const int32_t* expert_offsets, int num_experts, int rows,
+                                          int num_tokens, int top_k, int H, void* grad_y, float* grad_weights, void* stream) {
+    const int rc = check_moe("moe_unpermute_backward", dtype, num_tokens, top_k, H);
+    if (rc != LSG_OK) return rc;
+    if (rows < 0) return fail(LSG_ERR_INVALID, "moe_unpermute_backward: negative shape");
+    if (rows > static_cast<long long>(num_tokens) * top_k)
+        return fail(LSG_ERR_INVALID, "moe_unpermute_backward: more rows than (token, slot) pairs");
+    if (expert_offsets && num_experts < 1) return fail(LSG_ERR_INVALID, "moe_unpermute_backward: num_experts must be positive");
+    if (num_tokens == 0) return LSG_OK;
+    if (!inv_perm || !topk_weights || !grad_weights || (H > 0 && (!grad_out || (rows > 0 && (!y || !grad_y)))))
+        return fail(LSG_ERR_INVALID, "moe_unpermute_backward: null pointer");
+    return LSG_BY_DTYPE(unpermute_backward)(grad_out, y, inv_perm, topk_weights,
+                                            expert_offsets ? expert_offsets + num_experts : nullptr, rows, num_tokens, top_k, H,
+                                            grad_y, grad_weights, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lsg_moe_route_backward(const int32_t* topk_idx, const float* topk_weights, const float* grad_weights,
+                                      int num_tokens, int num_experts, int top_k, float* grad_logits, void* stream) {
+    if (num_tokens < 0) return fail(LSG_ERR_INVALID, "moe_route_backward: negative shape");
+    if (num_experts < 1 || num_experts > 1024 || top_k < 1 || top_k > kMaxSlots || top_k > num_experts)
+        return fail(LSG_ERR_INVALID, "moe_route_backward: need 1 <= top_k <= min(16, E) and E <= 1024 (E=%d, k=%d)",
+                    num_experts, top_k);
+    if (num_tokens == 0) return LSG_OK;
+    if (!topk_idx || !topk_weights || !grad_weights || !grad_logits)
+        return fail(LSG_ERR_INVALID, "moe_route_backward: null pointer");
+    LSG_CUDA_TRY(launch_kernel(moe_route_backward_kernel, dim3(static_cast<unsigned>((static_cast<long long>(num_tokens) + 7) / 8)),
+                               dim3(256), 0, static_cast<cudaStream_t>(stream), true, topk_idx, topk_weights, grad_weights,
+                               num_tokens, num_experts, top_k, grad_logits));
+    return LSG_OK;
+}

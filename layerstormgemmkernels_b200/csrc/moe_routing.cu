@@ -86,7 +86,9 @@ moe_route_kernel(const float* __restrict__ logits, int T, int E, int k, int32_t*
 //      exclusive scan of the totals over the experts (= expert_offsets),
 //   3. per chunk, each pair's rank among the earlier pairs of the same expert:
 //      earlier chunks (step 2), earlier warps of the chunk, earlier lanes of the warp.
-// Pairs whose expert id lies outside [0, E) are ignored.
+// Pairs whose expert id lies outside [0, E) get no row: their entry of inv is -1, and the rows
+// behind the last expert's, which belong to no pair, name pair 0 in perm so that a gather through
+// it stays in bounds.
 constexpr int kChunk = 256;
 
 __global__ void __launch_bounds__(kChunk)
@@ -197,7 +199,10 @@ moe_place_kernel(const int32_t* __restrict__ idx, int P, int E, const int32_t* _
         const int row = offsets[e] + chunk_base[static_cast<size_t>(e) * gridDim.x + blockIdx.x] + before + rank;
         perm[row] = i;
         inv[i] = row;
+    } else if (i < P) {
+        inv[i] = -1;
     }
+    if (i < P && i >= offsets[E]) perm[i] = 0;
 }
 
 // The three steps above in one CTA, for P <= 1024 pairs (decode-sized batches, where three
@@ -256,11 +261,15 @@ moe_permutation_small_kernel(const int32_t* __restrict__ idx, int P, int E, int3
     }
     if (tid == E - 1) offsets[E] = before + incl;
     __syncthreads();
+    const int placed = __syncthreads_count(e >= 0);
     if (e >= 0) {
         const int row = totals[e] + whist[warp * E + e] + rank;
         perm[row] = tid;
         inv[tid] = row;
+    } else if (tid < P) {
+        inv[tid] = -1;
     }
+    if (tid < P && tid >= placed) perm[tid] = 0;
 }
 
 // out[row, :] = hidden[perm[row] / k, :]   (bf16 rows, 16-byte vectors)
@@ -275,7 +284,8 @@ moe_gather_kernel(const uint4* __restrict__ hidden, const int32_t* __restrict__ 
     out[i] = __ldg(hidden + static_cast<size_t>(perm[row] / k) * vec_per_row + c);
 }
 
-// out[t, :] = sum_s w[t, s] * y[inv[t * k + s], :], slots in order, fp32 accumulate.
+// out[t, :] = sum_s w[t, s] * y[inv[t * k + s], :], slots in order, fp32 accumulate; a pair without a
+// row (inv < 0) adds nothing.
 __global__ void __launch_bounds__(256)
 moe_combine_kernel(const __nv_bfloat16* __restrict__ y, const int32_t* __restrict__ inv,
                    const float* __restrict__ w, int T, int k, int H, __nv_bfloat16* __restrict__ out) {
@@ -288,6 +298,7 @@ moe_combine_kernel(const __nv_bfloat16* __restrict__ y, const int32_t* __restric
     float a0 = 0.0f, a1 = 0.0f;
     for (int s = 0; s < k; ++s) {
         const int row = inv[static_cast<size_t>(t) * k + s];
+        if (row < 0) continue;
         const float ws = w[static_cast<size_t>(t) * k + s];
         const __nv_bfloat162 v = reinterpret_cast<const __nv_bfloat162*>(y + static_cast<size_t>(row) * H)[c];
         a0 = fmaf(ws, __bfloat162float(v.x), a0);
@@ -313,8 +324,8 @@ moe_combine_vec_kernel(const uint4* __restrict__ y, const int32_t* __restrict__ 
         for (int s = 0; s < KMAX; ++s) {
             if (s < k) {
                 const int row = __ldg(inv + static_cast<size_t>(t) * k + s);
-                ws[s] = __ldg(w + static_cast<size_t>(t) * k + s);
-                r[s] = __ldg(y + static_cast<size_t>(row) * vpr + v);
+                ws[s] = row >= 0 ? __ldg(w + static_cast<size_t>(t) * k + s) : 0.0f;
+                r[s] = row >= 0 ? __ldg(y + static_cast<size_t>(row) * vpr + v) : make_uint4(0, 0, 0, 0);
             }
         }
         float acc[8];

@@ -692,6 +692,217 @@ def nvfp4_grouped_gemm(A_base, B_base, D_base, scale_A_base, scale_B_base, alpha
 
 
 # ---------------------------------------------------------------------------
+# 8-bit integers with a scale per token and per output channel (additions; the reference's
+# 8-bit family is FP8)
+# ---------------------------------------------------------------------------
+_CODE = {torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16, torch.float32: capi.DTYPE_F32}
+_INT8_OUT = {"bf16": (capi.DTYPE_BF16, torch.bfloat16), "bfloat16": (capi.DTYPE_BF16, torch.bfloat16),
+             "fp16": (capi.DTYPE_F16, torch.float16), "float16": (capi.DTYPE_F16, torch.float16),
+             "fp32": (capi.DTYPE_F32, torch.float32), "float32": (capi.DTYPE_F32, torch.float32)}
+
+
+def _int8_out(s):
+    out = _INT8_OUT.get(s)
+    _require(out is not None, f"Unknown output dtype: {s}. Expected 'bf16', 'fp16' or 'fp32'.")
+    return out
+
+
+def _call(device, fn, *args):
+    """fn(*args, stream) on the current stream of `device`, whichever device is current."""
+    i = device.index
+    if i == torch.cuda.current_device():
+        capi.check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(i):
+            capi.check(fn(*args, torch.cuda.current_stream().cuda_stream))
+
+
+def _require_rows(op, name, t, dtypes, kinds):
+    _require(t.is_cuda and t.dtype in dtypes, f"{op}: {name} must be {kinds} on CUDA")
+    _require(t.dim() == 2 and (t.stride(1) == 1 or t.size(1) <= 1) and (t.size(0) <= 1 or t.stride(0) >= t.size(1)),
+             f"{op}: {name} must be [rows, columns] with contiguous rows that do not overlap")
+
+
+def _require_vector(op, name, t, dtype, shape, like):
+    _require(t.is_cuda and t.dtype == dtype and t.device == like.device and t.is_contiguous()
+             and tuple(t.shape) == tuple(shape),
+             f"{op}: {name} must be contiguous {str(dtype)[6:]} {list(shape)} on the inputs' device")
+
+
+def _ld(t):
+    return t.stride(0) if t.size(0) > 1 else max(t.size(1), 1)
+
+
+def _ldc(t):
+    # row stride of int8 codes; a single row has no next one, so its stride is what alignment asks for
+    return t.stride(0) if t.size(0) > 1 else (t.size(1) + 15) // 16 * 16
+
+
+_HALVES = (torch.bfloat16, torch.float16)
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _code_rows(rows, K, device):
+    """int8 [rows, K] whose rows start 16 bytes apart or a multiple of it, as int8_gemm reads them."""
+    ld = (K + 15) // 16 * 16
+    codes = torch.empty((rows, ld), dtype=torch.int8, device=device)
+    return (codes if ld == K else codes[:, :K]), ld
+
+
+def dynamic_int8_quant(input):
+    """bf16 or fp16 [M,K] -> (codes int8 [M,K], scales fp32 [M]): scale = max|row| / 127, codes the
+    nearest integers of 127 * row / max|row| (half-way cases to even).
+
+    An all-zero row gets scale 0, a row with an infinity or NaN scale NaN and codes 0.  Where K is
+    not a multiple of 16 the codes are a view of rows padded to one, the form int8_gemm takes."""
+    _require_rows("dynamic_int8_quant", "input", input, _HALVES, "BF16 or FP16")
+    M, K = input.shape
+    codes, ldq = _code_rows(M, K, input.device)
+    scales = torch.empty((M,), dtype=torch.float32, device=input.device)
+    _call(input.device, _lib.lsg_dynamic_int8_quant, input.data_ptr(), _ld(input), _CODE[input.dtype],
+          codes.data_ptr(), ldq, scales.data_ptr(), M, K)
+    return codes, scales
+
+
+def weight_int8_quant(weight):
+    """bf16 or fp16 [N,K] or [E,N,K] -> (codes int8 of that shape, scales fp32 [N] or [E,N]): one
+    scale per output channel, as dynamic_int8_quant.  [E,N,K] needs K % 16 == 0."""
+    _require(weight.is_cuda and weight.dtype in _HALVES, "weight_int8_quant: weight must be BF16 or FP16 on CUDA")
+    _require(weight.dim() in (2, 3) and weight.is_contiguous(),
+             "weight_int8_quant: weight must be contiguous [N, K] or [E, N, K]")
+    if weight.dim() == 2:
+        return dynamic_int8_quant(weight)
+    E, N, K = weight.shape
+    _require(K % 16 == 0, f"weight_int8_quant: K must be divisible by 16 for [E, N, K], got K={K}")
+    codes, scales = dynamic_int8_quant(weight.view(E * N, K))
+    return codes.view(E, N, K), scales.view(E, N)
+
+
+def silu_mul_int8_quant(gate, up):
+    """silu(gate) * up, formed in fp32, quantized per row: (codes int8 [M,K], scales fp32 [M]).
+    gate, up: bf16, fp16 or fp32 [M,K] with contiguous rows (halves of one [M, 2K] matrix will do)."""
+    _require_rows("silu_mul_int8_quant", "gate", gate, _FLOATS, "BF16, FP16 or FP32")
+    _require_rows("silu_mul_int8_quant", "up", up, _FLOATS, "BF16, FP16 or FP32")
+    _require(gate.shape == up.shape and gate.dtype == up.dtype and gate.device == up.device,
+             "silu_mul_int8_quant: gate and up must have the same shape, dtype and device")
+    M, K = gate.shape
+    codes, ldq = _code_rows(M, K, gate.device)
+    scales = torch.empty((M,), dtype=torch.float32, device=gate.device)
+    _call(gate.device, _lib.lsg_silu_mul_int8_quant, gate.data_ptr(), _ld(gate), up.data_ptr(), _ld(up),
+          _CODE[gate.dtype], codes.data_ptr(), ldq, scales.data_ptr(), M, K)
+    return codes, scales
+
+
+def int8_gemm(A, B, scale_A, scale_B, M, N, K, output_dtype):
+    """D[m,n] = scale_A[m] * scale_B[n] * sum_k A[m,k] B[n,k] of int8 A [M,K] and B [N,K], the sum
+    exact, one rounding to 'bf16', 'fp16' or 'fp32'.  1 <= K <= 131056; the rows of A and B start on
+    16-byte boundaries (a view of padded rows where K is not a multiple of 16)."""
+    code, tdtype = _int8_out(output_dtype)
+    M, N, K = int(M), int(N), int(K)
+    for name, t, rows in (("A", A, M), ("B", B, N)):
+        _require_rows("int8_gemm", name, t, (torch.int8,), "INT8")
+        _require(t.size(0) == rows and t.size(1) == K, f"int8_gemm: {name} shape mismatch")
+    _require(A.device == B.device, "int8_gemm: A and B must be on one device")
+    _require_vector("int8_gemm", "scale_A", scale_A, torch.float32, (M,), A)
+    _require_vector("int8_gemm", "scale_B", scale_B, torch.float32, (N,), A)
+    D = torch.empty((M, N), dtype=tdtype, device=A.device)
+    p = capi.Int8GemmParams(M, N, K, A.data_ptr(), _ldc(A), B.data_ptr(), _ldc(B), D.data_ptr(), scale_A.data_ptr(),
+                            scale_B.data_ptr(), code)
+    _call(A.device, _lib.lsg_int8_gemm, p)
+    return D
+
+
+def int8_gemm_from_bf16(x, weight, weight_scales, output_dtype="bf16"):
+    """bf16 or fp16 x [M,K] quantized per token, times the int8 weight [N,K]: dynamic_int8_quant and
+    int8_gemm in one call, the same bits."""
+    code, tdtype = _int8_out(output_dtype)
+    _require_rows("int8_gemm_from_bf16", "x", x, _HALVES, "BF16 or FP16")
+    _require_rows("int8_gemm_from_bf16", "weight", weight, (torch.int8,), "INT8")
+    (M, K), N = x.shape, weight.size(0)
+    _require(weight.size(1) == K and weight.device == x.device, "int8_gemm_from_bf16: weight must be [N, K] on x's device")
+    _require_vector("int8_gemm_from_bf16", "weight_scales", weight_scales, torch.float32, (N,), x)
+    D = torch.empty((M, N), dtype=tdtype, device=x.device)
+    ws_bytes = _lib.lsg_int8_gemm_from_bf16_workspace_bytes(M, K)
+    ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=x.device)
+    p = capi.Int8GemmParams(M, N, K, x.data_ptr(), _ld(x), weight.data_ptr(), _ldc(weight), D.data_ptr(), None,
+                            weight_scales.data_ptr(), code)
+    _call(x.device, _lib.lsg_int8_gemm_from_bf16, p, _CODE[x.dtype], ws.data_ptr(), ws_bytes)
+    return D
+
+
+def int8_grouped_gemm(A_base, B_base, D_base, scale_A_base, scale_B_base, expert_offsets, N, K, output_dtype):
+    """int8_gemm for rows grouped by expert, into D_base (returned): rows [offsets[e], offsets[e+1])
+    of A_base [T,K] times B_base[e] of [E,N,K].  Routed on the device; rows behind the last expert's
+    are left as they are."""
+    code, tdtype = _int8_out(output_dtype)
+    N, K = int(N), int(K)
+    _require_rows("int8_grouped_gemm", "A_base", A_base, (torch.int8,), "INT8")
+    T = A_base.size(0)
+    _require(A_base.size(1) == K, "int8_grouped_gemm: A_base.size(1) != K")
+    _require(B_base.is_cuda and B_base.dtype == torch.int8 and B_base.dim() == 3 and B_base.is_contiguous()
+             and B_base.size(1) == N and B_base.size(2) == K and B_base.device == A_base.device,
+             "int8_grouped_gemm: B_base must be contiguous INT8 [E, N, K] on A_base's device")
+    E = B_base.size(0)
+    _require(D_base.is_cuda and D_base.dtype == tdtype and D_base.is_contiguous() and D_base.device == A_base.device
+             and tuple(D_base.shape) == (T, N),
+             "int8_grouped_gemm: D_base must be contiguous [T, N] of output_dtype on A_base's device")
+    _require_vector("int8_grouped_gemm", "scale_A_base", scale_A_base, torch.float32, (T,), A_base)
+    _require_vector("int8_grouped_gemm", "scale_B_base", scale_B_base, torch.float32, (E, N), A_base)
+    _require_vector("int8_grouped_gemm", "expert_offsets", expert_offsets, torch.int32, (E + 1,), A_base)
+    p = capi.Int8GroupedGemmParams(E, N, K, A_base.data_ptr(), _ldc(A_base), B_base.data_ptr(), K, D_base.data_ptr(),
+                                   scale_A_base.data_ptr(), scale_B_base.data_ptr(), expert_offsets.data_ptr(), code)
+    _call(A_base.device, _lib.lsg_int8_grouped_gemm, p, T)
+    return D_base
+
+
+def moe_permute_int8(hidden, inv_perm, top_k):
+    """moe_permute and dynamic_int8_quant in one pass over bf16 or fp16 hidden [T,H]: (codes int8
+    [T*k,H], scales fp32 [T*k]), row inv_perm[t*k+s] holding token t.  Pairs without a row
+    (inv_perm < 0) are left out; rows no pair names are uninitialised."""
+    _require_rows("moe_permute_int8", "hidden", hidden, _HALVES, "BF16 or FP16")
+    (T, H), k = hidden.shape, int(top_k)
+    _require(k >= 1, "moe_permute_int8: top_k must be positive")
+    _require_vector("moe_permute_int8", "inv_perm", inv_perm, torch.int32, (T * k,), hidden)
+    codes, ldq = _code_rows(T * k, H, hidden.device)
+    scales = torch.empty((T * k,), dtype=torch.float32, device=hidden.device)
+    _call(hidden.device, _lib.lsg_moe_permute_int8, hidden.data_ptr(), _ld(hidden), _CODE[hidden.dtype],
+          inv_perm.data_ptr(), T, k, H, codes.data_ptr(), ldq, scales.data_ptr())
+    return codes, scales
+
+
+def int8_moe_ffn(hidden, expert_offsets, inv_perm, top_k, gate_up, gate_up_scales, down, down_scales,
+                 output_dtype="bf16"):
+    """Expert feed-forward block in 8-bit integers: row inv_perm[t*k+s] of the result [T*k,H] is
+    down_e(quant(silu(g) * u)), (g | u) = gate_up_e(quant(hidden[t])), for the row's expert e.
+
+    hidden bf16 or fp16 [T,H]; gate_up int8 [E,2I,H] (gate rows, then up rows) with scales fp32
+    [E,2I]; down int8 [E,H,I] with scales fp32 [E,H]; H and I multiples of 16.  Rows behind the
+    last expert's are uninitialised.  moe_unpermute takes the result back to the tokens."""
+    code, tdtype = _int8_out(output_dtype)
+    _require_rows("int8_moe_ffn", "hidden", hidden, _HALVES, "BF16 or FP16")
+    (T, H), k = hidden.shape, int(top_k)
+    _require(k >= 1, "int8_moe_ffn: top_k must be positive")
+    for name, t in (("gate_up", gate_up), ("down", down)):
+        _require(t.is_cuda and t.dtype == torch.int8 and t.dim() == 3 and t.is_contiguous() and t.device == hidden.device,
+                 f"int8_moe_ffn: {name} must be contiguous INT8 [E, rows, columns] on hidden's device")
+    E, I = gate_up.size(0), down.size(2)
+    _require(tuple(gate_up.shape) == (E, 2 * I, H) and tuple(down.shape) == (E, H, I),
+             "int8_moe_ffn: gate_up must be [E, 2I, H] and down [E, H, I]")
+    _require_vector("int8_moe_ffn", "gate_up_scales", gate_up_scales, torch.float32, (E, 2 * I), hidden)
+    _require_vector("int8_moe_ffn", "down_scales", down_scales, torch.float32, (E, H), hidden)
+    _require_vector("int8_moe_ffn", "expert_offsets", expert_offsets, torch.int32, (E + 1,), hidden)
+    _require_vector("int8_moe_ffn", "inv_perm", inv_perm, torch.int32, (T * k,), hidden)
+    D = torch.empty((T * k, H), dtype=tdtype, device=hidden.device)
+    ws_bytes = _lib.lsg_int8_moe_ffn_workspace_bytes(T, k, H, I)
+    ws = torch.empty((max(ws_bytes, 1),), dtype=torch.uint8, device=hidden.device)
+    p = capi.Int8MoeFfnParams(T, k, E, H, I, hidden.data_ptr(), _ld(hidden), _CODE[hidden.dtype],
+                              expert_offsets.data_ptr(), inv_perm.data_ptr(), gate_up.data_ptr(),
+                              gate_up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(), D.data_ptr(), code)
+    _call(hidden.device, _lib.lsg_int8_moe_ffn, p, ws.data_ptr(), ws_bytes)
+    return D
+
+
+# ---------------------------------------------------------------------------
 # MoE routing (additions; the reference takes pre-permuted rows)
 # ---------------------------------------------------------------------------
 def moe_route(logits, top_k):
@@ -734,16 +945,104 @@ def ep_expert_order(recv_counts, world, experts_per_rank, rows):
 
 
 def moe_permute(hidden, perm, top_k):
+    """out[row] = hidden[perm[row] // top_k], bf16, fp16 or fp32 [T,H] -> [rows,H]."""
     rows, H = perm.numel(), hidden.size(1)
+    if hidden.dtype != torch.bfloat16:
+        _require_dense("moe_permute", "hidden", hidden)
+        _require_vector("moe_permute", "perm", perm, torch.int32, (rows,), hidden)
+        out = torch.empty((rows, H), dtype=hidden.dtype, device=hidden.device)
+        _call(hidden.device, _lib.lsg_moe_permute_dtype, hidden.data_ptr(), _CODE[hidden.dtype], perm.data_ptr(), rows,
+              hidden.size(0), int(top_k), H, out.data_ptr())
+        return out
     out = torch.empty((rows, H), dtype=torch.bfloat16, device=hidden.device)
     capi.check(_lib.lsg_moe_permute(_ptr(hidden), _ptr(perm), rows, int(top_k), H, _ptr(out), _stream()))
     return out
 
 
 def moe_unpermute(y, inv_perm, topk_weights):
+    """out[t] = sum over slots of topk_weights[t,s] * y[inv_perm[t*k+s]], bf16, fp16 or fp32; pairs
+    without a row (inv_perm < 0) add nothing."""
     T, k = topk_weights.shape
     H = y.size(1)
+    if y.dtype != torch.bfloat16:
+        _require_dense("moe_unpermute", "y", y)
+        _require_vector("moe_unpermute", "inv_perm", inv_perm, torch.int32, (T * k,), y)
+        _require_vector("moe_unpermute", "topk_weights", topk_weights, torch.float32, (T, k), y)
+        out = torch.empty((T, H), dtype=y.dtype, device=y.device)
+        _call(y.device, _lib.lsg_moe_unpermute_dtype, y.data_ptr(), _CODE[y.dtype], inv_perm.data_ptr(),
+              topk_weights.data_ptr(), y.size(0), T, k, H, out.data_ptr())
+        return out
     out = torch.empty((T, H), dtype=torch.bfloat16, device=y.device)
     capi.check(_lib.lsg_moe_unpermute(_ptr(y), _ptr(inv_perm), _ptr(topk_weights), T, k, H, _ptr(out),
                                       _stream()))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Gradients of the MoE routing steps
+# ---------------------------------------------------------------------------
+def _require_dense(op, name, t):
+    _require(t.is_cuda and t.dtype in _FLOATS and t.dim() == 2 and t.is_contiguous(),
+             f"{op}: {name} must be contiguous BF16, FP16 or FP32 [rows, H] on CUDA")
+
+
+def moe_permute_backward(grad_rows, inv_perm, top_k):
+    """Gradient of moe_permute: grad_hidden[t] = sum over slots of grad_rows[inv_perm[t*k+s]], in
+    fp32 in the order of the slots.  grad_rows bf16, fp16 or fp32 [rows,H] -> [T,H] of its type;
+    pairs without a row (inv_perm < 0) add nothing."""
+    _require_dense("moe_permute_backward", "grad_rows", grad_rows)
+    (rows, H), k = grad_rows.shape, int(top_k)
+    _require(k >= 1 and inv_perm.dim() == 1 and inv_perm.numel() % k == 0,
+             "moe_permute_backward: inv_perm must hold top_k entries per token")
+    _require_vector("moe_permute_backward", "inv_perm", inv_perm, torch.int32, inv_perm.shape, grad_rows)
+    T = inv_perm.numel() // k
+    out = torch.empty((T, H), dtype=grad_rows.dtype, device=grad_rows.device)
+    _call(grad_rows.device, _lib.lsg_moe_permute_backward, grad_rows.data_ptr(), _CODE[grad_rows.dtype],
+          inv_perm.data_ptr(), rows, T, k, H, out.data_ptr())
+    return out
+
+
+def moe_unpermute_backward(grad_out, y, inv_perm, topk_weights, expert_offsets=None):
+    """Gradients of moe_unpermute: (grad_y, grad_weights) with
+    grad_y[inv_perm[t*k+s]] = topk_weights[t,s] * grad_out[t] and
+    grad_weights[t,s] = <y[inv_perm[t*k+s]], grad_out[t]> (0 for a pair without a row).
+
+    grad_out [T,H] and y [rows,H] bf16, fp16 or fp32, alike; grad_weights fp32 [T,k].  With
+    expert_offsets (int32, as moe_permutation returns them) the rows behind the last expert's are
+    cleared in grad_y; without them, rows that no pair names are uninitialised."""
+    op = "moe_unpermute_backward"
+    _require_dense(op, "grad_out", grad_out)
+    _require_dense(op, "y", y)
+    _require(y.dtype == grad_out.dtype and y.device == grad_out.device and y.size(1) == grad_out.size(1),
+             f"{op}: grad_out and y must have the same dtype, device and H")
+    _require(topk_weights.dim() == 2, f"{op}: topk_weights must be [T, k]")
+    (T, H), (rows, k) = grad_out.shape, (y.size(0), topk_weights.size(1))
+    _require_vector(op, "topk_weights", topk_weights, torch.float32, (T, k), y)
+    _require_vector(op, "inv_perm", inv_perm, torch.int32, (T * k,), y)
+    if expert_offsets is not None:
+        _require(expert_offsets.dim() == 1 and expert_offsets.numel() >= 2, f"{op}: expert_offsets must be [E + 1]")
+        _require_vector(op, "expert_offsets", expert_offsets, torch.int32, expert_offsets.shape, y)
+    grad_y = torch.empty_like(y)
+    grad_w = torch.empty((T, k), dtype=torch.float32, device=y.device)
+    _call(y.device, _lib.lsg_moe_unpermute_backward, grad_out.data_ptr(), y.data_ptr(), _CODE[y.dtype],
+          inv_perm.data_ptr(), topk_weights.data_ptr(), expert_offsets.data_ptr() if expert_offsets is not None else None,
+          expert_offsets.numel() - 1 if expert_offsets is not None else 0, rows, T, k, H, grad_y.data_ptr(),
+          grad_w.data_ptr())
+    return grad_y, grad_w
+
+
+def moe_route_backward(topk_idx, topk_weights, grad_weights, num_experts):
+    """Gradient of moe_route by its logits: fp32 [T,E] from the weights' gradient fp32 [T,k].  The
+    weights are the softmax over the chosen logits, so grad_logits[t, topk_idx[t,s]] =
+    w[t,s] * (grad_weights[t,s] - sum_r w[t,r] grad_weights[t,r]), and 0 elsewhere."""
+    op = "moe_route_backward"
+    _require(topk_idx.dim() == 2, f"{op}: topk_idx must be [T, k]")
+    T, k = topk_idx.shape
+    _require(topk_idx.is_cuda and topk_idx.dtype == torch.int32 and topk_idx.is_contiguous(),
+             f"{op}: topk_idx must be contiguous int32 [T, k] on CUDA")
+    _require_vector(op, "topk_weights", topk_weights, torch.float32, (T, k), topk_idx)
+    _require_vector(op, "grad_weights", grad_weights, torch.float32, (T, k), topk_idx)
+    out = torch.empty((T, int(num_experts)), dtype=torch.float32, device=topk_idx.device)
+    _call(topk_idx.device, _lib.lsg_moe_route_backward, topk_idx.data_ptr(), topk_weights.data_ptr(),
+          grad_weights.data_ptr(), T, int(num_experts), k, out.data_ptr())
     return out
