@@ -22,6 +22,9 @@ struct Int8Gemm {
 };
 
 int int8_gemm(const Int8Gemm& a, cudaStream_t s);
+// On the tensor cores (int8_mma.cu).  swiglu: B is [E, 2 N, K], gate rows in front of up rows, and D
+// fp32 silu(gate) * up.
+int int8_mma(const Int8Gemm& g, bool swiglu, cudaStream_t s);
 int int8_quant_rows(const void* x, long long ldx, int dtype, int8_t* codes, long long ldq, float* scales, long long rows,
                     int K, const int32_t* inv, int top_k, int out_rows, cudaStream_t s);
 int int8_quant_silu_mul(const void* gate, long long ldg, const void* up, long long ldu, int dtype, int8_t* codes,
@@ -39,44 +42,6 @@ __device__ __forceinline__ void store_out(void* D, int dtype, size_t at, float v
     if (dtype == LSG_DTYPE_F32) static_cast<float*>(D)[at] = v;
     else if (dtype == LSG_DTYPE_F16) static_cast<__half*>(D)[at] = __float2half_rn(v);
     else static_cast<__nv_bfloat16*>(D)[at] = __float2bfloat16_rn(v);
-}
-
-// The u-th unit of up to `tile` rows that belong to one expert, for rows grouped by expert: every
-// expert's rows cut into ceil(rows / tile) units, numbered from expert 0 on.  False behind the last.
-// Called by whole warps.  Offsets are taken as [0, total] whatever they hold.
-__device__ __forceinline__ bool find_unit(const int32_t* offsets, int E, int total, int tile, int u, int& expert, int& row0,
-                                          int& rows) {
-    const int lane = threadIdx.x & 31;
-    int before = 0;   // units of the experts in front of this group of 32
-    for (int e0 = 0; e0 < E; e0 += 32) {
-        const int e = e0 + lane;
-        int a = 0, b = 0;
-        if (e < E) {
-            a = min(max(__ldg(offsets + e), 0), total);
-            b = min(max(__ldg(offsets + e + 1), a), total);
-        }
-        const int units = (b - a + tile - 1) / tile;
-        int incl = units;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
-        }
-        const int sum = __shfl_sync(0xffffffffu, incl, 31);
-        if (u < before + sum) {
-            const unsigned above = __ballot_sync(0xffffffffu, u < before + incl);
-            const int at = __ffs(above) - 1;
-            const int first = before + __shfl_sync(0xffffffffu, incl - units, at);
-            a = __shfl_sync(0xffffffffu, a, at);
-            b = __shfl_sync(0xffffffffu, b, at);
-            expert = e0 + at;
-            row0 = a + (u - first) * tile;
-            rows = min(tile, b - row0);
-            return true;
-        }
-        before += sum;
-    }
-    return false;
 }
 
 #endif  // __CUDACC__

@@ -21,10 +21,9 @@ int8_dot_kernel(const Int8Gemm a) {
     pdl_wait_prior();
     const int lane = threadIdx.x & 31;
     const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
-    int expert = 0, r0 = blockIdx.y * 8, rows = min(8, a.M - r0);
-    if (a.expert_offsets && !find_unit(a.expert_offsets, a.E, a.M, 8, blockIdx.y, expert, r0, rows)) return;
-    if (n >= a.N || rows <= 0) return;
-    const int8_t* w = a.B + (static_cast<long long>(expert) * a.N + n) * a.ldb;
+    const int r0 = blockIdx.y * 8, rows = min(8, a.M - r0);
+    if (n >= a.N) return;
+    const int8_t* w = a.B + static_cast<long long>(n) * a.ldb;
     int acc[8];
 #pragma unroll
     for (int m = 0; m < 8; ++m) acc[m] = 0;
@@ -47,7 +46,7 @@ int8_dot_kernel(const Int8Gemm a) {
         for (int m = 1; m < 8; ++m) v = lane == m ? acc[m] : v;
         const int row = r0 + lane;
         store_out(a.D, a.out_dtype, static_cast<size_t>(row) * a.N + n,
-                  static_cast<float>(v) * a.scale_A[row] * a.scale_B[static_cast<long long>(expert) * a.N + n]);
+                  __fmul_rn(__fmul_rn(static_cast<float>(v), a.scale_A[row]), a.scale_B[n]));
     }
 }
 
@@ -68,9 +67,8 @@ int check(const char* op, int N, int K, const void* A, long long lda, const void
 }  // namespace
 
 int int8_gemm(const Int8Gemm& a, cudaStream_t s) {
-    const long long units = a.expert_offsets ? a.M / 8 + static_cast<long long>(a.E) : (a.M + 7) / 8;
-    if (units > 65535) return fail(LSG_ERR_UNSUPPORTED, "int8 product: too many rows");
-    LSG_CUDA_TRY(launch_kernel(int8_dot_kernel, dim3((a.N + 7) / 8, static_cast<unsigned>(units)), dim3(256), 0, s, true, a));
+    if (a.M > 8 || a.expert_offsets) return int8_mma(a, false, s);
+    LSG_CUDA_TRY(launch_kernel(int8_dot_kernel, dim3((a.N + 7) / 8, (a.M + 7) / 8), dim3(256), 0, s, true, a));
     return LSG_OK;
 }
 
@@ -160,7 +158,7 @@ extern "C" int lsg_int8_grouped_gemm(const lsg_int8_grouped_gemm_params* p, int 
 
 namespace {
 struct FfnPlan {
-    size_t codes, scales, gate_up, act, act_scales, total;
+    size_t codes, scales, h, act, act_scales, total;
     long long ldh, ldi;
 };
 FfnPlan ffn_plan(long long rows, int H, int I) {
@@ -169,8 +167,8 @@ FfnPlan ffn_plan(long long rows, int H, int I) {
     f.ldi = pad16(I);
     f.codes = 0;
     f.scales = f.codes + a256(static_cast<size_t>(rows) * f.ldh);
-    f.gate_up = f.scales + a256(static_cast<size_t>(rows) * 4);
-    f.act = f.gate_up + a256(static_cast<size_t>(rows) * 2 * I * 4);
+    f.h = f.scales + a256(static_cast<size_t>(rows) * 4);
+    f.act = f.h + a256(static_cast<size_t>(rows) * I * 4);
     f.act_scales = f.act + a256(static_cast<size_t>(rows) * f.ldi);
     f.total = f.act_scales + a256(static_cast<size_t>(rows) * 4);
     return f;
@@ -212,18 +210,18 @@ extern "C" int lsg_int8_moe_ffn(const lsg_int8_moe_ffn_params* p, void* workspac
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     int8_t* codes = reinterpret_cast<int8_t*>(ws + f.codes);
     float* scales = reinterpret_cast<float*>(ws + f.scales);
-    float* gu = reinterpret_cast<float*>(ws + f.gate_up);
+    float* h = reinterpret_cast<float*>(ws + f.h);
     int8_t* act = reinterpret_cast<int8_t*>(ws + f.act);
     float* act_scales = reinterpret_cast<float*>(ws + f.act_scales);
     rc = int8_quant_rows(p->hidden, p->ld_hidden, p->input_dtype, codes, f.ldh, scales, p->num_tokens, H, p->inv_perm, p->top_k, rows, s);
     if (rc != LSG_OK) return rc;
     Int8Gemm a = {};
     a.A = codes; a.lda = f.ldh; a.B = static_cast<const int8_t*>(p->gate_up); a.ldb = H;
-    a.D = gu; a.out_dtype = LSG_DTYPE_F32; a.scale_A = scales; a.scale_B = p->gate_up_scales;
-    a.M = rows; a.N = 2 * I; a.K = H; a.E = p->num_experts; a.expert_offsets = p->expert_offsets;
-    rc = int8_gemm(a, s);
+    a.D = h; a.out_dtype = LSG_DTYPE_F32; a.scale_A = scales; a.scale_B = p->gate_up_scales;
+    a.M = rows; a.N = I; a.K = H; a.E = p->num_experts; a.expert_offsets = p->expert_offsets;
+    rc = int8_mma(a, true, s);
     if (rc != LSG_OK) return rc;
-    rc = int8_quant_silu_mul(gu, 2ll * I, gu + I, 2ll * I, LSG_DTYPE_F32, act, f.ldi, act_scales, rows, I, s);
+    rc = int8_quant_rows(h, I, LSG_DTYPE_F32, act, f.ldi, act_scales, rows, I, nullptr, 1, 0, s);
     if (rc != LSG_OK) return rc;
     a.A = act; a.lda = f.ldi; a.B = static_cast<const int8_t*>(p->down); a.ldb = I;
     a.D = p->D; a.out_dtype = p->output_dtype; a.scale_A = act_scales; a.scale_B = p->down_scales;

@@ -1,0 +1,592 @@
+// The 8-bit integer products on the tensor cores: tcgen05.mma.kind::i8, int32 accumulators in tensor
+// memory, scales and rounding on the way out.
+//
+// The weight is the M operand of the instruction and the tokens are its N operand, so a lane of
+// tensor memory is an output channel and a column is a token.  One kernel then serves every row
+// count: N is 16 to 256 tokens in steps of 16, few tokens cost few tensor cycles, and a warp's
+// store of one token is contiguous whatever N and M are.
+//
+//   warps 0-7   epilogue: warp w owns tensor-memory lanes 32 (w % 4).. and every second piece of 16
+//               columns (tokens)
+//   warp 8      TMA producer: 128 weight rows and the tile's tokens, 128 bytes of K a stage
+//   warp 9      MMA issuer: 4 instructions (K = 32 each) a stage
+//
+// Three forms of the same kernel:
+//   pair    two CTAs share a 256 x 256 tile (cta_group::2): each loads 128 weight rows and half of
+//           the tokens, 32 KB a stage for what takes 48 KB in one CTA
+//   single  one CTA, 128 weight rows x up to 256 tokens
+//   split   few tiles: K divided among the CTAs of a cluster, the int32 partial sums added through
+//           distributed shared memory (exactly, so the cut does not show in the result)
+// SwiGLU: of every 32 lanes 16 are gate rows and 16 the up rows of the same channels (one
+// five-dimensional box of the stacked weight puts them there), a shuffle brings g and u together and
+// silu(g) * u is stored in fp32: the quantizer that follows reads 4 bytes instead of 8.
+// Persistent except for split; every wait is time-limited.
+#include "common.cuh"
+#include "host.h"
+#include "int8.cuh"
+#include "tcgen05.cuh"
+
+#include <atomic>
+
+namespace lsg {
+
+using namespace tc;
+
+namespace {
+
+constexpr int kRows = 128;                   // weight rows of a CTA
+constexpr int kKB = 128;                     // bytes of K in a stage
+constexpr int kABytes = kRows * kKB;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarps + 2) * 32;
+constexpr int kMaxStages = 12;
+constexpr int kTailBytes = 512 + 2 * 1025 * 4 + 64;    // barriers, flags, the experts' tiles and rows
+constexpr int kSmemMax = 227 * 1024 - 1024 - kTailBytes;
+
+struct MmaArgs {
+    void* D;
+    int out_dtype;
+    const float* sA;
+    const float* sB;
+    const int32_t* offsets;   // null: dense
+    int M, N, E, kblocks;     // N: output columns (of silu(g) * u for SwiGLU)
+    int tn;                   // tokens of the tensor map's box (of a CTA: half of a pair's)
+    int tile;                 // tokens of a tile at most
+    int n_tiles, stages, stage_bytes, tmem_cols;
+    unsigned int* status;
+    long long limit;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// cta_group::2: the barrier may be the other CTA's of the pair.
+template <int CG>
+__device__ __forceinline__ void tma_5d(void* dst, const CUtensorMap* map, int x, int y, int z, int v, int w, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+            ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(v), "r"(w), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+            ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(v), "r"(w), "r"(bar)
+            : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+            ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+            ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+// Completion of the MMAs so far, to this barrier (of both CTAs of a pair).
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+            "h"(static_cast<uint16_t>(3))
+            : "memory");
+    else
+        tc_commit(bar);
+}
+template <int CG>
+__device__ __forceinline__ void alloc_tmem(uint32_t* slot, uint32_t cols) {
+    if constexpr (CG == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        tmem_alloc(slot, cols);
+    }
+}
+template <int CG>
+__device__ __forceinline__ void free_tmem(uint32_t addr, uint32_t cols) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+    else
+        tmem_dealloc(addr, cols);
+}
+
+// int8 x int8 -> int32, both operands K-major.
+__device__ __forceinline__ uint32_t idesc_i8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// The tile a CTA (or pair) works on next.
+struct Tile {
+    int expert, row0, rows, height, n;   // height: tokens the MMA multiplies, a multiple of STEP
+};
+
+// Tiles of an expert share its rows evenly, in heights that are multiples of `step`.
+__device__ __forceinline__ Tile tile_of(const MmaArgs& a, const int* cum, const int* start, int w, int step) {
+    Tile t;
+    int r0, rows, units, local;
+    if (a.offsets) {
+        int lo = 0, hi = a.E - 1;            // the last expert whose first tile is at most w
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (cum[mid] * a.n_tiles <= w) lo = mid;
+            else hi = mid - 1;
+        }
+        t.expert = lo;
+        units = cum[lo + 1] - cum[lo];
+        local = w - cum[lo] * a.n_tiles;
+        r0 = start[lo];
+        rows = start[lo + 1] - r0;
+    } else {
+        t.expert = 0;
+        units = (a.M + a.tile - 1) / a.tile;
+        local = w;
+        r0 = 0;
+        rows = a.M;
+    }
+    t.n = local / units;
+    const int u = local - t.n * units;
+    const int even = (rows + units - 1) / units;
+    t.height = (even + step - 1) / step * step;
+    t.row0 = r0 + u * t.height;
+    t.rows = min(t.height, rows - u * t.height);
+    return t;
+}
+
+template <int CG, bool SWIGLU, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1)
+int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const MmaArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + a.stages * a.stage_bytes);
+    uint64_t* empty = full + kMaxStages;
+    uint64_t* acc_full = empty + kMaxStages;   // [2]
+    uint64_t* acc_empty = acc_full + 2;        // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* cum = reinterpret_cast<int*>(smem + a.stages * a.stage_bytes + 512);   // [E + 1] tiles of tokens before expert e
+    int* start = cum + 1025;                                                      // [E + 1] first row
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = (CG == 2 || SPLIT) ? cluster_rank() : 0;
+    const uint32_t ranks = SPLIT ? cluster_size() : 1;
+    constexpr int kStep = CG == 2 ? 32 : 16;
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < a.stages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], kEpiWarps * CG);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == kEpiWarps + 1) alloc_tmem<CG>(tmem_slot, a.tmem_cols);
+    pdl_wait_prior();
+    if (warp == 0 && a.offsets) {
+        // tiles per expert, summed; offsets are taken as a rising sequence inside [0, M]
+        int carry = 0, last = 0;
+        for (int e0 = 0; e0 < a.E; e0 += 32) {
+            const int e = e0 + lane;
+            const int lo = e < a.E ? min(max(__ldg(a.offsets + e), 0), a.M) : a.M;
+            const int hi = e < a.E ? min(max(__ldg(a.offsets + e + 1), 0), a.M) : a.M;
+            // a running maximum keeps the starts from falling
+            int s = lo;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s = max(s, v);
+            }
+            s = max(s, last);
+            const int end = max(hi, s);
+            const int units = e < a.E ? (end - s + a.tile - 1) / a.tile : 0;
+            int incl = units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            if (e < a.E) {
+                cum[e] = carry + incl - units;
+                start[e] = s;
+                if (e == a.E - 1) {
+                    cum[a.E] = carry + incl;
+                    start[a.E] = end;
+                }
+            }
+            carry += __shfl_sync(0xffffffffu, incl, 31);
+            last = __shfl_sync(0xffffffffu, s, 31);
+        }
+    }
+    tc_fence_before();
+    if constexpr (CG == 2 || SPLIT) cluster_sync();
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int total = (a.offsets ? cum[a.E] : (a.M + a.tile - 1) / a.tile) * a.n_tiles;
+    const int first = (CG == 2 || SPLIT) ? blockIdx.x / (SPLIT ? ranks : CG) : blockIdx.x;
+    const int stride = (CG == 2 || SPLIT) ? gridDim.x / (SPLIT ? ranks : CG) : gridDim.x;
+    // this CTA's K blocks
+    const int kb0 = SPLIT ? static_cast<int>(static_cast<long long>(a.kblocks) * rank / ranks) : 0;
+    const int kb1 = SPLIT ? static_cast<int>(static_cast<long long>(a.kblocks) * (rank + 1) / ranks) : a.kblocks;
+
+    if (warp == kEpiWarps) {
+        // ------------------------------ TMA producer ------------------------------
+        int s = 0;
+        uint32_t lap = 0;
+        bool ok = true;
+        for (int w = first; w < total && ok && !*abort_flag; w += stride) {
+            const Tile t = tile_of(a, cum, start, w, kStep);
+            const int x_row = t.row0 + (CG == 2 ? static_cast<int>(rank) * (t.height >> 1) : 0);
+            const int n_cta = (t.n * CG + (CG == 2 ? static_cast<int>(rank) : 0));
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (lap > 0)
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], (lap - 1) & 1, a.status, kDevWaitEmpty, 2000u, a.limit));
+                if (!ok) break;
+                if (elect_one()) {
+                    uint8_t* dst = smem + s * a.stage_bytes;
+                    uint32_t bar = smem_u32(&full[s]);
+                    if (CG == 2) bar = map_to_rank(bar, 0);
+                    // the leader's barrier counts the bytes of both CTAs
+                    if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[s], CG * a.stage_bytes);
+                    if constexpr (SWIGLU) tma_5d<CG>(dst, &tmW, kb * kKB, 0, 0, n_cta * (kRows / 32), t.expert, bar);
+                    else tma_5d<CG>(dst, &tmW, kb * kKB, n_cta * kRows, t.expert, 0, 0, bar);
+                    tma_2d<CG>(dst + kABytes, &tmX, kb * kKB, x_row, bar);
+                }
+                __syncwarp();
+                if (++s == a.stages) {
+                    s = 0;
+                    ++lap;
+                }
+            }
+        }
+        if (!ok) {
+            *abort_flag = 1;
+            // copies in flight land before the CTA ends
+            if (CG == 1 || rank == 0)
+                for (int i = 0; i < a.stages; ++i) {
+                    const uint32_t n = lap + (i < s ? 1 : 0);   // times stage i was filled
+                    if (n > 0) mbar_wait_bounded(&full[i], (n - 1) & 1, a.status, kDevWaitFull, 2000u, a.limit);
+                }
+        }
+    } else if (warp == kEpiWarps + 1) {
+        // ------------------------------ MMA issuer --------------------------------
+        int s = 0, ab = 0;
+        uint32_t lap = 0, acc_lap = 0;
+        bool ok = true;
+        if (CG == 1 || rank == 0) {
+            for (int w = first; w < total && ok && !*abort_flag; w += stride) {
+                const Tile t = tile_of(a, cum, start, w, kStep);
+                const uint32_t idesc = idesc_i8(CG * kRows, t.height);
+                if (acc_lap > 0)
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_empty[ab], (acc_lap - 1) & 1, a.status, kDevWaitTmem, 2000u, a.limit));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = tmem_base + ab * (a.tmem_cols >> 1);
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[s], lap & 1, a.status, kDevWaitFull, 2000u, a.limit));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t adesc = smem_desc_sw128(smem_u32(smem + s * a.stage_bytes));
+                    const uint64_t bdesc = smem_desc_sw128(smem_u32(smem + s * a.stage_bytes + kABytes));
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < kKB / 32; ++k)
+                            mma_i8<CG>(d, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > kb0 || k != 0) ? 1u : 0u);
+                        commit<CG>(&empty[s]);
+                        if (kb == kb1 - 1) commit<CG>(&acc_full[ab]);
+                    }
+                    __syncwarp();
+                    if (++s == a.stages) {
+                        s = 0;
+                        ++lap;
+                    }
+                }
+                ab ^= 1;
+                acc_lap += ab == 0;
+            }
+            if (!ok) *abort_flag = 1;
+        }
+    } else {
+        // ------------------------------ epilogue (warps 0-7) ----------------------
+        const int q = warp & 3, half = warp >> 2;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+        int ab = 0;
+        uint32_t acc_lap = 0;
+        bool ok = true;
+        for (int w = first; w < total && ok && !*abort_flag; w += stride) {
+            const Tile t = tile_of(a, cum, start, w, kStep);
+            const int n_cta = t.n * CG + (CG == 2 ? static_cast<int>(rank) : 0);
+            // output column of this lane, and where its weight scale lies
+            int n, sb_at, n_scales;
+            if constexpr (SWIGLU) {
+                n = n_cta * (kRows / 2) + q * 16 + (lane & 15);
+                sb_at = n + (lane >= 16 ? a.N : 0);
+                n_scales = 2 * a.N;
+            } else {
+                n = n_cta * kRows + q * 32 + lane;
+                sb_at = n;
+                n_scales = a.N;
+            }
+            const bool in = n < a.N;
+            const float sb = in ? __ldg(a.sB + static_cast<size_t>(t.expert) * n_scales + sb_at) : 0.0f;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], acc_lap & 1, a.status, kDevWaitMma, 2000u, a.limit));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t src = t_lane + ab * (a.tmem_cols >> 1);
+            if constexpr (SPLIT) {
+                // partial sums to this CTA's shared memory, [token][128 channels]; the stages are free:
+                // every MMA that reads them has completed
+                int* part = reinterpret_cast<int*>(smem);
+                for (int c = half * 16; c < t.height; c += 32) {
+                    uint32_t r[16];
+                    tmem_ld16(src + c, r);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) part[(c + i) * kRows + q * 32 + lane] = static_cast<int>(r[i]);
+                }
+            } else {
+                for (int c = half * 16; c < t.rows; c += 32) {
+                    uint32_t r[16];
+                    tmem_ld16(src + c, r);
+                    const int tok = t.row0 + c;
+                    const float sa_lane = __ldg(a.sA + min(tok + (lane & 15), a.M - 1));
+                    float v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        v[i] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i])), __shfl_sync(0xffffffffu, sa_lane, i)), sb);
+                    if constexpr (SWIGLU) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            // lanes 0-15 take token i, lanes 16-31 token i + 1
+                            const float got = __shfl_xor_sync(0xffffffffu, lane < 16 ? v[i + 1] : v[i], 16);
+                            const float g = lane < 16 ? v[i] : got, u = lane < 16 ? got : v[i + 1];
+                            const int row = tok + i + (lane >> 4);
+                            if (in && c + i + (lane >> 4) < t.rows)
+                                static_cast<float*>(a.D)[static_cast<size_t>(row) * a.N + n] = g / (1.0f + expf(-g)) * u;
+                        }
+                    } else {
+                        const size_t at = static_cast<size_t>(tok) * a.N + n;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (in && c + i < t.rows) store_out(a.D, a.out_dtype, at + static_cast<size_t>(i) * a.N, v[i]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (elect_one()) {
+                    if (CG == 2) arrive_remote(map_to_rank(smem_u32(&acc_empty[ab]), 0));
+                    else mbar_arrive(&acc_empty[ab]);
+                }
+                ab ^= 1;
+                acc_lap += ab == 0;
+            }
+        }
+        if (!ok) *abort_flag = 1;
+    }
+
+    tc_fence_before();
+    __syncwarp();
+    if constexpr (SPLIT) {
+        cluster_sync();
+        // every rank adds and writes its share of the tokens: a warp a token, four channels a lane
+        const int w = first;
+        if (w < total) {
+            const Tile t = tile_of(a, cum, start, w, kStep);
+            const int n = t.n * kRows + lane * 4;
+            float sb[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sb[i] = n + i < a.N ? __ldg(a.sB + static_cast<size_t>(t.expert) * a.N + n + i) : 0.0f;
+            for (int c = static_cast<int>(rank) + static_cast<int>(ranks) * warp; c < t.rows; c += static_cast<int>(ranks) * (kThreads / 32)) {
+                const uint32_t at = smem_u32(smem) + static_cast<uint32_t>((c * kRows + lane * 4) * 4);
+                int v[4] = {0, 0, 0, 0};
+                for (uint32_t r = 0; r < ranks; ++r) {
+                    const float4 p = ld_cluster_f4(at, r);
+                    v[0] += __float_as_int(p.x);
+                    v[1] += __float_as_int(p.y);
+                    v[2] += __float_as_int(p.z);
+                    v[3] += __float_as_int(p.w);
+                }
+                const int row = t.row0 + c;
+                const float sa = __ldg(a.sA + row);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < a.N)
+                        store_out(a.D, a.out_dtype, static_cast<size_t>(row) * a.N + n + i,
+                                  __fmul_rn(__fmul_rn(static_cast<float>(v[i]), sa), sb[i]));
+            }
+        }
+        __syncwarp();
+        cluster_sync();      // nobody leaves while its sums are read
+    } else if constexpr (CG == 2) {
+        cluster_sync();
+    } else {
+        __syncthreads();
+    }
+    if (warp == kEpiWarps + 1) {
+        tc_fence_after();
+        free_tmem<CG>(tmem_base, a.tmem_cols);
+    }
+}
+
+int encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(LSG_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, one,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(LSG_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(r));
+    return LSG_OK;
+}
+
+// The weight [E, N, K] (or [E, 2 N, K], gate rows in front of up rows): boxes of 128 rows.
+int weight_map(CUtensorMap* map, const Int8Gemm& g, bool swiglu) {
+    const cuuint64_t ld = static_cast<cuuint64_t>(g.ldb);
+    if (swiglu) {
+        const cuuint64_t n = static_cast<cuuint64_t>(g.N);
+        const cuuint64_t dims[5] = {static_cast<cuuint64_t>(g.K), 16, 2, n / 16, static_cast<cuuint64_t>(g.E)};
+        const cuuint64_t strides[4] = {ld, ld * n, ld * 16, ld * n * 2};
+        const cuuint32_t box[5] = {kKB, 16, 2, 4, 1};
+        return encode(map, 5, g.B, dims, strides, box);
+    }
+    const cuuint64_t dims[5] = {static_cast<cuuint64_t>(g.K), static_cast<cuuint64_t>(g.N), static_cast<cuuint64_t>(g.E), 1, 1};
+    const cuuint64_t all = ld * static_cast<cuuint64_t>(g.N);
+    const cuuint64_t strides[4] = {ld, all, all, all};
+    const cuuint32_t box[5] = {kKB, kRows, 1, 1, 1};
+    return encode(map, 5, g.B, dims, strides, box);
+}
+
+template <int CG, bool SWIGLU, bool SPLIT>
+int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const MmaArgs& a, int grid, int cluster, cudaStream_t s) {
+    static std::atomic<bool> configured[64];
+    int dev = 0;
+    LSG_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_relaxed)) {
+        LSG_CUDA_TRY(cudaFuncSetAttribute(int8_mma_kernel<CG, SWIGLU, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_relaxed);
+    }
+    const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + 1024 + kTailBytes;
+    LSG_CUDA_TRY(launch_clusters(int8_mma_kernel<CG, SWIGLU, SPLIT>, cluster, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, s,
+                                 true, tmW, tmX, a));
+    return LSG_OK;
+}
+
+int round_up(int v, int step) { return (v + step - 1) / step * step; }
+
+}  // namespace
+
+// D = A B^T with both scales; swiglu: B is [E, 2 N, K] and D fp32 silu(gate) * up.
+int int8_mma(const Int8Gemm& g, bool swiglu, cudaStream_t s) {
+    MmaArgs a = {};
+    a.D = g.D; a.out_dtype = g.out_dtype; a.sA = g.scale_A; a.sB = g.scale_B; a.offsets = g.expert_offsets;
+    a.M = g.M; a.N = g.N; a.E = g.E; a.kblocks = (g.K + kKB - 1) / kKB;
+    a.status = device_status_word();
+    a.limit = wait_limit_cycles();
+    const int sms = sm_count();
+    const int per_cta = swiglu ? kRows / 2 : kRows;             // output columns of a CTA
+    const int cta_tiles = (g.N + per_cta - 1) / per_cta;
+    // tokens of a tile: even shares of at most 256; by the average of the experts where rows are grouped
+    const long long share = g.expert_offsets ? (static_cast<long long>(g.M) + g.E - 1) / g.E : g.M;
+    int tile;
+    if (g.expert_offsets) {
+        tile = 16;
+        while (tile < 256 && tile < 2 * share) tile *= 2;
+    } else {
+        const int units = (g.M + 255) / 256;
+        tile = round_up((g.M + units - 1) / units, 16);
+    }
+    const long long units = g.expert_offsets ? g.M / tile + static_cast<long long>(g.E < g.M ? g.E : g.M) : (g.M + tile - 1) / tile;
+    const bool pair = tile > 128 && units * cta_tiles >= sms / 2;
+    int split = 1;
+    if (!pair && !swiglu && !g.expert_offsets) {
+        static const int ways[3] = {8, 4, 2};
+        static const int slots[3] = {15, 33, 74};               // clusters of that size that are resident
+        for (int i = 0; i < 3; ++i)
+            if (units * cta_tiles <= slots[i] && a.kblocks >= 2 * ways[i]) {
+                split = ways[i];
+                break;
+            }
+    }
+    if (pair) tile = round_up(tile, 32);
+    a.tile = tile;
+    a.tn = pair ? tile / 2 : tile;
+    a.n_tiles = pair ? (cta_tiles + 1) / 2 : cta_tiles;
+    a.stage_bytes = kABytes + round_up(a.tn * kKB, 1024);
+    a.stages = kSmemMax / a.stage_bytes < kMaxStages ? kSmemMax / a.stage_bytes : kMaxStages;
+    int cols = 64;
+    while (cols < 2 * tile) cols *= 2;
+    a.tmem_cols = cols;
+    const long long tiles = units * a.n_tiles;
+    if (tiles > 0x7fffffffll) return fail(LSG_ERR_UNSUPPORTED, "int8 product: too many tiles");
+
+    CUtensorMap tmW, tmX;
+    int rc = weight_map(&tmW, g, swiglu);
+    if (rc != LSG_OK) return rc;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(g.K), static_cast<cuuint64_t>(g.M)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(g.lda)};
+    const cuuint32_t box[2] = {kKB, static_cast<cuuint32_t>(a.tn)};
+    rc = encode(&tmX, 2, g.A, dims, strides, box);
+    if (rc != LSG_OK) return rc;
+
+    if (pair) {
+        const int grid = 2 * static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+        return swiglu ? launch<2, true, false>(tmW, tmX, a, grid, 2, s) : launch<2, false, false>(tmW, tmX, a, grid, 2, s);
+    }
+    if (split > 1) return launch<1, false, true>(tmW, tmX, a, static_cast<int>(tiles) * split, split, s);
+    const int grid = static_cast<int>(tiles < sms ? tiles : sms);
+    return swiglu ? launch<1, true, false>(tmW, tmX, a, grid, 1, s) : launch<1, false, false>(tmW, tmX, a, grid, 1, s);
+}
+
+}  // namespace lsg

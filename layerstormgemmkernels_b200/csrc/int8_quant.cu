@@ -271,6 +271,7 @@ int int8_quant_rows(const void* x, long long ldx, int dtype, int8_t* codes, long
     RowQuantArgs a = {};
     a.x = x; a.ldx = ldx; a.codes = codes; a.ldq = ldq; a.scales = scales; a.K = K;
     a.inv = inv; a.top_k = top_k; a.out_rows = out_rows;
+    if (dtype == LSG_DTYPE_F32) return launch_rows<float, false>(a, rows, s);
     return dtype == LSG_DTYPE_F16 ? launch_rows<__half, false>(a, rows, s) : launch_rows<__nv_bfloat16, false>(a, rows, s);
 }
 

@@ -163,7 +163,8 @@ def test_silu_mul_far_gates(ops):
 DENSE = [(1, 1, 1), (1, 7, 16), (1, 128, 4096), (2, 1000, 1008), (3, 257, 333), (4, 64, 64), (5, 129, 2048), (8, 1024, 14336),
          (9, 300, 4096), (16, 515, 1040), (17, 4099, 512), (31, 128, 144), (33, 96, 4000), (64, 640, 2064), (65, 1, 4096),
          (77, 2048, 7168), (127, 255, 100), (128, 256, 128), (129, 257, 2304), (200, 3000, 1024), (256, 512, 4096),
-         (257, 1025, 513), (300, 4096, 1024), (511, 130, 2000), (1000, 777, 1552), (1024, 2048, 2048)]
+         (257, 1025, 513), (300, 4096, 1024), (511, 130, 2000), (1000, 777, 1552), (1024, 2048, 2048),
+         (300, 9601, 136), (513, 4099, 400), (1001, 4352, 1040), (1500, 6000, 2320)]      # CTA pairs
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "fp32"])
@@ -238,12 +239,12 @@ def offsets_of(counts):
 
 
 GROUPS = [[1], [0], [3, 0, 0, 5], [0, 0, 9], [8, 8, 8], [1] * 40, [130, 0, 1, 257, 64], [0] * 33 + [17], [300, 2],
-          [16, 17, 31, 32, 33, 0, 127, 128, 129], [2, 1, 0, 0, 7] * 13]
+          [16, 17, 31, 32, 33, 0, 127, 128, 129], [2, 1, 0, 0, 7] * 13, [700, 1, 0, 1300], [257, 900, 600]]
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp32"])
 @pytest.mark.parametrize("counts", GROUPS, ids=lambda c: f"{len(c)}x{sum(c)}")
-@pytest.mark.parametrize("N,K", [(192, 256), (77, 1040)])
+@pytest.mark.parametrize("N,K", [(192, 256), (77, 1040), (3600, 80)])
 def test_grouped_gemm(ops, counts, N, K, kind):
     E, used = len(counts), sum(counts)
     T = used + 5                                # rows behind the last expert's stay as they are
@@ -299,7 +300,7 @@ def experts(g, E, H, I):
 
 @pytest.mark.parametrize("T,E,k,H,I", [(1, 8, 2, 64, 32), (1, 128, 8, 256, 96), (9, 4, 4, 512, 144), (40, 16, 4, 128, 256),
                                        (64, 128, 8, 256, 192), (200, 8, 2, 1024, 528), (700, 8, 2, 256, 128),
-                                       (3, 2, 1, 2048, 768), (129, 3, 3, 48, 272)])
+                                       (3, 2, 1, 2048, 768), (129, 3, 3, 48, 272), (600, 3, 2, 144, 1600)])
 @pytest.mark.parametrize("kind", ["bf16", "fp32"])
 def test_moe_ffn(ops, T, E, k, H, I, kind):
     """Route, sort, experts, combine: the block gives the bits of its four steps, and the steps are
