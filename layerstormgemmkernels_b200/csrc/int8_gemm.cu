@@ -13,43 +13,6 @@ namespace lsg {
 
 namespace {
 
-// One warp per output column and unit of up to eight token rows, lanes striding over 16-byte pieces
-// of the weight row.
-__global__ void __launch_bounds__(256)
-int8_dot_kernel(const Int8Gemm a) {
-    pdl_launch_dependents();
-    pdl_wait_prior();
-    const int lane = threadIdx.x & 31;
-    const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int r0 = blockIdx.y * 8, rows = min(8, a.M - r0);
-    if (n >= a.N) return;
-    const int8_t* w = a.B + static_cast<long long>(n) * a.ldb;
-    int acc[8];
-#pragma unroll
-    for (int m = 0; m < 8; ++m) acc[m] = 0;
-    for (int k = lane * 16; k < a.K; k += 512) {
-        const int4 wv = __ldg(reinterpret_cast<const int4*>(w + k));
-#pragma unroll
-        for (int m = 0; m < 8; ++m) {
-            if (m < rows) {
-                int4 xv = *reinterpret_cast<const int4*>(a.A + (r0 + m) * a.lda + k);
-                if (k + 16 > a.K) xv = keep_bytes(xv, a.K - k);
-                acc[m] = dp4a_ss(wv.x, xv.x, dp4a_ss(wv.y, xv.y, dp4a_ss(wv.z, xv.z, dp4a_ss(wv.w, xv.w, acc[m]))));
-            }
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < 8; ++m) acc[m] = __reduce_add_sync(0xffffffffu, acc[m]);
-    if (lane < rows) {
-        int v = acc[0];
-#pragma unroll
-        for (int m = 1; m < 8; ++m) v = lane == m ? acc[m] : v;
-        const int row = r0 + lane;
-        store_out(a.D, a.out_dtype, static_cast<size_t>(row) * a.N + n,
-                  __fmul_rn(__fmul_rn(static_cast<float>(v), a.scale_A[row]), a.scale_B[n]));
-    }
-}
-
 int check(const char* op, int N, int K, const void* A, long long lda, const void* B, long long ldb, const void* D, int dt) {
     if (dt != LSG_DTYPE_BF16 && dt != LSG_DTYPE_F16 && dt != LSG_DTYPE_F32)
         return fail(LSG_ERR_UNSUPPORTED, "%s: output dtype must be bf16, fp16 or f32", op);
@@ -67,9 +30,8 @@ int check(const char* op, int N, int K, const void* A, long long lda, const void
 }  // namespace
 
 int int8_gemm(const Int8Gemm& a, cudaStream_t s) {
-    if (a.M > 8 || a.expert_offsets) return int8_mma(a, false, s);
-    LSG_CUDA_TRY(launch_kernel(int8_dot_kernel, dim3((a.N + 7) / 8, (a.M + 7) / 8), dim3(256), 0, s, true, a));
-    return LSG_OK;
+    if (!a.expert_offsets && int8_gemv_takes(a.M, a.K)) return int8_gemv(a, -1, s);
+    return int8_mma(a, false, s);
 }
 
 }  // namespace lsg
@@ -98,7 +60,7 @@ extern "C" int lsg_int8_gemm(const lsg_int8_gemm_params* p, void* stream) {
 }
 
 extern "C" size_t lsg_int8_gemm_from_bf16_workspace_bytes(int M, int K) {
-    if (M <= 0 || K <= 0) return 0;
+    if (M <= 0 || K <= 0 || int8_gemv_takes(M, K)) return 0;
     return a256(static_cast<size_t>(M) * pad16(K)) + a256(static_cast<size_t>(M) * 4);
 }
 
@@ -109,28 +71,31 @@ extern "C" int lsg_int8_gemm_from_bf16(const lsg_int8_gemm_params* p, int input_
     if (input_dtype != LSG_DTYPE_BF16 && input_dtype != LSG_DTYPE_F16)
         return fail(LSG_ERR_UNSUPPORTED, "int8_gemm_from_bf16: input must be bf16 or fp16");
     if (p->M == 0 || p->N == 0) return LSG_OK;
-    // the activations may lie anywhere: their codes, in the workspace, are what the product reads
-    uint8_t* codes = static_cast<uint8_t*>(workspace);
-    const long long ldq = pad16(p->K);
-    const size_t need = lsg_int8_gemm_from_bf16_workspace_bytes(p->M, p->K);
-    if (p->K >= 1 && (!workspace || workspace_bytes < need))
-        return fail(LSG_ERR_WORKSPACE, "int8_gemm_from_bf16: workspace too small (have %zu, need %zu)",
-                    workspace ? workspace_bytes : size_t(0), need);
-    if (reinterpret_cast<uintptr_t>(workspace) & 255)
-        return fail(LSG_ERR_ALIGNMENT, "int8_gemm_from_bf16: workspace must be 256-byte aligned");
-    int rc = check("int8_gemm_from_bf16", p->N, p->K, codes, ldq, p->B, p->ldb, p->D, p->output_dtype);
+    if (p->lda < p->K) return fail(LSG_ERR_INVALID, "int8_gemm_from_bf16: a row stride is smaller than K");
+    // the activations may lie anywhere: the product reads their codes
+    const long long ldq = pad16(p->K > 0 ? p->K : 0);
+    int rc = check("int8_gemm_from_bf16", p->N, p->K, p->B, ldq, p->B, p->ldb, p->D, p->output_dtype);
     if (rc != LSG_OK) return rc;
     if (!p->A || !p->scale_B) return fail(LSG_ERR_INVALID, "int8_gemm_from_bf16: null pointer");
-    if (p->lda < p->K) return fail(LSG_ERR_INVALID, "int8_gemm_from_bf16: a row stride is smaller than K");
-    float* scales = reinterpret_cast<float*>(codes + a256(static_cast<size_t>(p->M) * ldq));
+    const size_t need = lsg_int8_gemm_from_bf16_workspace_bytes(p->M, p->K);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(LSG_ERR_WORKSPACE, "int8_gemm_from_bf16: workspace too small (have %zu, need %zu)",
+                    workspace ? workspace_bytes : size_t(0), need);
+    if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255))
+        return fail(LSG_ERR_ALIGNMENT, "int8_gemm_from_bf16: workspace must be 256-byte aligned");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     Int8Gemm a = {};
-    a.A = reinterpret_cast<const int8_t*>(codes); a.lda = ldq;
     a.B = static_cast<const int8_t*>(p->B); a.ldb = p->ldb;
-    a.D = p->D; a.out_dtype = p->output_dtype;
-    a.scale_A = scales; a.scale_B = p->scale_B;
+    a.D = p->D; a.out_dtype = p->output_dtype; a.scale_B = p->scale_B;
     a.M = p->M; a.N = p->N; a.K = p->K; a.E = 1;
-    rc = int8_quant_rows(p->A, p->lda, input_dtype, reinterpret_cast<int8_t*>(codes), ldq, scales, p->M, p->K, nullptr, 1, 0, s);
+    if (need == 0) {
+        a.A = static_cast<const int8_t*>(p->A); a.lda = p->lda;
+        return int8_gemv(a, input_dtype, s);
+    }
+    int8_t* codes = static_cast<int8_t*>(workspace);
+    float* scales = reinterpret_cast<float*>(codes + a256(static_cast<size_t>(p->M) * ldq));
+    a.A = codes; a.lda = ldq; a.scale_A = scales;
+    rc = int8_quant_rows(p->A, p->lda, input_dtype, codes, ldq, scales, p->M, p->K, nullptr, 1, 0, s);
     if (rc != LSG_OK) return rc;
     return int8_gemm(a, s);
 }

@@ -21,12 +21,11 @@
 // 16384 values, are read twice, value by value.
 #include "common.cuh"
 #include "host.h"
+#include "int8.cuh"
 
 namespace lsg {
 
 namespace {
-
-constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer, in the low byte
 
 struct RowQuantArgs {
     const void* x;        // [rows, K], row stride ldx values (gate of silu_mul)
@@ -39,46 +38,6 @@ struct RowQuantArgs {
     const int32_t* inv;   // scatter: [rows * top_k] destination rows; null = row to row
     int top_k;
     int out_rows;
-};
-
-template <typename T> struct Elem;
-template <> struct Elem<__nv_bfloat16> {
-    static constexpr int kVecs = 1;   // 16-byte loads for eight values
-    static __device__ __forceinline__ float get(const void* p, size_t i) {
-        return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-    }
-    static __device__ __forceinline__ void unpack(const uint4* v, float (&f)[8]) {
-        const uint32_t w[4] = {v->x, v->y, v->z, v->w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-};
-template <> struct Elem<__half> {
-    static constexpr int kVecs = 1;
-    static __device__ __forceinline__ float get(const void* p, size_t i) {
-        return __half2float(static_cast<const __half*>(p)[i]);
-    }
-    static __device__ __forceinline__ void unpack(const uint4* v, float (&f)[8]) {
-        const uint32_t w[4] = {v->x, v->y, v->z, v->w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            f[2 * i] = h.x;
-            f[2 * i + 1] = h.y;
-        }
-    }
-};
-template <> struct Elem<float> {
-    static constexpr int kVecs = 2;
-    static __device__ __forceinline__ float get(const void* p, size_t i) { return static_cast<const float*>(p)[i]; }
-    static __device__ __forceinline__ void unpack(const uint4* v, float (&f)[8]) {
-        const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
-    }
 };
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
@@ -95,40 +54,13 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t m) {
     return __reduce_max_sync(0xffffffffu, lane < n ? part[lane] : 0u);
 }
 
-// The row's constants: y = x * mul is 127 x, moved by a power of two where 127 a or 1 / a would leave
-// the range of fp32; den = a moved alike.
-struct RowScale {
-    float scale, mul, den, rcp;
-    bool dead;   // all zero, or not finite: codes are 0
-};
-__device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
-    RowScale r;
-    const float a = __uint_as_float(amax_bits);
-    const bool finite = amax_bits < 0x7F800000u;
-    r.dead = !finite || amax_bits == 0;
-    r.scale = finite ? a / 127.0f : __uint_as_float(0x7FC00000u);
-    const float s = a > 0x1p100f ? 0x1p-64f : (a < 0x1p-100f ? 0x1p64f : 1.0f);
-    r.mul = 127.0f * s;
-    r.den = a * s;
-    r.rcp = r.dead ? 0.0f : 1.0f / r.den;
-    return r;
-}
-__device__ __forceinline__ uint32_t code_bits(float x, const RowScale& r) {
-    const float y = x * r.mul;
-    const float t = y * r.rcp;
-    return __float_as_uint(fmaf(fmaf(-t, r.den, y), r.rcp, t) + kMagic);
-}
-__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
-
 // V pieces of eight values per thread.
 template <typename T, bool SILU, int V>
 __global__ void __launch_bounds__(V == 4 ? 512 : 1024)
 quant_rows_kernel(const RowQuantArgs a) {
     pdl_launch_dependents();
     pdl_wait_prior();
-    constexpr int L = Elem<T>::kVecs;
+    constexpr int L = Int8In<T>::kVecs;
     const long long row = blockIdx.x;
     const int nvec = a.K >> 3;
     const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ldx);
@@ -153,8 +85,8 @@ quant_rows_kernel(const RowQuantArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float g[8], u[8];
-            Elem<T>::unpack(raw[i], g);
-            Elem<T>::unpack(ur[i], u);
+            Int8In<T>::unpack(raw[i], g);
+            Int8In<T>::unpack(ur[i], u);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 h[i][j] = silu_mul(g[j], u[j]);
@@ -165,7 +97,7 @@ quant_rows_kernel(const RowQuantArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float f[8];
-            Elem<T>::unpack(raw[i], f);
+            Int8In<T>::unpack(raw[i], f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(f[j])));
         }
@@ -179,7 +111,7 @@ quant_rows_kernel(const RowQuantArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = h[i][j];
         } else {
-            Elem<T>::unpack(raw[i], f);
+            Int8In<T>::unpack(raw[i], f);
         }
         uint32_t q[8];
 #pragma unroll
@@ -209,8 +141,8 @@ quant_rows_any_kernel(const RowQuantArgs a) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* up = SILU ? static_cast<const T*>(a.up) + row * a.ldu : nullptr;
     auto value = [&](int k) {
-        const float g = Elem<T>::get(x, k);
-        return SILU ? silu_mul(g, Elem<T>::get(up, k)) : g;
+        const float g = Int8In<T>::get(x, k);
+        return SILU ? silu_mul(g, Int8In<T>::get(up, k)) : g;
     };
     uint32_t m = 0;
     for (int k = threadIdx.x; k < a.K; k += 256) m = max(m, __float_as_uint(fabsf(value(k))));

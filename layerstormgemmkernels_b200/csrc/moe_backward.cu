@@ -32,29 +32,49 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
 // P values as one load or store: 16 bytes, or a single value where rows are not whole pieces.
 template <typename T, int P> struct alignas(sizeof(T) * P) Piece { T v[P]; };
 
-// out[t] = sum over slots, in order, of (w ? w[t,s] : 1) * y[inv[t,s]].
-template <typename T, int P>
+// The rows of a token's slots, and their loads of piece c all under way at once; -1: no row.
+template <int K>
+__device__ __forceinline__ void slot_rows(const int32_t* inv, size_t at, int rows, int k, int (&row)[K]) {
+#pragma unroll
+    for (int s = 0; s < K; ++s) {
+        row[s] = s < k ? __ldg(inv + at + s) : -1;
+        if (row[s] >= rows) row[s] = -1;
+    }
+}
+template <typename T, int P, int K>
+__device__ __forceinline__ void load_slots(const Piece<T, P>* y, const int (&row)[K], int per_row, int c, Piece<T, P> (&v)[K]) {
+#pragma unroll
+    for (int s = 0; s < K; ++s) {
+        if (row[s] >= 0) v[s] = y[static_cast<size_t>(row[s]) * per_row + c];
+        else
+#pragma unroll
+            for (int i = 0; i < P; ++i) v[s].v[i] = from_f<T>(0.0f);
+    }
+}
+
+// out[t] = sum over slots, in order, of (w ? w[t,s] : 1) * y[inv[t,s]]; k <= K.
+template <typename T, int P, int K>
 __global__ void __launch_bounds__(256)
 moe_sum_slots_kernel(const Piece<T, P>* __restrict__ y, const int32_t* __restrict__ inv, const float* __restrict__ w,
                      int rows, int k, int per_row, Piece<T, P>* __restrict__ out) {
     pdl_launch_dependents();
     pdl_wait_prior();
     const size_t t = blockIdx.x;
+    int row[K];
+    float ws[K];
+    slot_rows(inv, t * k, rows, k, row);
+#pragma unroll
+    for (int s = 0; s < K; ++s) ws[s] = row[s] < 0 ? 0.0f : (w ? __ldg(w + t * k + s) : 1.0f);
     for (int c = threadIdx.x; c < per_row; c += blockDim.x) {
-        float acc[P];
+        Piece<T, P> v[K], o;
+        load_slots(y, row, per_row, c, v);
 #pragma unroll
-        for (int i = 0; i < P; ++i) acc[i] = 0.0f;
-        for (int s = 0; s < k; ++s) {
-            const int row = __ldg(inv + t * k + s);
-            if (row < 0 || row >= rows) continue;
-            const float ws = w ? __ldg(w + t * k + s) : 1.0f;
-            const Piece<T, P> p = y[static_cast<size_t>(row) * per_row + c];
+        for (int i = 0; i < P; ++i) {
+            float acc = 0.0f;
 #pragma unroll
-            for (int i = 0; i < P; ++i) acc[i] = fmaf(ws, to_f(p.v[i]), acc[i]);
+            for (int s = 0; s < K; ++s) acc = fmaf(ws[s], to_f(v[s].v[i]), acc);
+            o.v[i] = from_f<T>(acc);
         }
-        Piece<T, P> o;
-#pragma unroll
-        for (int i = 0; i < P; ++i) o.v[i] = from_f<T>(acc[i]);
         out[t * per_row + c] = o;
     }
 }
@@ -74,7 +94,7 @@ moe_copy_rows_kernel(const Piece<T, P>* __restrict__ x, const int32_t* __restric
 }
 
 // One CTA per token: grad_out[t] is read once for all its slots.
-template <typename T, int P>
+template <typename T, int P, int K>
 __global__ void __launch_bounds__(256)
 moe_unpermute_backward_kernel(const Piece<T, P>* __restrict__ grad_out, const Piece<T, P>* __restrict__ y,
                               const int32_t* __restrict__ inv, const float* __restrict__ w,
@@ -82,36 +102,37 @@ moe_unpermute_backward_kernel(const Piece<T, P>* __restrict__ grad_out, const Pi
                               Piece<T, P>* __restrict__ grad_y, float* __restrict__ grad_w) {
     pdl_launch_dependents();
     pdl_wait_prior();
-    __shared__ float part[8][kMaxSlots];
+    __shared__ float part[8][K];
     const size_t t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float dot[kMaxSlots];
+    int row[K];
+    float ws[K], dot[K];
+    slot_rows(inv, t * k, rows, k, row);
 #pragma unroll
-    for (int s = 0; s < kMaxSlots; ++s) dot[s] = 0.0f;
+    for (int s = 0; s < K; ++s) {
+        ws[s] = s < k ? __ldg(w + t * k + s) : 0.0f;
+        dot[s] = 0.0f;
+    }
     for (int c = threadIdx.x; c < per_row; c += blockDim.x) {
+        Piece<T, P> v[K];
         const Piece<T, P> g = grad_out[t * per_row + c];
+        load_slots(y, row, per_row, c, v);
 #pragma unroll
-        for (int s = 0; s < kMaxSlots; ++s) {
-            if (s < k) {
-                const int row = __ldg(inv + t * k + s);
-                if (row >= 0 && row < rows) {
-                    const float ws = __ldg(w + t * k + s);
-                    const size_t at = static_cast<size_t>(row) * per_row + c;
-                    const Piece<T, P> v = y[at];
-                    Piece<T, P> o;
+        for (int s = 0; s < K; ++s) {
+            if (row[s] >= 0) {
+                Piece<T, P> o;
 #pragma unroll
-                    for (int i = 0; i < P; ++i) {
-                        const float gf = to_f(g.v[i]);
-                        dot[s] = fmaf(to_f(v.v[i]), gf, dot[s]);
-                        o.v[i] = from_f<T>(ws * gf);
-                    }
-                    grad_y[at] = o;
+                for (int i = 0; i < P; ++i) {
+                    const float gf = to_f(g.v[i]);
+                    dot[s] = fmaf(to_f(v[s].v[i]), gf, dot[s]);
+                    o.v[i] = from_f<T>(ws[s] * gf);
                 }
+                grad_y[static_cast<size_t>(row[s]) * per_row + c] = o;
             }
         }
     }
 #pragma unroll
-    for (int s = 0; s < kMaxSlots; ++s) {
+    for (int s = 0; s < K; ++s) {
         if (s < k) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) dot[s] += __shfl_xor_sync(0xffffffffu, dot[s], o);
@@ -126,15 +147,13 @@ moe_unpermute_backward_kernel(const Piece<T, P>* __restrict__ grad_out, const Pi
     }
     // rows behind the last expert's belong to no pair
     if (rows_used) {
-        const int used = __ldg(rows_used);
-        for (int s = 0; s < k; ++s) {
-            const size_t row = t * k + s;
-            if (row >= static_cast<size_t>(max(used, 0)) && row < static_cast<size_t>(rows)) {
-                Piece<T, P> z;
+        const size_t used = static_cast<size_t>(max(__ldg(rows_used), 0));
+        const size_t end = min((t + 1) * k, static_cast<size_t>(rows));
+        for (size_t r = max(t * k, used); r < end; ++r) {
+            Piece<T, P> z;
 #pragma unroll
-                for (int i = 0; i < P; ++i) z.v[i] = from_f<T>(0.0f);
-                for (int c = threadIdx.x; c < per_row; c += blockDim.x) grad_y[row * per_row + c] = z;
-            }
+            for (int i = 0; i < P; ++i) z.v[i] = from_f<T>(0.0f);
+            for (int c = threadIdx.x; c < per_row; c += blockDim.x) grad_y[r * per_row + c] = z;
         }
     }
 }
@@ -172,18 +191,34 @@ int threads_for(int per_row) { return per_row >= 256 ? 256 : (per_row < 1 ? 32 :
 
 bool whole_pieces(int H, size_t size, uintptr_t at) { return (static_cast<size_t>(H) * size) % 16 == 0 && (at & 15) == 0; }
 
+template <typename T, int P, int K>
+int launch_sum(const void* y, const int32_t* inv, const float* w, int rows, int tokens, int k, int per_row, void* out, cudaStream_t s) {
+    LSG_CUDA_TRY(launch_kernel(moe_sum_slots_kernel<T, P, K>, dim3(static_cast<unsigned>(tokens)), dim3(threads_for(per_row)), 0, s,
+                               true, static_cast<const Piece<T, P>*>(y), inv, w, rows, k, per_row, static_cast<Piece<T, P>*>(out)));
+    return LSG_OK;
+}
+template <typename T, int P, int K>
+int launch_unpermute_backward(const void* grad_out, const void* y, const int32_t* inv, const float* w, const int32_t* used, int rows,
+                              int tokens, int k, int per_row, void* grad_y, float* grad_w, cudaStream_t s) {
+    LSG_CUDA_TRY(launch_kernel(moe_unpermute_backward_kernel<T, P, K>, dim3(static_cast<unsigned>(tokens)),
+                               dim3(threads_for(per_row)), 0, s, true, static_cast<const Piece<T, P>*>(grad_out),
+                               static_cast<const Piece<T, P>*>(y), inv, w, used, rows, k, per_row,
+                               static_cast<Piece<T, P>*>(grad_y), grad_w));
+    return LSG_OK;
+}
+
+// K: slots held in registers, the next of 2, 4, 8, 16.
+#define LSG_BY_SLOTS(fn, P, ...)                                                                       \
+    (k <= 2 ? fn<T, P, 2>(__VA_ARGS__)                                                                 \
+            : (k <= 4 ? fn<T, P, 4>(__VA_ARGS__) : (k <= 8 ? fn<T, P, 8>(__VA_ARGS__) : fn<T, P, 16>(__VA_ARGS__))))
+
 template <typename T>
 int sum_slots(const void* y, const int32_t* inv, const float* w, int rows, int tokens, int k, int H, void* out,
               cudaStream_t s) {
     constexpr int P = 16 / sizeof(T);
-    const dim3 grid(static_cast<unsigned>(tokens));
     if (whole_pieces(H, sizeof(T), reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)))
-        LSG_CUDA_TRY(launch_kernel(moe_sum_slots_kernel<T, P>, grid, dim3(threads_for(H / P)), 0, s, true,
-                                   static_cast<const Piece<T, P>*>(y), inv, w, rows, k, H / P, static_cast<Piece<T, P>*>(out)));
-    else
-        LSG_CUDA_TRY(launch_kernel(moe_sum_slots_kernel<T, 1>, grid, dim3(threads_for(H)), 0, s, true,
-                                   static_cast<const Piece<T, 1>*>(y), inv, w, rows, k, H, static_cast<Piece<T, 1>*>(out)));
-    return LSG_OK;
+        return LSG_BY_SLOTS(launch_sum, P, y, inv, w, rows, tokens, k, H / P, out, s);
+    return LSG_BY_SLOTS(launch_sum, 1, y, inv, w, rows, tokens, k, H, out, s);
 }
 
 template <typename T>
@@ -203,16 +238,9 @@ template <typename T>
 int unpermute_backward(const void* grad_out, const void* y, const int32_t* inv, const float* w, const int32_t* used, int rows,
                        int tokens, int k, int H, void* grad_y, float* grad_w, cudaStream_t s) {
     constexpr int P = 16 / sizeof(T);
-    const dim3 grid(static_cast<unsigned>(tokens));
     if (whole_pieces(H, sizeof(T), reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(grad_y)))
-        LSG_CUDA_TRY(launch_kernel(moe_unpermute_backward_kernel<T, P>, grid, dim3(threads_for(H / P)), 0, s, true,
-                                   static_cast<const Piece<T, P>*>(grad_out), static_cast<const Piece<T, P>*>(y), inv, w, used,
-                                   rows, k, H / P, static_cast<Piece<T, P>*>(grad_y), grad_w));
-    else
-        LSG_CUDA_TRY(launch_kernel(moe_unpermute_backward_kernel<T, 1>, grid, dim3(threads_for(H)), 0, s, true,
-                                   static_cast<const Piece<T, 1>*>(grad_out), static_cast<const Piece<T, 1>*>(y), inv, w, used,
-                                   rows, k, H, static_cast<Piece<T, 1>*>(grad_y), grad_w));
-    return LSG_OK;
+        return LSG_BY_SLOTS(launch_unpermute_backward, P, grad_out, y, inv, w, used, rows, tokens, k, H / P, grad_y, grad_w, s);
+    return LSG_BY_SLOTS(launch_unpermute_backward, 1, grad_out, y, inv, w, used, rows, tokens, k, H, grad_y, grad_w, s);
 }
 
 int check_moe(const char* op, int dtype, int tokens, int k, int H) {

@@ -38,11 +38,13 @@ def test_gemm_nothing_to_do(capi):
 
 
 def test_gemm_from_bf16_refusals(capi):
-    need = capi.lib.lsg_int8_gemm_from_bf16_workspace_bytes(4, 64)
-    assert need == 512 and capi.lib.lsg_int8_gemm_from_bf16_workspace_bytes(0, 64) == 0
-    assert capi.lib.lsg_int8_gemm_from_bf16_workspace_bytes(3, 100) == 512 + 256
+    need = capi.lib.lsg_int8_gemm_from_bf16_workspace_bytes(40, 64)
+    assert need == 40 * 64 + 256 and capi.lib.lsg_int8_gemm_from_bf16_workspace_bytes(0, 64) == 0
+    assert capi.lib.lsg_int8_gemm_from_bf16_workspace_bytes(30, 100) == 3584 + 256   # rows of 112 bytes
+    assert capi.lib.lsg_int8_gemm_from_bf16_workspace_bytes(3, 100) == 0             # quantized inside the mat-vec
 
-    def call(dtype=0, ws=P, size=need, **kw):
+    def call(dtype=0, ws=P, size=need, M=40, **kw):
+        kw["M"] = M
         capi.check(capi.lib.lsg_int8_gemm_from_bf16(ctypes.byref(gemm(capi, **kw)), dtype, ws, size, None))
     for kw, error, text in ((dict(dtype=1), RuntimeError, "bf16 or fp16"), (dict(ws=None), RuntimeError, "workspace"),
                             (dict(size=need - 1), RuntimeError, "workspace"), (dict(ws=P + 16), RuntimeError, "256-byte"),
