@@ -52,10 +52,19 @@ __device__ __forceinline__ void store_out(void* D, int dtype, size_t at, float v
     else static_cast<__nv_bfloat16*>(D)[at] = __float2bfloat16_rn(v);
 }
 
+// Magnitudes order like their bit patterns, infinity and NaN on top.
+__device__ __forceinline__ uint32_t max_halves(uint32_t m, const uint4* v) {
+    const uint32_t w[4] = {v->x, v->y, v->z, v->w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    return m;
+}
+
 // Values of the quantizers' input types, eight at a time from 16-byte loads.
 template <typename T> struct Int8In;
 template <> struct Int8In<__nv_bfloat16> {
     static constexpr int kVecs = 1;   // 16-byte loads for eight values
+    static constexpr bool kOneFma = true;
     static __device__ __forceinline__ float get(const void* p, size_t i) {
         return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
     }
@@ -67,9 +76,13 @@ template <> struct Int8In<__nv_bfloat16> {
             f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
         }
     }
+    // running maximum of the magnitudes' bit patterns, two at a time, and its fp32 form
+    static __device__ __forceinline__ uint32_t top(uint32_t m, const uint4* v) { return max_halves(m, v); }
+    static __device__ __forceinline__ uint32_t top_bits(uint32_t m) { return max(m & 0xFFFFu, m >> 16) << 16; }
 };
 template <> struct Int8In<__half> {
     static constexpr int kVecs = 1;
+    static constexpr bool kOneFma = false;
     static __device__ __forceinline__ float get(const void* p, size_t i) {
         return __half2float(static_cast<const __half*>(p)[i]);
     }
@@ -82,44 +95,84 @@ template <> struct Int8In<__half> {
             f[2 * i + 1] = h.y;
         }
     }
+    static __device__ __forceinline__ uint32_t top(uint32_t m, const uint4* v) { return max_halves(m, v); }
+    static __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
+        const __half_raw h = {static_cast<unsigned short>(max(m & 0xFFFFu, m >> 16))};
+        return __float_as_uint(__half2float(h));
+    }
 };
 template <> struct Int8In<float> {
     static constexpr int kVecs = 2;
+    static constexpr bool kOneFma = true;
     static __device__ __forceinline__ float get(const void* p, size_t i) { return static_cast<const float*>(p)[i]; }
     static __device__ __forceinline__ void unpack(const uint4* v, float (&f)[8]) {
         const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
     }
+    static __device__ __forceinline__ uint32_t top(uint32_t m, const uint4* v) {
+        const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+        return m;
+    }
+    static __device__ __forceinline__ uint32_t top_bits(uint32_t m) { return m; }
 };
 
 constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer, in the low byte
 
-// The row's constants: y = x * mul is 127 x, moved by a power of two where 127 a or 1 / a would leave
-// the range of fp32; den = a moved alike.
+// The row's constants.  c is 127 / a rounded up: one fma(x, c, kMagic) rounds the exact x c to the
+// nearest integer, and for bf16 that is the integer of 127 x / a: a quotient that is not half-way lies
+// at least 2^-(9 + d) from half-way (d: by how many powers of two a exceeds x) and x c at most
+// 2^-(15 + d) from the quotient; a quotient can be half-way only when a is 127 times a power of two,
+// where c is exact, or when it is 63.5 (127 is prime), where c on the upper side takes it to 64, the
+// even neighbour.  fp16 has other half-way cases (a = 381, x = 1.5): it forms the correctly rounded
+// quotient from the exact 127 x instead.  Rows below 2^-100 are moved up so that c stays finite.
 struct RowScale {
-    float scale, mul, den, rcp;
+    float scale, c, den, rcp;
     bool dead;   // all zero, or not finite: codes are 0
+    bool tiny;
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
     RowScale r;
     const float a = __uint_as_float(amax_bits);
     const bool finite = amax_bits < 0x7F800000u;
     r.dead = !finite || amax_bits == 0;
+    r.tiny = a < 0x1p-100f;
     r.scale = finite ? a / 127.0f : __uint_as_float(0x7FC00000u);
-    const float s = a > 0x1p100f ? 0x1p-64f : (a < 0x1p-100f ? 0x1p64f : 1.0f);
-    r.mul = 127.0f * s;
-    r.den = a * s;
-    r.rcp = r.dead ? 0.0f : 1.0f / r.den;
+    r.den = r.dead ? 1.0f : (r.tiny ? a * 0x1p64f : a);
+    r.c = __fdiv_ru(127.0f, r.den);
+    r.rcp = 1.0f / r.den;
     return r;
 }
+template <typename T>
 __device__ __forceinline__ uint32_t code_bits(float x, const RowScale& r) {
-    const float y = x * r.mul;
-    const float t = y * r.rcp;
-    return __float_as_uint(fmaf(fmaf(-t, r.den, y), r.rcp, t) + kMagic);
+    if constexpr (!Int8In<T>::kOneFma) {
+        const float y = x * 127.0f;
+        const float t = y * r.rcp;
+        return __float_as_uint(fmaf(fmaf(-t, r.den, y), r.rcp, t) + kMagic);
+    } else {
+        return __float_as_uint(fmaf(x, r.c, kMagic));
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint8_t code1(float x, const RowScale& r) {
+    return r.dead ? 0 : static_cast<uint8_t>(code_bits<T>(r.tiny ? x * 0x1p64f : x, r) & 0xFFu);
 }
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+template <typename T>
+__device__ __forceinline__ uint2 code8(float (&f)[8], const RowScale& r) {
+    if (r.dead) return make_uint2(0, 0);
+    if (r.tiny) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= 0x1p64f;
+    }
+    uint32_t q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = code_bits<T>(f[j], r);
+    return make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
 }
 
 #endif  // __CUDACC__

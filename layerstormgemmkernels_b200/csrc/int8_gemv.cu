@@ -37,11 +37,9 @@ __device__ __forceinline__ void quantize_rows(const Int8Gemm& a, int8_t* codes, 
             if (whole) {
                 for (int v = threadIdx.x; v < a.K / 8; v += kGemvThreads) {
                     const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row) + v);
-                    float f[8];
-                    Int8In<T>::unpack(&raw, f);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(fabsf(f[j])));
+                    top = Int8In<T>::top(top, &raw);
                 }
+                top = Int8In<T>::top_bits(top);
             } else {
                 for (int k = threadIdx.x; k < a.K; k += kGemvThreads) top = max(top, __float_as_uint(fabsf(Int8In<T>::get(row, k))));
             }
@@ -64,17 +62,13 @@ __device__ __forceinline__ void quantize_rows(const Int8Gemm& a, int8_t* codes, 
             for (int v = threadIdx.x; v < a.K / 8; v += kGemvThreads) {
                 const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row) + v);
                 float f[8];
-                uint32_t c[8];
                 Int8In<T>::unpack(&raw, f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) c[j] = code_bits(f[j], r);
-                reinterpret_cast<uint2*>(q)[v] =
-                    r.dead ? make_uint2(0, 0) : make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+                reinterpret_cast<uint2*>(q)[v] = code8<T>(f, r);
             }
             if (threadIdx.x == 0 && (a.K & 8)) reinterpret_cast<uint2*>(q)[a.K / 8] = make_uint2(0, 0);
         } else {
             for (int k = threadIdx.x; k < ldq; k += kGemvThreads)
-                q[k] = k < a.K && !r.dead ? static_cast<int8_t>(code_bits(Int8In<T>::get(row, k), r) & 0xFFu) : int8_t(0);
+                q[k] = k < a.K ? static_cast<int8_t>(code1<T>(Int8In<T>::get(row, k), r)) : int8_t(0);
         }
     }
 }

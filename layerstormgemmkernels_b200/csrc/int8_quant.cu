@@ -6,12 +6,8 @@
 // An all-zero row gets scale 0 and codes 0; a row with an infinity or a NaN gets scale NaN and
 // codes 0, so that whatever it is multiplied with is NaN and not a number that looks right.
 //
-// The code is the rounding of the exact quotient for bf16 and fp16 inputs: 127 x has at most 18
-// bits and is exact in fp32, fma(fma(-t, a, y), 1/a, t) is the correctly rounded quotient y / a,
-// and a quotient of two 11-bit numbers that is not half-way between two integers is at least 2^-20
-// (relative to the larger of the integers' spacing and itself, 2^-12 at 127) away from half-way,
-// more than fp32 moves it.  fl(x / scale) would not do: the scale is rounded, so quotients next to
-// a half-way point fall on either side of it.
+// The codes are those of the exact quotient (row_scale says how).  fl(x / scale) would not do: the
+// scale is rounded, so quotients next to a half-way point fall on either side of it.
 //
 // The activation silu(g) * u of silu_mul stays in fp32 up to its code (rounding it to bf16 first
 // moves one value in fifteen by a code).
@@ -56,15 +52,15 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t m) {
 
 // V pieces of eight values per thread.
 template <typename T, bool SILU, int V>
-__global__ void __launch_bounds__(V == 4 ? 512 : 1024)
+__global__ void __launch_bounds__(V <= 2 ? 1024 : 512)
 quant_rows_kernel(const RowQuantArgs a) {
     pdl_launch_dependents();
     pdl_wait_prior();
-    constexpr int L = Int8In<T>::kVecs;
+    using In = Int8In<T>;
+    constexpr int L = In::kVecs;
     const long long row = blockIdx.x;
     const int nvec = a.K >> 3;
     const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ldx);
-    const uint4* up = SILU ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.up) + row * a.ldu) : nullptr;
     uint4 raw[V][L];
     float h[SILU ? V : 1][8];
     uint32_t m = 0;
@@ -75,6 +71,7 @@ quant_rows_kernel(const RowQuantArgs a) {
         for (int l = 0; l < L; ++l) raw[i][l] = v < nvec ? __ldg(x + v * L + l) : make_uint4(0, 0, 0, 0);
     }
     if constexpr (SILU) {
+        const uint4* up = reinterpret_cast<const uint4*>(static_cast<const T*>(a.up) + row * a.ldu);
         uint4 ur[V][L];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -85,8 +82,8 @@ quant_rows_kernel(const RowQuantArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float g[8], u[8];
-            Int8In<T>::unpack(raw[i], g);
-            Int8In<T>::unpack(ur[i], u);
+            In::unpack(raw[i], g);
+            In::unpack(ur[i], u);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 h[i][j] = silu_mul(g[j], u[j]);
@@ -95,28 +92,20 @@ quant_rows_kernel(const RowQuantArgs a) {
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float f[8];
-            Int8In<T>::unpack(raw[i], f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(f[j])));
-        }
+        for (int i = 0; i < V; ++i) m = In::top(m, raw[i]);
+        m = In::top_bits(m);
     }
     const RowScale r = row_scale(block_max_bits(m));
     uint2 out[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        float f[8];
         if constexpr (SILU) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = h[i][j];
+            out[i] = code8<float>(h[i], r);
         } else {
-            Int8In<T>::unpack(raw[i], f);
+            float f[8];
+            In::unpack(raw[i], f);
+            out[i] = code8<T>(f, r);
         }
-        uint32_t q[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = code_bits(f[j], r);
-        out[i] = r.dead ? make_uint2(0, 0) : make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
     }
     const int copies = a.inv ? a.top_k : 1;
     for (int s = 0; s < copies; ++s) {
@@ -149,7 +138,7 @@ quant_rows_any_kernel(const RowQuantArgs a) {
     const RowScale r = row_scale(block_max_bits(m));
     const int copies = a.inv ? a.top_k : 1;
     for (int k = threadIdx.x; k < a.K; k += 256) {
-        const int8_t q = r.dead ? int8_t(0) : static_cast<int8_t>(code_bits(value(k), r) & 0xFFu);
+        const int8_t q = static_cast<int8_t>(SILU ? code1<float>(value(k), r) : code1<T>(value(k), r));
         for (int s = 0; s < copies; ++s) {
             const long long dst = a.inv ? __ldg(a.inv + row * a.top_k + s) : row;
             if (a.inv && (dst < 0 || dst >= a.out_rows)) continue;
@@ -175,10 +164,13 @@ int launch_rows(const RowQuantArgs& a, long long rows, cudaStream_t s) {
         LSG_CUDA_TRY(launch_kernel(quant_rows_any_kernel<T, SILU>, grid, dim3(256), 0, s, true, a));
         return LSG_OK;
     }
-    const int v = nvec <= 256 ? 1 : (nvec <= 1024 ? 2 : 4);
+    // Four pieces a thread make small CTAs, so that loads of one row cover the arithmetic of others:
+    // 4096 x 4096 bf16 7.6 us (10.0 with two pieces), 4096 x 14336 27.1 (38.9).  SiLU holds twice the
+    // inputs and its results in registers: two pieces, 8192 x 14336 f32 222 us (265 with four).
+    const int v = nvec <= 128 ? 1 : (SILU ? 2 : 4);
     const dim3 block(static_cast<unsigned>(((nvec + v - 1) / v + 31) / 32 * 32));
     if (v == 1) LSG_CUDA_TRY(launch_kernel(quant_rows_kernel<T, SILU, 1>, grid, block, 0, s, true, a));
-    else if (v == 2) LSG_CUDA_TRY(launch_kernel(quant_rows_kernel<T, SILU, 2>, grid, block, 0, s, true, a));
+    else if constexpr (SILU) LSG_CUDA_TRY(launch_kernel(quant_rows_kernel<T, SILU, 2>, grid, block, 0, s, true, a));
     else LSG_CUDA_TRY(launch_kernel(quant_rows_kernel<T, SILU, 4>, grid, block, 0, s, true, a));
     return LSG_OK;
 }
