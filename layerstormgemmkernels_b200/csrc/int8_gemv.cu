@@ -1,15 +1,16 @@
 // The 8-bit integer product for up to four token rows: a streaming mat-vec.
 //
-// Bound by the weight bytes, N * K once.  One CTA per SM; a warp takes one weight row at a time (two
-// from two token rows on, so that a piece of the activation read from shared memory serves two), its
-// lanes 16 bytes a step, eight steps under way; the activation codes lie in shared memory, and dp4a forms
-// the exact int32 sums.  Activations that come as bf16 or fp16 are quantized by every CTA for itself
+// Bound by the weight bytes, N * K once.  One CTA of 16 warps per SM; every warp streams its own weight
+// rows, in pieces of up to 4 KB by bulk copies into a private ring of up to three slots (192 KB under way
+// per SM from the first microsecond on), and forms the exact int32 sums with dp4a against the activation
+// codes in shared memory.  Activations that come as bf16 or fp16 are quantized by every CTA for itself
 // while its first weights arrive (the arithmetic of the row quantizer, the same codes and scales): one
-// launch instead of two.  The warps of a CTA are as many as divide the SM's share of the rows best.
+// launch instead of two.
 #include "common.cuh"
 #include "host.h"
 #include "int8.cuh"
 
+#include <algorithm>
 #include <atomic>
 
 namespace lsg {
@@ -17,13 +18,18 @@ namespace lsg {
 namespace {
 
 constexpr int kGemvRows = 2;               // token rows
-constexpr int kGemvSmem = 128 * 1024;      // of activation codes
-constexpr int kSteps = 8;                  // 16-byte loads of a lane under way
+constexpr int kGemvWarps = 16;
+constexpr int kGemvThreads = kGemvWarps * 32;
+constexpr int kPiece = 4096;               // bytes of a weight row in a slot
+constexpr int kSlots = 3;
+constexpr int kSlotBytes = kGemvWarps * kPiece;              // one slot of every warp
+constexpr int kGemvSmem = 227 * 1024 - 1024;                 // slots and codes; the barriers are static
+constexpr int kGemvCodes = kGemvSmem - kSlotBytes;           // codes leave one slot at least
 
 template <typename T, int MR>
 __device__ __forceinline__ void quantize_rows(const Int8Gemm& a, int8_t* codes, int ldq, float (&scale)[MR]) {
-    __shared__ uint32_t part[32][MR];
-    const int threads = blockDim.x, warps = threads >> 5;
+    __shared__ uint32_t part[kGemvWarps][MR];
+    constexpr int threads = kGemvThreads, warps = kGemvWarps;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const T* x = reinterpret_cast<const T*>(a.A);
     const bool whole = a.K % 8 == 0 && ((reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(a.lda * 2)) & 15) == 0;
@@ -68,40 +74,44 @@ __device__ __forceinline__ void quantize_rows(const Int8Gemm& a, int8_t* codes, 
     }
 }
 
-// X: the activations' type, int8_t for codes.  MR: rows held (a.M <= MR).  RW: weight rows of a warp.
-template <typename X, int MR, int RW>
-__global__ void __launch_bounds__(RW == 1 ? 896 : 512, 1)
-int8_gemv_kernel(const Int8Gemm a, int ldq) {
-    extern __shared__ __align__(16) int8_t codes[];   // [a.M][ldq], zero behind K
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int threads = blockDim.x;
-    const int stride = gridDim.x * warps * RW;
-    int n0 = (blockIdx.x * warps + warp) * RW;
+// X: the activations' type, int8_t for codes.  MR: rows held (a.M <= MR).
+template <typename X, int MR>
+__global__ void __launch_bounds__(kGemvThreads, 1)
+int8_gemv_kernel(const Int8Gemm a, int ldq, int slots, unsigned int* status, long long limit) {
+    extern __shared__ __align__(128) uint8_t smem[];   // [slots][kGemvWarps][kPiece], then codes [a.M][ldq], zero behind K
+    __shared__ uint64_t full[kSlots][kGemvWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int8_t* codes = reinterpret_cast<int8_t*>(smem + slots * kSlotBytes);
     pdl_launch_dependents();
-    const int8_t* w[RW];
-    auto rows_at = [&](int n) {
-#pragma unroll
-        for (int r = 0; r < RW; ++r) w[r] = a.B + static_cast<long long>(min(n + r, a.N - 1)) * a.ldb;
+    const int first = blockIdx.x * kGemvWarps + warp, stride = gridDim.x * kGemvWarps;
+    const int per_row = (ldq + kPiece - 1) / kPiece;
+    const int pieces = first < a.N ? ((a.N - 1 - first) / stride + 1) * per_row : 0;
+    // piece i of this warp: its bytes and where they lie
+    auto piece_at = [&](int i, int& bytes) {
+        const int row = i / per_row, c = i - row * per_row;
+        bytes = min(kPiece, ldq - c * kPiece);
+        return a.B + static_cast<long long>(first + row * stride) * a.ldb + c * kPiece;
     };
-    rows_at(n0);
-    // the weights may be what the kernel in front writes, so only a hint goes out before the wait
-    if (n0 < a.N)
-#pragma unroll
-        for (int r = 0; r < RW; ++r)
-            for (int k = lane * 128; k < min(a.K, 4096); k += 4096) asm volatile("prefetch.global.L2 [%0];" ::"l"(w[r] + k));
+    auto copy = [&](int i, int slot) {
+        int bytes;
+        const int8_t* src = piece_at(i, bytes);
+        mbar_arrive_expect_tx(&full[slot][warp], bytes);
+        bulk_g2s(smem + slot * kSlotBytes + warp * kPiece, src, bytes, &full[slot][warp]);
+    };
+    if (lane == 0) {
+        for (int s = 0; s < slots; ++s) mbar_init(&full[s][warp], 1);
+        mbar_fence_init();
+        // the weights may be what the kernel in front writes, so only a hint goes out before the wait
+        for (int i = 0; i < min(slots, pieces); ++i) {
+            int bytes;
+            const int8_t* src = piece_at(i, bytes);
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+        }
+    }
     pdl_wait_prior();
-
-    int4 wv[RW][kSteps];
-    auto fetch = [&](int k0) {
-#pragma unroll
-        for (int r = 0; r < RW; ++r)
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int k = k0 + (i * 32 + lane) * 16;
-                wv[r][i] = k < a.K ? __ldg(reinterpret_cast<const int4*>(w[r] + k)) : make_int4(0, 0, 0, 0);
-            }
-    };
-    if (n0 < a.N) fetch(0);
+    if (lane == 0)
+        for (int i = 0; i < min(slots, pieces); ++i) copy(i, i);
+    __syncwarp();
 
     float scale[MR];
     if constexpr (sizeof(X) == 2) {
@@ -111,111 +121,120 @@ int8_gemv_kernel(const Int8Gemm a, int ldq) {
         for (int m = 0; m < MR; ++m) {
             scale[m] = m < a.M ? __ldg(a.scale_A + m) : 0.0f;
             if (m < a.M)
-                for (int k = threadIdx.x * 16; k < ldq; k += threads * 16) {
+                for (int k = threadIdx.x * 16; k < ldq; k += kGemvThreads * 16) {
                     int4 v = __ldg(reinterpret_cast<const int4*>(a.A + m * a.lda + k));
                     if (k + 16 > a.K) v = keep_bytes(v, a.K - k);
                     *reinterpret_cast<int4*>(codes + m * ldq + k) = v;
                 }
         }
     }
+    // lane i: the scale of this warp's row i (of 32; a load per row would stop the stream for its latency)
+    auto channel_scales = [&](int row) {
+        const long long at = first + static_cast<long long>(row + lane) * stride;
+        return at < a.N ? __ldg(a.scale_B + at) : 0.0f;
+    };
+    float sb = channel_scales(0);
     __syncthreads();
 
-    constexpr int kSpan = kSteps * 512;
-    for (; n0 < a.N; n0 += stride) {
-        int acc[MR][RW];
+    int acc[MR], slot = 0, c = 0, n = first, r = 0;
+    uint32_t lap = 0;
 #pragma unroll
-        for (int m = 0; m < MR; ++m)
-#pragma unroll
-            for (int r = 0; r < RW; ++r) acc[m][r] = 0;
-        for (int k0 = 0;;) {
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int k = k0 + (i * 32 + lane) * 16;
-                if (k < a.K) {
-#pragma unroll
-                    for (int m = 0; m < MR; ++m) {
-                        if (m < a.M) {
-                            const int4 xv = *reinterpret_cast<const int4*>(codes + m * ldq + k);
-#pragma unroll
-                            for (int r = 0; r < RW; ++r)
-                                acc[m][r] = dp4a_ss(wv[r][i].x, xv.x, dp4a_ss(wv[r][i].y, xv.y,
-                                            dp4a_ss(wv[r][i].z, xv.z, dp4a_ss(wv[r][i].w, xv.w, acc[m][r]))));
-                        }
-                    }
-                }
+    for (int m = 0; m < MR; ++m) acc[m] = 0;
+    for (int i = 0; i < pieces; ++i) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[slot][warp], lap & 1, status, kDevWaitFull, 2000u, limit))) {
+            // give up, but not before the copies behind this one have landed
+            for (int j = 1; j < slots && i + j < pieces; ++j) {
+                const int other = (slot + j) % slots;
+                mbar_wait_bounded(&full[other][warp], (lap + (slot + j >= slots ? 1 : 0)) & 1, status, kDevWaitFull, 2000u, limit);
             }
-            k0 += kSpan;
-            if (k0 >= a.K) break;
-            fetch(k0);
+            return;
         }
-        const int n_out = n0;
-        if (n0 + stride < a.N) {   // the next row is under way while this one is summed and written
-            rows_at(n0 + stride);
-            fetch(0);
+        const uint8_t* w = smem + slot * kSlotBytes + warp * kPiece;
+        const int8_t* x = codes + c * kPiece;
+        const int bytes = min(kPiece, ldq - c * kPiece);
+        if (bytes == kPiece) {
+#pragma unroll
+            for (int k = lane * 16; k < kPiece; k += 512) {
+                const int4 wv = *reinterpret_cast<const int4*>(w + k);
+#pragma unroll
+                for (int m = 0; m < MR; ++m)
+                    if (m < a.M) {
+                        const int4 xv = *reinterpret_cast<const int4*>(x + m * ldq + k);
+                        acc[m] = dp4a_ss(wv.x, xv.x, dp4a_ss(wv.y, xv.y, dp4a_ss(wv.z, xv.z, dp4a_ss(wv.w, xv.w, acc[m]))));
+                    }
+            }
+        } else {
+            for (int k = lane * 16; k < bytes; k += 512) {
+                const int4 wv = *reinterpret_cast<const int4*>(w + k);
+#pragma unroll
+                for (int m = 0; m < MR; ++m)
+                    if (m < a.M) {
+                        const int4 xv = *reinterpret_cast<const int4*>(x + m * ldq + k);
+                        acc[m] = dp4a_ss(wv.x, xv.x, dp4a_ss(wv.y, xv.y, dp4a_ss(wv.z, xv.z, dp4a_ss(wv.w, xv.w, acc[m]))));
+                    }
+            }
         }
+        __syncwarp();
+        if (lane == 0 && i + slots < pieces) copy(i + slots, slot);
+        if (++slot == slots) {
+            slot = 0;
+            ++lap;
+        }
+        if (++c == per_row) {
+            // lane m writes token row m
+            int v = 0;
+            float sa = 0.0f;
 #pragma unroll
-        for (int m = 0; m < MR; ++m)
-#pragma unroll
-            for (int r = 0; r < RW; ++r) acc[m][r] = __reduce_add_sync(0xffffffffu, acc[m][r]);
-        // lane m * RW + r writes row m of channel n0 + r
-        int v = acc[0][0];
-        float sa = scale[0];
-#pragma unroll
-        for (int m = 0; m < MR; ++m)
-#pragma unroll
-            for (int r = 0; r < RW; ++r)
-                if (lane == m * RW + r) {
-                    v = acc[m][r];
+            for (int m = 0; m < MR; ++m) {
+                const int sum = __reduce_add_sync(0xffffffffu, acc[m]);
+                if (lane == m) {
+                    v = sum;
                     sa = scale[m];
                 }
-        const int m = lane / RW, n = n_out + lane % RW;
-        if (m < a.M && n < a.N && lane < MR * RW)
-            store_out(a.D, a.out_dtype, static_cast<size_t>(m) * a.N + n,
-                      __fmul_rn(__fmul_rn(static_cast<float>(v), sa), __ldg(a.scale_B + n)));
+                acc[m] = 0;
+            }
+            const float sb_row = __shfl_sync(0xffffffffu, sb, r & 31);
+            if (lane < a.M)
+                store_out(a.D, a.out_dtype, static_cast<size_t>(lane) * a.N + n,
+                          __fmul_rn(__fmul_rn(static_cast<float>(v), sa), sb_row));
+            c = 0;
+            n += stride;
+            if ((++r & 31) == 0) sb = channel_scales(r);
+        }
     }
 }
 
-template <typename X, int MR, int RW>
+template <typename X, int MR>
 int launch(const Int8Gemm& a, cudaStream_t s) {
     static std::atomic<bool> configured[64];
     int dev = 0;
     LSG_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_relaxed)) {
-        LSG_CUDA_TRY(cudaFuncSetAttribute(int8_gemv_kernel<X, MR, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemvSmem));
+        LSG_CUDA_TRY(cudaFuncSetAttribute(int8_gemv_kernel<X, MR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemvSmem));
         if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_relaxed);
     }
-    const int ldq = (a.K + 15) & ~15;
-    const int sms = sm_count(), most = RW == 1 ? 28 : 16;
-    const int share = static_cast<int>((static_cast<long long>(a.N) + static_cast<long long>(sms) * RW - 1) / (static_cast<long long>(sms) * RW));
-    int warps = most;
-    if (share <= most) {
-        warps = share < 4 ? 4 : share;   // every row at once; four warps at least to quantize with
-    } else {
-        long long best = -1;
-        for (int w = most; w >= most / 2; --w) {
-            const long long idle = static_cast<long long>((share + w - 1) / w) * w - share;   // row slots left empty
-            if (best < 0 || idle < best) {
-                best = idle;
-                warps = w;
-            }
-        }
-    }
-    const long long ctas = (static_cast<long long>(a.N) + warps * RW - 1) / (warps * RW);
-    LSG_CUDA_TRY(launch_kernel(int8_gemv_kernel<X, MR, RW>, dim3(static_cast<unsigned>(ctas < sms ? ctas : sms)), dim3(warps * 32),
-                               static_cast<size_t>(a.M) * ldq, s, true, a, ldq));
+    const int ldq = (a.K + 15) & ~15, sms = sm_count();
+    const int codes = a.M * ldq;
+    const int ctas = std::min(sms, (a.N + kGemvWarps - 1) / kGemvWarps);
+    // no more slots than a warp has pieces
+    const int pieces = ((a.N - 1) / (ctas * kGemvWarps) + 1) * ((ldq + kPiece - 1) / kPiece);
+    const int slots = std::min(std::min(kSlots, pieces), (kGemvSmem - codes) / kSlotBytes);
+    LSG_CUDA_TRY(launch_kernel(int8_gemv_kernel<X, MR>, dim3(static_cast<unsigned>(ctas)), dim3(kGemvThreads),
+                               static_cast<size_t>(slots) * kSlotBytes + codes, s, true, a, ldq, slots, device_status_word(),
+                               wait_limit_cycles()));
     return LSG_OK;
 }
 
 template <typename X>
 int by_rows(const Int8Gemm& a, cudaStream_t s) {
-    if (a.M == 1) return launch<X, 1, 1>(a, s);
-    return launch<X, 2, 2>(a, s);
+    if (a.M == 1) return launch<X, 1>(a, s);
+    return launch<X, 2>(a, s);
 }
 
 }  // namespace
 
 bool int8_gemv_takes(int M, int K) {
-    return M >= 1 && M <= kGemvRows && static_cast<long long>(M) * ((K + 15) & ~15) <= kGemvSmem;
+    return M >= 1 && M <= kGemvRows && static_cast<long long>(M) * ((K + 15) & ~15) <= kGemvCodes;
 }
 
 int int8_gemv(const Int8Gemm& a, int x_dtype, cudaStream_t s) {

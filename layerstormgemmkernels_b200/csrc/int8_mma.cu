@@ -8,8 +8,8 @@
 //
 //   warps 0-7   epilogue: warp w owns tensor-memory lanes 32 (w % 4).. and every second piece of 16
 //               columns (tokens)
-//   warp 8      TMA producer: 128 weight rows and the tile's tokens, 128 bytes of K a stage
-//   warp 9      MMA issuer: 4 instructions (K = 32 each) a stage
+//   warp 8      TMA producer: 128 weight rows and the tile's tokens, 128 or 256 bytes of K a stage
+//   warp 9      MMA issuer: 4 instructions (K = 32 each) for 128 bytes of K
 //
 // Three forms of the same kernel:
 //   pair    two CTAs share a 256 x 256 tile (cta_group::2): each loads 128 weight rows and half of
@@ -26,6 +26,7 @@
 #include "int8.cuh"
 #include "tcgen05.cuh"
 
+#include <algorithm>
 #include <atomic>
 
 namespace lsg {
@@ -52,7 +53,7 @@ struct MmaArgs {
     int M, N, E, kblocks;     // N: output columns (of silu(g) * u for SwiGLU)
     int tn;                   // tokens of the tensor map's box (of a CTA: half of a pair's)
     int tile;                 // tokens of a tile at most
-    int n_tiles, stages, stage_bytes, tmem_cols;
+    int n_tiles, stages, sub, block_bytes, tmem_cols;   // stages of `sub` K blocks of block_bytes
     unsigned int* status;
     long long limit;
 };
@@ -204,13 +205,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const MmaArgs a) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + a.stages * a.stage_bytes);
+    const int stage_bytes = a.sub * a.block_bytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + a.stages * stage_bytes);
     uint64_t* empty = full + kMaxStages;
     uint64_t* acc_full = empty + kMaxStages;   // [2]
     uint64_t* acc_empty = acc_full + 2;        // [2]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* cum = reinterpret_cast<int*>(smem + a.stages * a.stage_bytes + 512);   // [E + 1] tiles of tokens before expert e
+    int* scan = reinterpret_cast<int*>(tmem_slot + 2);                           // [16]
+    int* cum = reinterpret_cast<int*>(smem + a.stages * stage_bytes + 512);      // [E + 1] tiles of tokens before expert e
     int* start = cum + 1025;                                                      // [E + 1] first row
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -232,40 +235,71 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         mbar_fence_init();
     }
     if (warp == kEpiWarps + 1) alloc_tmem<CG>(tmem_slot, a.tmem_cols);
+    if (!a.offsets && warp == kEpiWarps && elect_one()) {
+        // the first tile's weights on their way into L2 while the kernel in front finishes: a hint, since
+        // that kernel may be the one that writes them
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmW) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmX) : "memory");
+        const int kb_first = SPLIT ? static_cast<int>(static_cast<long long>(a.kblocks) * rank / ranks) : 0;
+        const int n_first = static_cast<int>(blockIdx.x) / static_cast<int>(SPLIT ? ranks : 1) / ((a.M + a.tile - 1) / a.tile);
+        if (a.M <= a.tile && !SWIGLU && CG == 1)
+            for (int kb = kb_first; kb < min(a.kblocks, kb_first + a.stages * a.sub); ++kb)
+                asm volatile("cp.async.bulk.prefetch.tensor.5d.L2.global [%0, {%1, %2, %3, %4, %4}];" ::"l"(&tmW), "r"(kb * kKB),
+                             "r"(n_first * kRows), "r"(0), "r"(0)
+                             : "memory");
+    }
     pdl_wait_prior();
-    if (warp == 0 && a.offsets) {
-        // tiles per expert, summed; offsets are taken as a rising sequence inside [0, M]
-        int carry = 0, last = 0;
-        for (int e0 = 0; e0 < a.E; e0 += 32) {
-            const int e = e0 + lane;
-            const int lo = e < a.E ? min(max(__ldg(a.offsets + e), 0), a.M) : a.M;
-            const int hi = e < a.E ? min(max(__ldg(a.offsets + e + 1), 0), a.M) : a.M;
-            // a running maximum keeps the starts from falling
-            int s = lo;
+    if (a.offsets && threadIdx.x < 256) {
+        // Tiles per expert, summed; offsets are taken as a rising sequence inside [0, M].  A thread has
+        // `per` consecutive experts: a running maximum over the starts, then a running sum of the tiles.
+        const int per = (a.E + 255) >> 8, e0 = threadIdx.x * per;
+        int lo[4], hi[4];
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, s, o);
-                if (lane >= o) s = max(s, v);
-            }
-            s = max(s, last);
-            const int end = max(hi, s);
-            const int units = e < a.E ? (end - s + a.tile - 1) / a.tile : 0;
-            int incl = units;
+        for (int j = 0; j < 4; ++j) {
+            const bool have = j < per && e0 + j < a.E;
+            lo[j] = have ? min(max(__ldg(a.offsets + e0 + j), 0), a.M) : 0;
+            hi[j] = have ? min(max(__ldg(a.offsets + e0 + j + 1), 0), a.M) : 0;
+        }
+        int top = max(max(lo[0], lo[1]), max(lo[2], lo[3]));
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
-            }
-            if (e < a.E) {
-                cum[e] = carry + incl - units;
-                start[e] = s;
-                if (e == a.E - 1) {
-                    cum[a.E] = carry + incl;
-                    start[a.E] = end;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, top, o);
+            if (lane >= o) top = max(top, v);
+        }
+        if (lane == 31) scan[warp] = top;
+        int before = __shfl_up_sync(0xffffffffu, top, 1);
+        if (lane == 0) before = 0;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        for (int i = 0; i < warp; ++i) before = max(before, scan[i]);
+        int units = 0, n[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            lo[j] = before = max(before, lo[j]);
+            hi[j] = max(hi[j], lo[j]);
+            n[j] = j < per && e0 + j < a.E ? (hi[j] - lo[j] + a.tile - 1) / a.tile : 0;
+            units += n[j];
+        }
+        int incl = units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) scan[8 + warp] = incl;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        int at = incl - units;
+        for (int i = 0; i < warp; ++i) at += scan[8 + i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j < per && e0 + j < a.E) {
+                cum[e0 + j] = at;
+                start[e0 + j] = lo[j];
+                at += n[j];
+                if (e0 + j == a.E - 1) {
+                    cum[a.E] = at;
+                    start[a.E] = hi[j];
                 }
             }
-            carry += __shfl_sync(0xffffffffu, incl, 31);
-            last = __shfl_sync(0xffffffffu, s, 31);
         }
     }
     tc_fence_before();
@@ -290,19 +324,25 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             const Tile t = tile_of(a, cum, start, w, kStep);
             const int x_row = t.row0 + (CG == 2 ? static_cast<int>(rank) * (t.height >> 1) : 0);
             const int n_cta = (t.n * CG + (CG == 2 ? static_cast<int>(rank) : 0));
-            for (int kb = kb0; kb < kb1; ++kb) {
+            for (int kb = kb0; kb < kb1; kb += a.sub) {
                 if (lap > 0)
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], (lap - 1) & 1, a.status, kDevWaitEmpty, 2000u, a.limit));
                 if (!ok) break;
                 if (elect_one()) {
-                    uint8_t* dst = smem + s * a.stage_bytes;
+                    uint8_t* dst = smem + s * stage_bytes;
                     uint32_t bar = smem_u32(&full[s]);
                     if (CG == 2) bar = map_to_rank(bar, 0);
+                    const int blocks = min(a.sub, kb1 - kb);
                     // the leader's barrier counts the bytes of both CTAs
-                    if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[s], CG * a.stage_bytes);
-                    if constexpr (SWIGLU) tma_5d<CG>(dst, &tmW, kb * kKB, 0, 0, n_cta * (kRows / 32), t.expert, bar);
-                    else tma_5d<CG>(dst, &tmW, kb * kKB, n_cta * kRows, t.expert, 0, 0, bar);
-                    tma_2d<CG>(dst + kABytes, &tmX, kb * kKB, x_row, bar);
+                    if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[s], CG * blocks * (kABytes + a.tn * kKB));
+                    for (int j = 0; j < blocks; ++j) {
+                        if constexpr (SWIGLU)
+                            tma_5d<CG>(dst + j * a.block_bytes, &tmW, (kb + j) * kKB, 0, 0, n_cta * (kRows / 32), t.expert, bar);
+                        else
+                            tma_5d<CG>(dst + j * a.block_bytes, &tmW, (kb + j) * kKB, n_cta * kRows, t.expert, 0, 0, bar);
+                    }
+                    for (int j = 0; j < blocks; ++j)
+                        tma_2d<CG>(dst + j * a.block_bytes + kABytes, &tmX, (kb + j) * kKB, x_row, bar);
                 }
                 __syncwarp();
                 if (++s == a.stages) {
@@ -334,18 +374,20 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + ab * (a.tmem_cols >> 1);
-                for (int kb = kb0; kb < kb1; ++kb) {
+                for (int kb = kb0; kb < kb1; kb += a.sub) {
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[s], lap & 1, a.status, kDevWaitFull, 2000u, a.limit));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t adesc = smem_desc_sw128(smem_u32(smem + s * a.stage_bytes));
-                    const uint64_t bdesc = smem_desc_sw128(smem_u32(smem + s * a.stage_bytes + kABytes));
                     if (elect_one()) {
+                        for (int j = 0; j < min(a.sub, kb1 - kb); ++j) {
+                            const uint32_t at = smem_u32(smem + s * stage_bytes + j * a.block_bytes);
+                            const uint64_t adesc = smem_desc_sw128(at), bdesc = smem_desc_sw128(at + kABytes);
 #pragma unroll
-                        for (int k = 0; k < kKB / 32; ++k)
-                            mma_i8<CG>(d, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > kb0 || k != 0) ? 1u : 0u);
+                            for (int k = 0; k < kKB / 32; ++k)
+                                mma_i8<CG>(d, adesc + 2 * k, bdesc + 2 * k, idesc, (kb + j > kb0 || k != 0) ? 1u : 0u);
+                        }
                         commit<CG>(&empty[s]);
-                        if (kb == kb1 - 1) commit<CG>(&acc_full[ab]);
+                        if (kb + a.sub >= kb1) commit<CG>(&acc_full[ab]);
                     }
                     __syncwarp();
                     if (++s == a.stages) {
@@ -381,6 +423,9 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             }
             const bool in = n < a.N;
             const float sb = in ? __ldg(a.sB + static_cast<size_t>(t.expert) * n_scales + sb_at) : 0.0f;
+            // the scales of a piece's 16 tokens, fetched a piece ahead
+            auto token_scale = [&](int c) { return __ldg(a.sA + min(t.row0 + c + (lane & 15), a.M - 1)); };
+            float sa_next = SPLIT ? 0.0f : token_scale(half * 16);
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], acc_lap & 1, a.status, kDevWaitMma, 2000u, a.limit));
             if (!ok) break;
             tc_fence_after();
@@ -400,7 +445,8 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                     uint32_t r[16];
                     tmem_ld16(src + c, r);
                     const int tok = t.row0 + c;
-                    const float sa_lane = __ldg(a.sA + min(tok + (lane & 15), a.M - 1));
+                    const float sa_lane = sa_next;
+                    sa_next = token_scale(c + 32);
                     float v[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
@@ -517,7 +563,7 @@ int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const MmaArgs& a, int
         LSG_CUDA_TRY(cudaFuncSetAttribute(int8_mma_kernel<CG, SWIGLU, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_relaxed);
     }
-    const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + 1024 + kTailBytes;
+    const size_t smem = static_cast<size_t>(a.stages) * a.sub * a.block_bytes + 1024 + kTailBytes;
     LSG_CUDA_TRY(launch_clusters(int8_mma_kernel<CG, SWIGLU, SPLIT>, cluster, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, s,
                                  true, tmW, tmX, a));
     return LSG_OK;
@@ -563,8 +609,11 @@ int int8_mma(const Int8Gemm& g, bool swiglu, cudaStream_t s) {
     a.tile = tile;
     a.tn = pair ? tile / 2 : tile;
     a.n_tiles = pair ? (cta_tiles + 1) / 2 : cta_tiles;
-    a.stage_bytes = kABytes + round_up(a.tn * kKB, 1024);
-    a.stages = kSmemMax / a.stage_bytes < kMaxStages ? kSmemMax / a.stage_bytes : kMaxStages;
+    a.block_bytes = kABytes + round_up(a.tn * kKB, 1024);
+    // Few tokens: two or three K blocks a stage, so that what is asked of a weight row at a time is 256 or
+    // 384 bytes (64 tokens of 128 experts, 2048 / 768: 123 -> 112 us; one 8 x 14336 x 4096 16.5 -> 14.1)
+    a.sub = pair ? 1 : std::min(3, std::max(1, 56 * 1024 / a.block_bytes));
+    a.stages = kSmemMax / (a.sub * a.block_bytes) < kMaxStages ? kSmemMax / (a.sub * a.block_bytes) : kMaxStages;
     int cols = 64;
     while (cols < 2 * tile) cols *= 2;
     a.tmem_cols = cols;
