@@ -24,15 +24,15 @@ struct Int8Gemm {
     const int32_t* expert_offsets;   // null: dense
 };
 
-int int8_gemm(const Int8Gemm& a, cudaStream_t s);
+int int8_gemm(const Int8Gemm& a, bool early, cudaStream_t s);
 // A few rows on a streaming mat-vec (int8_gemv.cu): whether a call of these sizes goes there, and the
 // call, with A as codes (x_dtype < 0) or as bf16 / fp16 activations that it quantizes on the way (lda in
 // values, scale_A unused).
 bool int8_gemv_takes(int M, int K);
 int int8_gemv(const Int8Gemm& a, int x_dtype, cudaStream_t s);
 // On the tensor cores (int8_mma.cu).  swiglu: B is [E, 2 N, K], gate rows in front of up rows, and D
-// fp32 silu(gate) * up.
-int int8_mma(const Int8Gemm& g, bool swiglu, cudaStream_t s);
+// fp32 silu(gate) * up.  early: the launch in front on the stream is int8_quant_rows, which writes A.
+int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s);
 int int8_quant_rows(const void* x, long long ldx, int dtype, int8_t* codes, long long ldq, float* scales, long long rows,
                     int K, const int32_t* inv, int top_k, int out_rows, cudaStream_t s);
 int int8_quant_silu_mul(const void* gate, long long ldg, const void* up, long long ldu, int dtype, int8_t* codes,
@@ -50,6 +50,26 @@ __device__ __forceinline__ void store_out(void* D, int dtype, size_t at, float v
     if (dtype == LSG_DTYPE_F32) static_cast<float*>(D)[at] = v;
     else if (dtype == LSG_DTYPE_F16) static_cast<__half*>(D)[at] = __float2half_rn(v);
     else static_cast<__nv_bfloat16*>(D)[at] = __float2bfloat16_rn(v);
+}
+
+// Four neighbouring values, aligned to themselves.
+__device__ __forceinline__ void store_out4(void* D, int dtype, size_t at, const float (&v)[4]) {
+    if (dtype == LSG_DTYPE_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(D) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        return;
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (dtype == LSG_DTYPE_F16) {
+            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(D) + at) = make_uint2(w[0], w[1]);
 }
 
 // Magnitudes order like their bit patterns, infinity and NaN on top.

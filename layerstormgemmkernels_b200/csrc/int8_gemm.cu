@@ -29,9 +29,9 @@ int check(const char* op, int N, int K, const void* A, long long lda, const void
 
 }  // namespace
 
-int int8_gemm(const Int8Gemm& a, cudaStream_t s) {
+int int8_gemm(const Int8Gemm& a, bool early, cudaStream_t s) {
     if (!a.expert_offsets && int8_gemv_takes(a.M, a.K)) return int8_gemv(a, -1, s);
-    return int8_mma(a, false, s);
+    return int8_mma(a, false, early, s);
 }
 
 }  // namespace lsg
@@ -56,7 +56,7 @@ extern "C" int lsg_int8_gemm(const lsg_int8_gemm_params* p, void* stream) {
     a.D = p->D; a.out_dtype = p->output_dtype;
     a.scale_A = p->scale_A; a.scale_B = p->scale_B;
     a.M = p->M; a.N = p->N; a.K = p->K; a.E = 1;
-    return int8_gemm(a, static_cast<cudaStream_t>(stream));
+    return int8_gemm(a, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t lsg_int8_gemm_from_bf16_workspace_bytes(int M, int K) {
@@ -97,7 +97,7 @@ extern "C" int lsg_int8_gemm_from_bf16(const lsg_int8_gemm_params* p, int input_
     a.A = codes; a.lda = ldq; a.scale_A = scales;
     rc = int8_quant_rows(p->A, p->lda, input_dtype, codes, ldq, scales, p->M, p->K, nullptr, 1, 0, s);
     if (rc != LSG_OK) return rc;
-    return int8_gemm(a, s);
+    return int8_gemm(a, true, s);
 }
 
 extern "C" int lsg_int8_grouped_gemm(const lsg_int8_grouped_gemm_params* p, int total_tokens, void* stream) {
@@ -118,7 +118,7 @@ extern "C" int lsg_int8_grouped_gemm(const lsg_int8_grouped_gemm_params* p, int 
     a.scale_A = p->scale_A_base; a.scale_B = p->scale_B_base;
     a.M = total_tokens; a.N = p->N; a.K = p->K; a.E = p->num_experts;
     a.expert_offsets = p->expert_offsets;
-    return int8_gemm(a, static_cast<cudaStream_t>(stream));
+    return int8_gemm(a, false, static_cast<cudaStream_t>(stream));
 }
 
 namespace {
@@ -184,12 +184,12 @@ extern "C" int lsg_int8_moe_ffn(const lsg_int8_moe_ffn_params* p, void* workspac
     a.A = codes; a.lda = f.ldh; a.B = static_cast<const int8_t*>(p->gate_up); a.ldb = H;
     a.D = h; a.out_dtype = LSG_DTYPE_F32; a.scale_A = scales; a.scale_B = p->gate_up_scales;
     a.M = rows; a.N = I; a.K = H; a.E = p->num_experts; a.expert_offsets = p->expert_offsets;
-    rc = int8_mma(a, true, s);
+    rc = int8_mma(a, true, true, s);
     if (rc != LSG_OK) return rc;
     rc = int8_quant_rows(h, I, LSG_DTYPE_F32, act, f.ldi, act_scales, rows, I, nullptr, 1, 0, s);
     if (rc != LSG_OK) return rc;
     a.A = act; a.lda = f.ldi; a.B = static_cast<const int8_t*>(p->down); a.ldb = I;
     a.D = p->D; a.out_dtype = p->output_dtype; a.scale_A = act_scales; a.scale_B = p->down_scales;
     a.N = H; a.K = I;
-    return int8_gemm(a, s);
+    return int8_gemm(a, true, s);
 }

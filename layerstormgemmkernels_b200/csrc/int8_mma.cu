@@ -54,6 +54,7 @@ struct MmaArgs {
     int tn;                   // tokens of the tensor map's box (of a CTA: half of a pair's)
     int tile;                 // tokens of a tile at most
     int n_tiles, stages, sub, block_bytes, tmem_cols;   // stages of `sub` K blocks of block_bytes
+    int early;   // the kernel in front is the row quantizer: weights and offsets are there before it ends
     unsigned int* status;
     long long limit;
 };
@@ -61,11 +62,6 @@ struct MmaArgs {
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
 }
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
@@ -200,12 +196,13 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const int* cum, const 
     return t;
 }
 
-template <int CG, bool SWIGLU, bool SPLIT>
+template <int CG, bool SWIGLU, int SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const MmaArgs a) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int stage_bytes = a.sub * a.block_bytes;
+    const int sub = CG == 2 ? 1 : a.sub;
+    const int stage_bytes = sub * a.block_bytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + a.stages * stage_bytes);
     uint64_t* empty = full + kMaxStages;
     uint64_t* acc_full = empty + kMaxStages;   // [2]
@@ -217,8 +214,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     int* start = cum + 1025;                                                      // [E + 1] first row
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = (CG == 2 || SPLIT) ? cluster_rank() : 0;
-    const uint32_t ranks = SPLIT ? cluster_size() : 1;
+    const uint32_t rank = (CG == 2 || SPLIT > 1) ? cluster_rank() : 0;
     constexpr int kStep = CG == 2 ? 32 : 16;
 
     pdl_launch_dependents();
@@ -235,20 +231,11 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         mbar_fence_init();
     }
     if (warp == kEpiWarps + 1) alloc_tmem<CG>(tmem_slot, a.tmem_cols);
-    if (!a.offsets && warp == kEpiWarps && elect_one()) {
-        // the first tile's weights on their way into L2 while the kernel in front finishes: a hint, since
-        // that kernel may be the one that writes them
+    if (warp == kEpiWarps && elect_one()) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmW) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmX) : "memory");
-        const int kb_first = SPLIT ? static_cast<int>(static_cast<long long>(a.kblocks) * rank / ranks) : 0;
-        const int n_first = static_cast<int>(blockIdx.x) / static_cast<int>(SPLIT ? ranks : 1) / ((a.M + a.tile - 1) / a.tile);
-        if (a.M <= a.tile && !SWIGLU && CG == 1)
-            for (int kb = kb_first; kb < min(a.kblocks, kb_first + a.stages * a.sub); ++kb)
-                asm volatile("cp.async.bulk.prefetch.tensor.5d.L2.global [%0, {%1, %2, %3, %4, %4}];" ::"l"(&tmW), "r"(kb * kKB),
-                             "r"(n_first * kRows), "r"(0), "r"(0)
-                             : "memory");
     }
-    pdl_wait_prior();
+    if (!a.early) pdl_wait_prior();
     if (a.offsets && threadIdx.x < 256) {
         // Tiles per expert, summed; offsets are taken as a rising sequence inside [0, M].  A thread has
         // `per` consecutive experts: a running maximum over the starts, then a running sum of the tiles.
@@ -303,46 +290,62 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         }
     }
     tc_fence_before();
-    if constexpr (CG == 2 || SPLIT) cluster_sync();
+    if constexpr (CG == 2 || SPLIT > 1) cluster_sync();
     else __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
     const int total = (a.offsets ? cum[a.E] : (a.M + a.tile - 1) / a.tile) * a.n_tiles;
-    const int first = (CG == 2 || SPLIT) ? blockIdx.x / (SPLIT ? ranks : CG) : blockIdx.x;
-    const int stride = (CG == 2 || SPLIT) ? gridDim.x / (SPLIT ? ranks : CG) : gridDim.x;
+    const int first = blockIdx.x / (CG * SPLIT);
+    const int stride = gridDim.x / (CG * SPLIT);
     // this CTA's K blocks
-    const int kb0 = SPLIT ? static_cast<int>(static_cast<long long>(a.kblocks) * rank / ranks) : 0;
-    const int kb1 = SPLIT ? static_cast<int>(static_cast<long long>(a.kblocks) * (rank + 1) / ranks) : a.kblocks;
+    const int kb0 = SPLIT > 1 ? static_cast<int>(a.kblocks * rank / SPLIT) : 0;
+    const int kb1 = SPLIT > 1 ? static_cast<int>(a.kblocks * (rank + 1) / SPLIT) : a.kblocks;
 
     if (warp == kEpiWarps) {
         // ------------------------------ TMA producer ------------------------------
         int s = 0;
         uint32_t lap = 0;
         bool ok = true;
+        const int blocks_all = CG == 2 ? 1 : sub;
+        // the weights of stage i, K blocks kb.., and the bytes that its barrier waits for
+        auto load_weights = [&](int i, int kb, const Tile& t, int n_cta, int blocks) {
+            uint8_t* dst = smem + i * stage_bytes;
+            const uint32_t bar = CG == 2 ? map_to_rank(smem_u32(&full[i]), 0) : smem_u32(&full[i]);
+            // the leader's barrier counts the bytes of both CTAs
+            if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[i], CG * blocks * (kABytes + a.tn * kKB));
+            for (int j = 0; j < blocks; ++j) {
+                if constexpr (SWIGLU)
+                    tma_5d<CG>(dst + j * a.block_bytes, &tmW, (kb + j) * kKB, 0, 0, n_cta * (kRows / 32), t.expert, bar);
+                else
+                    tma_5d<CG>(dst + j * a.block_bytes, &tmW, (kb + j) * kKB, n_cta * kRows, t.expert, 0, 0, bar);
+            }
+        };
+        int ahead = 0;   // stages whose weights are under way before the kernel in front has ended
+        if (a.early) {
+            if (first < total) {
+                const Tile t = tile_of(a, cum, start, first, kStep);
+                const int n_cta = t.n * CG + (CG == 2 ? static_cast<int>(rank) : 0);
+                for (int kb = kb0; kb < kb1 && ahead < a.stages; kb += blocks_all, ++ahead)
+                    if (elect_one()) load_weights(ahead, kb, t, n_cta, CG == 2 ? 1 : min(sub, kb1 - kb));
+                __syncwarp();
+            }
+            pdl_wait_prior();
+        }
         for (int w = first; w < total && ok && !*abort_flag; w += stride) {
             const Tile t = tile_of(a, cum, start, w, kStep);
             const int x_row = t.row0 + (CG == 2 ? static_cast<int>(rank) * (t.height >> 1) : 0);
-            const int n_cta = (t.n * CG + (CG == 2 ? static_cast<int>(rank) : 0));
-            for (int kb = kb0; kb < kb1; kb += a.sub) {
+            const int n_cta = t.n * CG + (CG == 2 ? static_cast<int>(rank) : 0);
+            for (int kb = kb0; kb < kb1; kb += sub) {
                 if (lap > 0)
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], (lap - 1) & 1, a.status, kDevWaitEmpty, 2000u, a.limit));
                 if (!ok) break;
                 if (elect_one()) {
-                    uint8_t* dst = smem + s * stage_bytes;
-                    uint32_t bar = smem_u32(&full[s]);
-                    if (CG == 2) bar = map_to_rank(bar, 0);
-                    const int blocks = min(a.sub, kb1 - kb);
-                    // the leader's barrier counts the bytes of both CTAs
-                    if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[s], CG * blocks * (kABytes + a.tn * kKB));
-                    for (int j = 0; j < blocks; ++j) {
-                        if constexpr (SWIGLU)
-                            tma_5d<CG>(dst + j * a.block_bytes, &tmW, (kb + j) * kKB, 0, 0, n_cta * (kRows / 32), t.expert, bar);
-                        else
-                            tma_5d<CG>(dst + j * a.block_bytes, &tmW, (kb + j) * kKB, n_cta * kRows, t.expert, 0, 0, bar);
-                    }
-                    for (int j = 0; j < blocks; ++j)
-                        tma_2d<CG>(dst + j * a.block_bytes + kABytes, &tmX, (kb + j) * kKB, x_row, bar);
+                    const int blocks = CG == 2 ? 1 : min(sub, kb1 - kb);
+                    if (lap > 0 || s >= ahead) load_weights(s, kb, t, n_cta, blocks);
+                    uint8_t* dst = smem + s * stage_bytes + kABytes;
+                    const uint32_t bar = CG == 2 ? map_to_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
+                    for (int j = 0; j < blocks; ++j) tma_2d<CG>(dst + j * a.block_bytes, &tmX, (kb + j) * kKB, x_row, bar);
                 }
                 __syncwarp();
                 if (++s == a.stages) {
@@ -362,6 +365,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         }
     } else if (warp == kEpiWarps + 1) {
         // ------------------------------ MMA issuer --------------------------------
+        if (a.early) pdl_wait_prior();
         int s = 0, ab = 0;
         uint32_t lap = 0, acc_lap = 0;
         bool ok = true;
@@ -374,12 +378,13 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + ab * (a.tmem_cols >> 1);
-                for (int kb = kb0; kb < kb1; kb += a.sub) {
+                for (int kb = kb0; kb < kb1; kb += sub) {
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[s], lap & 1, a.status, kDevWaitFull, 2000u, a.limit));
                     if (!ok) break;
                     tc_fence_after();
+                    const int blocks = CG == 2 ? 1 : min(sub, kb1 - kb);
                     if (elect_one()) {
-                        for (int j = 0; j < min(a.sub, kb1 - kb); ++j) {
+                        for (int j = 0; j < blocks; ++j) {
                             const uint32_t at = smem_u32(smem + s * stage_bytes + j * a.block_bytes);
                             const uint64_t adesc = smem_desc_sw128(at), bdesc = smem_desc_sw128(at + kABytes);
 #pragma unroll
@@ -387,7 +392,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                                 mma_i8<CG>(d, adesc + 2 * k, bdesc + 2 * k, idesc, (kb + j > kb0 || k != 0) ? 1u : 0u);
                         }
                         commit<CG>(&empty[s]);
-                        if (kb + a.sub >= kb1) commit<CG>(&acc_full[ab]);
+                        if (kb + sub >= kb1) commit<CG>(&acc_full[ab]);
                     }
                     __syncwarp();
                     if (++s == a.stages) {
@@ -402,6 +407,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         }
     } else {
         // ------------------------------ epilogue (warps 0-7) ----------------------
+        if (a.early) pdl_wait_prior();
         const int q = warp & 3, half = warp >> 2;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
         int ab = 0;
@@ -422,15 +428,15 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 n_scales = a.N;
             }
             const bool in = n < a.N;
-            const float sb = in ? __ldg(a.sB + static_cast<size_t>(t.expert) * n_scales + sb_at) : 0.0f;
+            const float sb = SPLIT == 1 && in ? __ldg(a.sB + static_cast<size_t>(t.expert) * n_scales + sb_at) : 0.0f;
             // the scales of a piece's 16 tokens, fetched a piece ahead
             auto token_scale = [&](int c) { return __ldg(a.sA + min(t.row0 + c + (lane & 15), a.M - 1)); };
-            float sa_next = SPLIT ? 0.0f : token_scale(half * 16);
+            float sa_next = SPLIT > 1 ? 0.0f : token_scale(half * 16);
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], acc_lap & 1, a.status, kDevWaitMma, 2000u, a.limit));
             if (!ok) break;
             tc_fence_after();
             const uint32_t src = t_lane + ab * (a.tmem_cols >> 1);
-            if constexpr (SPLIT) {
+            if constexpr (SPLIT > 1) {
                 // partial sums to this CTA's shared memory, [token][128 channels]; the stages are free:
                 // every MMA that reads them has completed
                 int* part = reinterpret_cast<int*>(smem);
@@ -483,34 +489,53 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
 
     tc_fence_before();
     __syncwarp();
-    if constexpr (SPLIT) {
+    if constexpr (SPLIT > 1) {
+        // Every rank adds and writes its share of the tokens: a warp U tokens at a time, four channels a
+        // lane, all loads of the partial sums under way together.
+        constexpr int U = SPLIT == 8 ? 1 : (SPLIT == 4 ? 2 : 4);
+        constexpr int kApart = SPLIT * (kThreads / 32);
+        const Tile t = tile_of(a, cum, start, first, kStep);
+        const int n = t.n * kRows + lane * 4;
+        float sb[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sb[i] = n + i < a.N ? __ldg(a.sB + n + i) : 0.0f;
+        const size_t size = a.out_dtype == LSG_DTYPE_F32 ? 4 : 2;
+        const bool whole = n + 3 < a.N && (a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.D) & (4 * size - 1)) == 0;
         cluster_sync();
-        // every rank adds and writes its share of the tokens: a warp a token, four channels a lane
-        const int w = first;
-        if (w < total) {
-            const Tile t = tile_of(a, cum, start, w, kStep);
-            const int n = t.n * kRows + lane * 4;
-            float sb[4];
+        for (int c0 = static_cast<int>(rank) + SPLIT * warp; c0 < t.rows; c0 += U * kApart) {
+            float4 p[U][SPLIT];
+            float sa[U];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sb[i] = n + i < a.N ? __ldg(a.sB + static_cast<size_t>(t.expert) * a.N + n + i) : 0.0f;
-            for (int c = static_cast<int>(rank) + static_cast<int>(ranks) * warp; c < t.rows; c += static_cast<int>(ranks) * (kThreads / 32)) {
+            for (int u = 0; u < U; ++u) {
+                const int c = min(c0 + u * kApart, t.rows - 1);
+                sa[u] = __ldg(a.sA + t.row0 + c);
                 const uint32_t at = smem_u32(smem) + static_cast<uint32_t>((c * kRows + lane * 4) * 4);
-                int v[4] = {0, 0, 0, 0};
-                for (uint32_t r = 0; r < ranks; ++r) {
-                    const float4 p = ld_cluster_f4(at, r);
-                    v[0] += __float_as_int(p.x);
-                    v[1] += __float_as_int(p.y);
-                    v[2] += __float_as_int(p.z);
-                    v[3] += __float_as_int(p.w);
-                }
-                const int row = t.row0 + c;
-                const float sa = __ldg(a.sA + row);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n + i < a.N)
-                        store_out(a.D, a.out_dtype, static_cast<size_t>(row) * a.N + n + i,
-                                  __fmul_rn(__fmul_rn(static_cast<float>(v[i]), sa), sb[i]));
+                for (int r = 0; r < SPLIT; ++r) p[u][r] = ld_cluster_f4(at, r);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int c = c0 + u * kApart;
+                if (c >= t.rows) break;
+                int v[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < SPLIT; ++r) {
+                    v[0] += __float_as_int(p[u][r].x);
+                    v[1] += __float_as_int(p[u][r].y);
+                    v[2] += __float_as_int(p[u][r].z);
+                    v[3] += __float_as_int(p[u][r].w);
+                }
+                float o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = __fmul_rn(__fmul_rn(static_cast<float>(v[i]), sa[u]), sb[i]);
+                const size_t at = static_cast<size_t>(t.row0 + c) * a.N + n;
+                if (whole) {
+                    store_out4(a.D, a.out_dtype, at, o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (n + i < a.N) store_out(a.D, a.out_dtype, at + i, o[i]);
+                }
             }
         }
         __syncwarp();
@@ -554,7 +579,7 @@ int weight_map(CUtensorMap* map, const Int8Gemm& g, bool swiglu) {
     return encode(map, 5, g.B, dims, strides, box);
 }
 
-template <int CG, bool SWIGLU, bool SPLIT>
+template <int CG, bool SWIGLU, int SPLIT>
 int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const MmaArgs& a, int grid, int cluster, cudaStream_t s) {
     static std::atomic<bool> configured[64];
     int dev = 0;
@@ -573,11 +598,14 @@ int round_up(int v, int step) { return (v + step - 1) / step * step; }
 
 }  // namespace
 
-// D = A B^T with both scales; swiglu: B is [E, 2 N, K] and D fp32 silu(gate) * up.
-int int8_mma(const Int8Gemm& g, bool swiglu, cudaStream_t s) {
+// D = A B^T with both scales; swiglu: B is [E, 2 N, K] and D fp32 silu(gate) * up.  early: A comes from
+// the row quantizer launched right in front.  That kernel lets this one start only after its own wait,
+// so everything launched before it has ended: offsets are read and weights loaded while it still runs.
+int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
     MmaArgs a = {};
     a.D = g.D; a.out_dtype = g.out_dtype; a.sA = g.scale_A; a.sB = g.scale_B; a.offsets = g.expert_offsets;
     a.M = g.M; a.N = g.N; a.E = g.E; a.kblocks = (g.K + kKB - 1) / kKB;
+    a.early = early ? 1 : 0;
     a.status = device_status_word();
     a.limit = wait_limit_cycles();
     const int sms = sm_count();
@@ -631,11 +659,13 @@ int int8_mma(const Int8Gemm& g, bool swiglu, cudaStream_t s) {
 
     if (pair) {
         const int grid = 2 * static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
-        return swiglu ? launch<2, true, false>(tmW, tmX, a, grid, 2, s) : launch<2, false, false>(tmW, tmX, a, grid, 2, s);
+        return swiglu ? launch<2, true, 1>(tmW, tmX, a, grid, 2, s) : launch<2, false, 1>(tmW, tmX, a, grid, 2, s);
     }
-    if (split > 1) return launch<1, false, true>(tmW, tmX, a, static_cast<int>(tiles) * split, split, s);
+    if (split == 8) return launch<1, false, 8>(tmW, tmX, a, static_cast<int>(tiles) * 8, 8, s);
+    if (split == 4) return launch<1, false, 4>(tmW, tmX, a, static_cast<int>(tiles) * 4, 4, s);
+    if (split == 2) return launch<1, false, 2>(tmW, tmX, a, static_cast<int>(tiles) * 2, 2, s);
     const int grid = static_cast<int>(tiles < sms ? tiles : sms);
-    return swiglu ? launch<1, true, false>(tmW, tmX, a, grid, 1, s) : launch<1, false, false>(tmW, tmX, a, grid, 1, s);
+    return swiglu ? launch<1, true, 1>(tmW, tmX, a, grid, 1, s) : launch<1, false, 1>(tmW, tmX, a, grid, 1, s);
 }
 
 }  // namespace lsg

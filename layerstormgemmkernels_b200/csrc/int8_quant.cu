@@ -54,8 +54,9 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t m) {
 template <typename T, bool SILU, int V>
 __global__ void __launch_bounds__(V <= 2 ? 1024 : 512)
 quant_rows_kernel(const RowQuantArgs a) {
-    pdl_launch_dependents();
+    // in this order: what starts after this kernel may rely on everything in front of it having ended
     pdl_wait_prior();
+    pdl_launch_dependents();
     using In = Int8In<T>;
     constexpr int L = In::kVecs;
     const long long row = blockIdx.x;
@@ -124,8 +125,8 @@ quant_rows_kernel(const RowQuantArgs a) {
 template <typename T, bool SILU>
 __global__ void __launch_bounds__(256)
 quant_rows_any_kernel(const RowQuantArgs a) {
-    pdl_launch_dependents();
     pdl_wait_prior();
+    pdl_launch_dependents();
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* up = SILU ? static_cast<const T*>(a.up) + row * a.ldu : nullptr;
