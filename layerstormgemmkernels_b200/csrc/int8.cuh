@@ -52,6 +52,15 @@ __device__ __forceinline__ void store_out(void* D, int dtype, size_t at, float v
     else static_cast<__nv_bfloat16*>(D)[at] = __float2bfloat16_rn(v);
 }
 
+template <typename T> __device__ __forceinline__ T out_of(float v);
+template <> __device__ __forceinline__ float out_of(float v) { return v; }
+template <> __device__ __forceinline__ __half out_of(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 out_of(float v) { return __float2bfloat16_rn(v); }
+
+// silu(g) * u in fp32; the quotient by __fdividef (two ulp, half the instructions of a division; its
+// zero for a denominator above 2^126 is what exp(87) leaves of any g).
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
+
 // Four neighbouring values, aligned to themselves.
 __device__ __forceinline__ void store_out4(void* D, int dtype, size_t at, const float (&v)[4]) {
     if (dtype == LSG_DTYPE_F32) {

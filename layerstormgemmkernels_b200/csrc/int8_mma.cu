@@ -41,7 +41,7 @@ constexpr int kABytes = kRows * kKB;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kMaxStages = 12;
-constexpr int kTailBytes = 512 + 2 * 1025 * 4 + 64;    // barriers, flags, the experts' tiles and rows
+constexpr int kTailBytes = 512 + 1024 + 2 * 1025 * 4 + 64;    // barriers, flags; token scales; the experts' tiles and rows
 constexpr int kSmemMax = 227 * 1024 - 1024 - kTailBytes;
 
 struct MmaArgs {
@@ -156,7 +156,27 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+    // the registers pass through, so that nothing reads them earlier
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
+// Sixteen tokens (rows of D) of one output column to p, p + N, ...; the first `count` of them.
+template <typename T>
+__device__ __forceinline__ void store_column(T* p, size_t ld, const float (&v)[16], int count) {
+    if (count >= 16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i, p += ld) *p = out_of<T>(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i, p += ld)
+            if (i < count) *p = out_of<T>(v[i]);
+    }
 }
 
 // The tile a CTA (or pair) works on next.
@@ -210,7 +230,8 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* scan = reinterpret_cast<int*>(tmem_slot + 2);                           // [16]
-    int* cum = reinterpret_cast<int*>(smem + a.stages * stage_bytes + 512);      // [E + 1] tiles of tokens before expert e
+    float* scales = reinterpret_cast<float*>(smem + a.stages * stage_bytes + 512);   // [epilogue warps][2][16] of the tokens
+    int* cum = reinterpret_cast<int*>(smem + a.stages * stage_bytes + 512 + 1024);   // [E + 1] tiles of tokens before expert e
     int* start = cum + 1025;                                                      // [E + 1] first row
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -429,7 +450,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             }
             const bool in = n < a.N;
             const float sb = SPLIT == 1 && in ? __ldg(a.sB + static_cast<size_t>(t.expert) * n_scales + sb_at) : 0.0f;
-            // the scales of a piece's 16 tokens, fetched a piece ahead
+            // the scales of a piece's 16 tokens, fetched a piece ahead and handed round through shared memory
             auto token_scale = [&](int c) { return __ldg(a.sA + min(t.row0 + c + (lane & 15), a.M - 1)); };
             float sa_next = SPLIT > 1 ? 0.0f : token_scale(half * 16);
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], acc_lap & 1, a.status, kDevWaitMma, 2000u, a.limit));
@@ -443,36 +464,60 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 for (int c = half * 16; c < t.height; c += 32) {
                     uint32_t r[16];
                     tmem_ld16(src + c, r);
+                    tmem_ld_wait(r);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) part[(c + i) * kRows + q * 32 + lane] = static_cast<int>(r[i]);
                 }
             } else {
-                for (int c = half * 16; c < t.rows; c += 32) {
-                    uint32_t r[16];
-                    tmem_ld16(src + c, r);
-                    const int tok = t.row0 + c;
-                    const float sa_lane = sa_next;
+                float* sa_buf = scales + warp * 32;
+                auto piece = [&](const uint32_t (&r)[16], int c) {
+                    if (lane < 16) sa_buf[lane] = sa_next;
+                    __syncwarp();
                     sa_next = token_scale(c + 32);
                     float v[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        v[i] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i])), __shfl_sync(0xffffffffu, sa_lane, i)), sb);
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 sa = *reinterpret_cast<const float4*>(sa_buf + i);
+                        v[i] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i])), sa.x), sb);
+                        v[i + 1] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i + 1])), sa.y), sb);
+                        v[i + 2] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i + 2])), sa.z), sb);
+                        v[i + 3] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i + 3])), sa.w), sb);
+                    }
+                    sa_buf = scales + warp * 32 + ((c >> 1) & 16 ? 0 : 16);   // the other half for the next piece
                     if constexpr (SWIGLU) {
+                        float* p = static_cast<float*>(a.D) + static_cast<size_t>(t.row0 + c + (lane >> 4)) * a.N + n;
+                        const int left = t.rows - c - (lane >> 4);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
+                        for (int i = 0; i < 16; i += 2, p += 2 * static_cast<size_t>(a.N)) {
                             // lanes 0-15 take token i, lanes 16-31 token i + 1
                             const float got = __shfl_xor_sync(0xffffffffu, lane < 16 ? v[i + 1] : v[i], 16);
                             const float g = lane < 16 ? v[i] : got, u = lane < 16 ? got : v[i + 1];
-                            const int row = tok + i + (lane >> 4);
-                            if (in && c + i + (lane >> 4) < t.rows)
-                                static_cast<float*>(a.D)[static_cast<size_t>(row) * a.N + n] = g / (1.0f + expf(-g)) * u;
+                            if (in && i < left) *p = silu_mul(g, u);
                         }
-                    } else {
-                        const size_t at = static_cast<size_t>(tok) * a.N + n;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (in && c + i < t.rows) store_out(a.D, a.out_dtype, at + static_cast<size_t>(i) * a.N, v[i]);
+                    } else if (in) {
+                        const size_t at = static_cast<size_t>(t.row0 + c) * a.N + n;
+                        const int count = t.rows - c;
+                        if (a.out_dtype == LSG_DTYPE_BF16) store_column(static_cast<__nv_bfloat16*>(a.D) + at, a.N, v, count);
+                        else if (a.out_dtype == LSG_DTYPE_F16) store_column(static_cast<__half*>(a.D) + at, a.N, v, count);
+                        else store_column(static_cast<float*>(a.D) + at, a.N, v, count);
                     }
+                };
+                // two pieces in registers: one is read while the other is worked on
+                uint32_t r0[16], r1[16];
+                int c = half * 16;
+                if (c < t.rows) {
+                    tmem_ld16(src + c, r0);
+                    tmem_ld_wait(r0);
+                }
+                while (c < t.rows) {
+                    if (c + 32 < t.rows) tmem_ld16(src + c + 32, r1);
+                    piece(r0, c);
+                    if (c + 32 >= t.rows) break;
+                    tmem_ld_wait(r1);
+                    if (c + 64 < t.rows) tmem_ld16(src + c + 64, r0);
+                    piece(r1, c + 32);
+                    if (c + 64 < t.rows) tmem_ld_wait(r0);
+                    c += 64;
                 }
                 tc_fence_before();
                 __syncwarp();

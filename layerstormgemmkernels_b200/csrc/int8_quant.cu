@@ -36,8 +36,6 @@ struct RowQuantArgs {
     int out_rows;
 };
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
-
 // Bits of the largest magnitude of the CTA's values; magnitudes order like their bit patterns, with
 // infinity and NaN on top, so nothing that is not finite is lost.
 __device__ __forceinline__ uint32_t block_max_bits(uint32_t m) {
