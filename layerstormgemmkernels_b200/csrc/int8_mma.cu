@@ -6,10 +6,10 @@
 // count: N is 16 to 256 tokens in steps of 16, few tokens cost few tensor cycles, and a warp's
 // store of one token is contiguous whatever N and M are.
 //
-//   warps 0-7   epilogue: warp w owns tensor-memory lanes 32 (w % 4).. and every second piece of 16
-//               columns (tokens)
-//   warp 8      TMA producer: 128 weight rows and the tile's tokens, 128 or 256 bytes of K a stage
-//   warp 9      MMA issuer: 4 instructions (K = 32 each) for 128 bytes of K
+//   first warps epilogue: warp w owns tensor-memory lanes 32 (w % 4).. and the pieces of 16 columns
+//               (tokens) w / 4, w / 4 + groups, ..
+//   next warp   TMA producer: 128 weight rows and the tile's tokens, 128 or 256 bytes of K a stage
+//   last warp   MMA issuer: 4 instructions (K = 32 each) for 128 bytes of K
 //
 // Three forms of the same kernel:
 //   pair    two CTAs share a 256 x 256 tile (cta_group::2): each loads 128 weight rows and half of
@@ -38,10 +38,12 @@ namespace {
 constexpr int kRows = 128;                   // weight rows of a CTA
 constexpr int kKB = 128;                     // bytes of K in a stage
 constexpr int kABytes = kRows * kKB;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiGroups = 2;               // of four warps: 128 lanes of tensor memory
+constexpr int kEpiWarps = 4 * kEpiGroups;
+constexpr int kPieces = 16 * kEpiGroups;     // columns from one piece of a warp to its next
 constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kMaxStages = 12;
-constexpr int kTailBytes = 512 + 1024 + 2 * 1025 * 4 + 64;    // barriers, flags; token scales; the experts' tiles and rows
+constexpr int kTailBytes = 512 + kEpiWarps * 128 + 2 * 1025 * 4 + 64;    // barriers, flags; token scales; the experts' tiles and rows
 constexpr int kSmemMax = 227 * 1024 - 1024 - kTailBytes;
 
 struct MmaArgs {
@@ -181,10 +183,10 @@ __device__ __forceinline__ void store_column(T* p, size_t ld, const float (&v)[1
 
 // The tile a CTA (or pair) works on next.
 struct Tile {
-    int expert, row0, rows, height, n;   // height: tokens the MMA multiplies, a multiple of STEP
+    int expert, row0, rows, height, n;   // height: tokens the MMA multiplies, a multiple of `step`
 };
 
-// Tiles of an expert share its rows evenly, in heights that are multiples of `step`.
+// Tiles of an expert share its rows evenly, in multiples of `step`; the last one multiplies what is left.
 __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const int* cum, const int* start, int w, int step) {
     Tile t;
     int r0, rows, units, local;
@@ -210,9 +212,10 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const int* cum, const 
     t.n = local / units;
     const int u = local - t.n * units;
     const int even = (rows + units - 1) / units;
-    t.height = (even + step - 1) / step * step;
-    t.row0 = r0 + u * t.height;
-    t.rows = min(t.height, rows - u * t.height);
+    const int apart = (even + step - 1) / step * step;
+    t.row0 = r0 + u * apart;
+    t.rows = min(apart, rows - u * apart);
+    t.height = (t.rows + step - 1) / step * step;
     return t;
 }
 
@@ -231,7 +234,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* scan = reinterpret_cast<int*>(tmem_slot + 2);                           // [16]
     float* scales = reinterpret_cast<float*>(smem + a.stages * stage_bytes + 512);   // [epilogue warps][2][16] of the tokens
-    int* cum = reinterpret_cast<int*>(smem + a.stages * stage_bytes + 512 + 1024);   // [E + 1] tiles of tokens before expert e
+    int* cum = reinterpret_cast<int*>(smem + a.stages * stage_bytes + 512 + kEpiWarps * 128);   // [E + 1] tiles of tokens before expert e
     int* start = cum + 1025;                                                      // [E + 1] first row
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -427,9 +430,9 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             if (!ok) *abort_flag = 1;
         }
     } else {
-        // ------------------------------ epilogue (warps 0-7) ----------------------
+        // ------------------------------ epilogue ---------------------------------
         if (a.early) pdl_wait_prior();
-        const int q = warp & 3, half = warp >> 2;
+        const int q = warp & 3, group = warp >> 2;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
         int ab = 0;
         uint32_t acc_lap = 0;
@@ -452,7 +455,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             const float sb = SPLIT == 1 && in ? __ldg(a.sB + static_cast<size_t>(t.expert) * n_scales + sb_at) : 0.0f;
             // the scales of a piece's 16 tokens, fetched a piece ahead and handed round through shared memory
             auto token_scale = [&](int c) { return __ldg(a.sA + min(t.row0 + c + (lane & 15), a.M - 1)); };
-            float sa_next = SPLIT > 1 ? 0.0f : token_scale(half * 16);
+            float sa_next = SPLIT > 1 ? 0.0f : token_scale(group * 16);
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[ab], acc_lap & 1, a.status, kDevWaitMma, 2000u, a.limit));
             if (!ok) break;
             tc_fence_after();
@@ -461,7 +464,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 // partial sums to this CTA's shared memory, [token][128 channels]; the stages are free:
                 // every MMA that reads them has completed
                 int* part = reinterpret_cast<int*>(smem);
-                for (int c = half * 16; c < t.height; c += 32) {
+                for (int c = group * 16; c < t.height; c += kPieces) {
                     uint32_t r[16];
                     tmem_ld16(src + c, r);
                     tmem_ld_wait(r);
@@ -469,11 +472,13 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                     for (int i = 0; i < 16; ++i) part[(c + i) * kRows + q * 32 + lane] = static_cast<int>(r[i]);
                 }
             } else {
-                float* sa_buf = scales + warp * 32;
+                int flip = 0;
                 auto piece = [&](const uint32_t (&r)[16], int c) {
+                    float* sa_buf = scales + warp * 32 + flip;
+                    flip ^= 16;   // the other half for the next piece
                     if (lane < 16) sa_buf[lane] = sa_next;
                     __syncwarp();
-                    sa_next = token_scale(c + 32);
+                    sa_next = token_scale(c + kPieces);
                     float v[16];
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
@@ -483,7 +488,6 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                         v[i + 2] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i + 2])), sa.z), sb);
                         v[i + 3] = __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(r[i + 3])), sa.w), sb);
                     }
-                    sa_buf = scales + warp * 32 + ((c >> 1) & 16 ? 0 : 16);   // the other half for the next piece
                     if constexpr (SWIGLU) {
                         float* p = static_cast<float*>(a.D) + static_cast<size_t>(t.row0 + c + (lane >> 4)) * a.N + n;
                         const int left = t.rows - c - (lane >> 4);
@@ -504,20 +508,20 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 };
                 // two pieces in registers: one is read while the other is worked on
                 uint32_t r0[16], r1[16];
-                int c = half * 16;
+                int c = group * 16;
                 if (c < t.rows) {
                     tmem_ld16(src + c, r0);
                     tmem_ld_wait(r0);
                 }
                 while (c < t.rows) {
-                    if (c + 32 < t.rows) tmem_ld16(src + c + 32, r1);
+                    if (c + kPieces < t.rows) tmem_ld16(src + c + kPieces, r1);
                     piece(r0, c);
-                    if (c + 32 >= t.rows) break;
+                    if (c + kPieces >= t.rows) break;
                     tmem_ld_wait(r1);
-                    if (c + 64 < t.rows) tmem_ld16(src + c + 64, r0);
-                    piece(r1, c + 32);
-                    if (c + 64 < t.rows) tmem_ld_wait(r0);
-                    c += 64;
+                    if (c + 2 * kPieces < t.rows) tmem_ld16(src + c + 2 * kPieces, r0);
+                    piece(r1, c + kPieces);
+                    if (c + 2 * kPieces < t.rows) tmem_ld_wait(r0);
+                    c += 2 * kPieces;
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -683,9 +687,10 @@ int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
     a.tn = pair ? tile / 2 : tile;
     a.n_tiles = pair ? (cta_tiles + 1) / 2 : cta_tiles;
     a.block_bytes = kABytes + round_up(a.tn * kKB, 1024);
-    // Few tokens: two or three K blocks a stage, so that what is asked of a weight row at a time is 256 or
-    // 384 bytes (64 tokens of 128 experts, 2048 / 768: 123 -> 112 us; one 8 x 14336 x 4096 16.5 -> 14.1)
-    a.sub = pair ? 1 : std::min(3, std::max(1, 56 * 1024 / a.block_bytes));
+    // Up to 128 tokens: two to four K blocks a stage, so that what is asked of a weight row at a time is 256
+    // to 512 bytes (256 tokens, 8 experts of 4096 / 14336: 278 us with stages of 56 KB, 261 with 74 KB, 272
+    // with 110 KB; 128 x 14336 x 4096 20.6 with one block, then 18.3, 16.2, 18.2).
+    a.sub = pair ? 1 : std::min(4, std::max(1, 74 * 1024 / a.block_bytes));
     a.stages = kSmemMax / (a.sub * a.block_bytes) < kMaxStages ? kSmemMax / (a.sub * a.block_bytes) : kMaxStages;
     int cols = 64;
     while (cols < 2 * tile) cols *= 2;
