@@ -700,67 +700,22 @@ def nvfp4_grouped_gemm(A_base, B_base, D_base, scale_A_base, scale_B_base, alpha
 # 8-bit integers with a scale per token and per output channel (additions; the reference's
 # 8-bit family is FP8)
 # ---------------------------------------------------------------------------
-_CODE = {torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16, torch.float32: capi.DTYPE_F32}
-_INT8_OUT = {"bf16": (capi.DTYPE_BF16, torch.bfloat16), "bfloat16": (capi.DTYPE_BF16, torch.bfloat16),
-             "fp16": (capi.DTYPE_F16, torch.float16), "float16": (capi.DTYPE_F16, torch.float16),
-             "fp32": (capi.DTYPE_F32, torch.float32), "float32": (capi.DTYPE_F32, torch.float32)}
+class _HostModule:
+    """layerstormgemmkernels_b200.torch_ext.lsg_torch_ops: argument checks, allocation and the C call of
+    the operators below, in C++ because an eager call at decode sizes costs its host work (9 us through
+    ctypes, half of that here).  Imported with the first call; without it the call raises."""
+
+    def __getattr__(self, name):
+        try:
+            from .torch_ext import lsg_torch_ops
+        except ImportError as e:
+            raise ImportError("lsg_torch_ops is not built: run `python -m layerstormgemmkernels_b200.torch_ext.build_ext`") from e
+        fn = getattr(lsg_torch_ops, name)
+        setattr(self, name, fn)
+        return fn
 
 
-def _int8_out(s):
-    out = _INT8_OUT.get(s)
-    _require(out is not None, f"Unknown output dtype: {s}. Expected 'bf16', 'fp16' or 'fp32'.")
-    return out
-
-
-def _call(t, fn, *args):
-    """fn(*args, stream) on the current stream of t's device, whichever device is current."""
-    i = t.get_device()
-    if i == torch._C._cuda_getDevice():
-        status = fn(*args, _raw_stream(i))
-    else:
-        with torch.cuda.device(i):
-            status = fn(*args, _raw_stream(i))
-    if status:
-        capi.check(status)
-
-
-# An eager call at decode sizes costs its host work, so the checks below are few attribute reads
-# (get_device() is negative for a CPU tensor) and form their messages only where they fail.
-def _require_rows(op, name, t, dtypes, kinds):
-    """The shape of t, a CUDA matrix of one of the dtypes whose rows are contiguous and do not overlap."""
-    if t.dtype not in dtypes or t.get_device() < 0:
-        raise RuntimeError(f"{op}: {name} must be {kinds} on CUDA")
-    shape = t.shape
-    if len(shape) != 2 or not (t.is_contiguous() or ((t.stride(1) == 1 or shape[1] <= 1)
-                                                     and (shape[0] <= 1 or t.stride(0) >= shape[1]))):
-        raise RuntimeError(f"{op}: {name} must be [rows, columns] with contiguous rows that do not overlap")
-    return shape
-
-
-def _require_vector(op, name, t, dtype, shape, like):
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != like.get_device() or not t.is_contiguous():
-        raise RuntimeError(f"{op}: {name} must be contiguous {str(dtype)[6:]} {list(shape)} on the inputs' device")
-
-
-def _ld(t, shape):
-    return t.stride(0) if shape[0] > 1 else max(shape[1], 1)
-
-
-def _ldc(t, shape):
-    # row stride of int8 codes; a single row has no next one, so its stride is what alignment asks for
-    return t.stride(0) if shape[0] > 1 else (shape[1] + 15) // 16 * 16
-
-
-_INT8 = (torch.int8,)
-_HALVES = (torch.bfloat16, torch.float16)
-_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
-
-
-def _code_rows(rows, K, like):
-    """int8 [rows, K] whose rows start 16 bytes apart or a multiple of it, as int8_gemm reads them."""
-    ld = (K + 15) // 16 * 16
-    codes = like.new_empty((rows, ld), dtype=torch.int8)
-    return (codes if ld == K else codes[:, :K]), ld
+_host = _HostModule()
 
 
 def dynamic_int8_quant(input):
@@ -769,18 +724,14 @@ def dynamic_int8_quant(input):
 
     An all-zero row gets scale 0, a row with an infinity or NaN scale NaN and codes 0.  Where K is
     not a multiple of 16 the codes are a view of rows padded to one, the form int8_gemm takes."""
-    M, K = shape = _require_rows("dynamic_int8_quant", "input", input, _HALVES, "BF16 or FP16")
-    codes, ldq = _code_rows(M, K, input)
-    scales = input.new_empty((M,), dtype=torch.float32)
-    _call(input, _lib.lsg_dynamic_int8_quant, input.data_ptr(), _ld(input, shape), _CODE[input.dtype],
-          codes.data_ptr(), ldq, scales.data_ptr(), M, K)
-    return codes, scales
+    return _host.dynamic_int8_quant(input)
 
 
 def weight_int8_quant(weight):
     """bf16 or fp16 [N,K] or [E,N,K] -> (codes int8 of that shape, scales fp32 [N] or [E,N]): one
     scale per output channel, as dynamic_int8_quant.  [E,N,K] needs K % 16 == 0."""
-    _require(weight.is_cuda and weight.dtype in _HALVES, "weight_int8_quant: weight must be BF16 or FP16 on CUDA")
+    _require(weight.is_cuda and weight.dtype in (torch.bfloat16, torch.float16),
+             "weight_int8_quant: weight must be BF16 or FP16 on CUDA")
     _require(weight.dim() in (2, 3) and weight.is_contiguous(),
              "weight_int8_quant: weight must be contiguous [N, K] or [E, N, K]")
     if weight.dim() == 2:
@@ -794,87 +745,35 @@ def weight_int8_quant(weight):
 def silu_mul_int8_quant(gate, up):
     """silu(gate) * up, formed in fp32, quantized per row: (codes int8 [M,K], scales fp32 [M]).
     gate, up: bf16, fp16 or fp32 [M,K] with contiguous rows (halves of one [M, 2K] matrix will do)."""
-    M, K = shape = _require_rows("silu_mul_int8_quant", "gate", gate, _FLOATS, "BF16, FP16 or FP32")
-    _require_rows("silu_mul_int8_quant", "up", up, _FLOATS, "BF16, FP16 or FP32")
-    _require(shape == up.shape and gate.dtype == up.dtype and gate.get_device() == up.get_device(),
-             "silu_mul_int8_quant: gate and up must have the same shape, dtype and device")
-    codes, ldq = _code_rows(M, K, gate)
-    scales = gate.new_empty((M,), dtype=torch.float32)
-    _call(gate, _lib.lsg_silu_mul_int8_quant, gate.data_ptr(), _ld(gate, shape), up.data_ptr(), _ld(up, shape),
-          _CODE[gate.dtype], codes.data_ptr(), ldq, scales.data_ptr(), M, K)
-    return codes, scales
+    return _host.silu_mul_int8_quant(gate, up)
 
 
 def int8_gemm(A, B, scale_A, scale_B, M, N, K, output_dtype):
     """D[m,n] = scale_A[m] * scale_B[n] * sum_k A[m,k] B[n,k] of int8 A [M,K] and B [N,K], the sum
     exact, one rounding to 'bf16', 'fp16' or 'fp32'.  1 <= K <= 131056; the rows of A and B start on
     16-byte boundaries (a view of padded rows where K is not a multiple of 16)."""
-    code, tdtype = _int8_out(output_dtype)
-    a = _require_rows("int8_gemm", "A", A, _INT8, "INT8")
-    b = _require_rows("int8_gemm", "B", B, _INT8, "INT8")
-    if a != (M, K):
-        raise RuntimeError("int8_gemm: A shape mismatch")
-    if b != (N, K) or A.get_device() != B.get_device():
-        raise RuntimeError("int8_gemm: B shape mismatch, or A and B on different devices")
-    _require_vector("int8_gemm", "scale_A", scale_A, torch.float32, (M,), A)
-    _require_vector("int8_gemm", "scale_B", scale_B, torch.float32, (N,), A)
-    D = A.new_empty((M, N), dtype=tdtype)
-    p = capi.Int8GemmParams(M, N, K, A.data_ptr(), _ldc(A, a), B.data_ptr(), _ldc(B, b), D.data_ptr(),
-                            scale_A.data_ptr(), scale_B.data_ptr(), code)
-    _call(A, _lib.lsg_int8_gemm, p)
-    return D
+    return _host.int8_gemm(A, B, scale_A, scale_B, M, N, K, output_dtype)
 
 
 def int8_gemm_from_bf16(x, weight, weight_scales, output_dtype="bf16"):
     """bf16 or fp16 x [M,K] quantized per token, times the int8 weight [N,K]: dynamic_int8_quant and
     int8_gemm in one call, the same bits."""
-    code, tdtype = _int8_out(output_dtype)
-    M, K = rows = _require_rows("int8_gemm_from_bf16", "x", x, _HALVES, "BF16 or FP16")
-    N, k = channels = _require_rows("int8_gemm_from_bf16", "weight", weight, _INT8, "INT8")
-    if k != K or weight.get_device() != x.get_device():
-        raise RuntimeError("int8_gemm_from_bf16: weight must be [N, K] on x's device")
-    _require_vector("int8_gemm_from_bf16", "weight_scales", weight_scales, torch.float32, (N,), x)
-    D = x.new_empty((M, N), dtype=tdtype)
-    ws_bytes = _lib.lsg_int8_gemm_from_bf16_workspace_bytes(M, K)
-    ws = x.new_empty((ws_bytes,), dtype=torch.uint8).data_ptr() if ws_bytes else None
-    p = capi.Int8GemmParams(M, N, K, x.data_ptr(), _ld(x, rows), weight.data_ptr(), _ldc(weight, channels),
-                            D.data_ptr(), None, weight_scales.data_ptr(), code)
-    _call(x, _lib.lsg_int8_gemm_from_bf16, p, _CODE[x.dtype], ws, ws_bytes)
-    return D
+    return _host.int8_gemm_from_bf16(x, weight, weight_scales, output_dtype)
 
 
 def int8_grouped_gemm(A_base, B_base, D_base, scale_A_base, scale_B_base, expert_offsets, N, K, output_dtype):
     """int8_gemm for rows grouped by expert, into D_base (returned): rows [offsets[e], offsets[e+1])
     of A_base [T,K] times B_base[e] of [E,N,K].  Routed on the device; rows behind the last expert's
     are left as they are."""
-    code, tdtype = _int8_out(output_dtype)
-    T, k = rows = _require_rows("int8_grouped_gemm", "A_base", A_base, _INT8, "INT8")
-    _require(k == K, "int8_grouped_gemm: A_base.size(1) != K")
-    E = B_base.size(0) if B_base.dim() else 0
-    _require_vector("int8_grouped_gemm", "B_base", B_base, torch.int8, (E, N, K), A_base)
-    _require_vector("int8_grouped_gemm", "D_base", D_base, tdtype, (T, N), A_base)
-    _require_vector("int8_grouped_gemm", "scale_A_base", scale_A_base, torch.float32, (T,), A_base)
-    _require_vector("int8_grouped_gemm", "scale_B_base", scale_B_base, torch.float32, (E, N), A_base)
-    _require_vector("int8_grouped_gemm", "expert_offsets", expert_offsets, torch.int32, (E + 1,), A_base)
-    p = capi.Int8GroupedGemmParams(E, N, K, A_base.data_ptr(), _ldc(A_base, rows), B_base.data_ptr(), K, D_base.data_ptr(),
-                                   scale_A_base.data_ptr(), scale_B_base.data_ptr(), expert_offsets.data_ptr(), code)
-    _call(A_base, _lib.lsg_int8_grouped_gemm, p, T)
-    return D_base
+    return _host.int8_grouped_gemm(A_base, B_base, D_base, scale_A_base, scale_B_base, expert_offsets, N, K,
+                                   output_dtype)
 
 
 def moe_permute_int8(hidden, inv_perm, top_k):
     """moe_permute and dynamic_int8_quant in one pass over bf16 or fp16 hidden [T,H]: (codes int8
     [T*k,H], scales fp32 [T*k]), row inv_perm[t*k+s] holding token t.  Pairs without a row
     (inv_perm < 0) are left out; rows no pair names are uninitialised."""
-    T, H = shape = _require_rows("moe_permute_int8", "hidden", hidden, _HALVES, "BF16 or FP16")
-    k = int(top_k)
-    _require(k >= 1, "moe_permute_int8: top_k must be positive")
-    _require_vector("moe_permute_int8", "inv_perm", inv_perm, torch.int32, (T * k,), hidden)
-    codes, ldq = _code_rows(T * k, H, hidden)
-    scales = hidden.new_empty((T * k,), dtype=torch.float32)
-    _call(hidden, _lib.lsg_moe_permute_int8, hidden.data_ptr(), _ld(hidden, shape), _CODE[hidden.dtype],
-          inv_perm.data_ptr(), T, k, H, codes.data_ptr(), ldq, scales.data_ptr())
-    return codes, scales
+    return _host.moe_permute_int8(hidden, inv_perm, top_k)
 
 
 def int8_moe_ffn(hidden, expert_offsets, inv_perm, top_k, gate_up, gate_up_scales, down, down_scales,
@@ -885,26 +784,8 @@ def int8_moe_ffn(hidden, expert_offsets, inv_perm, top_k, gate_up, gate_up_scale
     hidden bf16 or fp16 [T,H]; gate_up int8 [E,2I,H] (gate rows, then up rows) with scales fp32
     [E,2I]; down int8 [E,H,I] with scales fp32 [E,H]; H and I multiples of 16.  Rows behind the
     last expert's are uninitialised.  moe_unpermute takes the result back to the tokens."""
-    code, tdtype = _int8_out(output_dtype)
-    T, H = shape = _require_rows("int8_moe_ffn", "hidden", hidden, _HALVES, "BF16 or FP16")
-    k = int(top_k)
-    _require(k >= 1, "int8_moe_ffn: top_k must be positive")
-    _require(gate_up.dim() == 3 and down.dim() == 3, "int8_moe_ffn: gate_up must be [E, 2I, H] and down [E, H, I]")
-    E, I = gate_up.size(0), down.size(2)
-    _require_vector("int8_moe_ffn", "gate_up", gate_up, torch.int8, (E, 2 * I, H), hidden)
-    _require_vector("int8_moe_ffn", "down", down, torch.int8, (E, H, I), hidden)
-    _require_vector("int8_moe_ffn", "gate_up_scales", gate_up_scales, torch.float32, (E, 2 * I), hidden)
-    _require_vector("int8_moe_ffn", "down_scales", down_scales, torch.float32, (E, H), hidden)
-    _require_vector("int8_moe_ffn", "expert_offsets", expert_offsets, torch.int32, (E + 1,), hidden)
-    _require_vector("int8_moe_ffn", "inv_perm", inv_perm, torch.int32, (T * k,), hidden)
-    D = hidden.new_empty((T * k, H), dtype=tdtype)
-    ws_bytes = _lib.lsg_int8_moe_ffn_workspace_bytes(T, k, H, I)
-    ws = hidden.new_empty((max(ws_bytes, 1),), dtype=torch.uint8)
-    p = capi.Int8MoeFfnParams(T, k, E, H, I, hidden.data_ptr(), _ld(hidden, shape), _CODE[hidden.dtype],
-                              expert_offsets.data_ptr(), inv_perm.data_ptr(), gate_up.data_ptr(),
-                              gate_up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(), D.data_ptr(), code)
-    _call(hidden, _lib.lsg_int8_moe_ffn, p, ws.data_ptr(), ws_bytes)
-    return D
+    return _host.int8_moe_ffn(hidden, expert_offsets, inv_perm, top_k, gate_up, gate_up_scales, down, down_scales,
+                              output_dtype)
 
 
 # ---------------------------------------------------------------------------
@@ -949,15 +830,27 @@ def ep_expert_order(recv_counts, world, experts_per_rank, rows):
     return offs, order[:rows], inv[:rows]
 
 
+_CODE = {torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16, torch.float32: capi.DTYPE_F32}
+
+
+def _require_rows_of(op, t, others):
+    # t: the rows; others: (name, tensor, dtype, shape) that go with them
+    _require(t.is_cuda and t.dtype in _CODE and t.dim() == 2 and t.is_contiguous(),
+             f"{op}: rows must be contiguous BF16, FP16 or FP32 [rows, H] on CUDA")
+    for name, o, dtype, shape in others:
+        _require(o.device == t.device and o.dtype == dtype and o.is_contiguous() and tuple(o.shape) == shape,
+                 f"{op}: {name} must be contiguous {dtype} {shape} on the rows' device")
+
+
 def moe_permute(hidden, perm, top_k):
     """out[row] = hidden[perm[row] // top_k], bf16, fp16 or fp32 [T,H] -> [rows,H]."""
     rows, H = perm.numel(), hidden.size(1)
     if hidden.dtype != torch.bfloat16:
-        _require_dense("moe_permute", "hidden", hidden)
-        _require_vector("moe_permute", "perm", perm, torch.int32, (rows,), hidden)
-        out = hidden.new_empty((rows, H), dtype=hidden.dtype)
-        _call(hidden, _lib.lsg_moe_permute_dtype, hidden.data_ptr(), _CODE[hidden.dtype], perm.data_ptr(), rows,
-              hidden.size(0), int(top_k), H, out.data_ptr())
+        _require_rows_of("moe_permute", hidden, [("perm", perm, torch.int32, (rows,))])
+        with torch.cuda.device(hidden.device):
+            out = torch.empty((rows, H), dtype=hidden.dtype, device=hidden.device)
+            capi.check(_lib.lsg_moe_permute_dtype(hidden.data_ptr(), _CODE[hidden.dtype], perm.data_ptr(), rows,
+                                                  hidden.size(0), int(top_k), H, out.data_ptr(), _stream()))
         return out
     out = hidden.new_empty((rows, H), dtype=torch.bfloat16)
     capi.check(_lib.lsg_moe_permute(hidden.data_ptr(), perm.data_ptr(), rows, int(top_k), H, out.data_ptr(), _stream()))
@@ -970,12 +863,12 @@ def moe_unpermute(y, inv_perm, topk_weights):
     T, k = topk_weights.shape
     H = y.size(1)
     if y.dtype != torch.bfloat16:
-        _require_dense("moe_unpermute", "y", y)
-        _require_vector("moe_unpermute", "inv_perm", inv_perm, torch.int32, (T * k,), y)
-        _require_vector("moe_unpermute", "topk_weights", topk_weights, torch.float32, (T, k), y)
-        out = y.new_empty((T, H), dtype=y.dtype)
-        _call(y, _lib.lsg_moe_unpermute_dtype, y.data_ptr(), _CODE[y.dtype], inv_perm.data_ptr(),
-              topk_weights.data_ptr(), y.size(0), T, k, H, out.data_ptr())
+        _require_rows_of("moe_unpermute", y, [("inv_perm", inv_perm, torch.int32, (T * k,)),
+                                              ("topk_weights", topk_weights, torch.float32, (T, k))])
+        with torch.cuda.device(y.device):
+            out = torch.empty((T, H), dtype=y.dtype, device=y.device)
+            capi.check(_lib.lsg_moe_unpermute_dtype(y.data_ptr(), _CODE[y.dtype], inv_perm.data_ptr(),
+                                                    topk_weights.data_ptr(), y.size(0), T, k, H, out.data_ptr(), _stream()))
         return out
     out = y.new_empty((T, H), dtype=torch.bfloat16)
     capi.check(_lib.lsg_moe_unpermute(y.data_ptr(), inv_perm.data_ptr(), topk_weights.data_ptr(), T, k, H,
@@ -986,25 +879,11 @@ def moe_unpermute(y, inv_perm, topk_weights):
 # ---------------------------------------------------------------------------
 # Gradients of the MoE routing steps
 # ---------------------------------------------------------------------------
-def _require_dense(op, name, t):
-    if t.dtype not in _FLOATS or t.get_device() < 0 or t.dim() != 2 or not t.is_contiguous():
-        raise RuntimeError(f"{op}: {name} must be contiguous BF16, FP16 or FP32 [rows, H] on CUDA")
-    return t.shape
-
-
 def moe_permute_backward(grad_rows, inv_perm, top_k):
     """Gradient of moe_permute: grad_hidden[t] = sum over slots of grad_rows[inv_perm[t*k+s]], in
     fp32 in the order of the slots.  grad_rows bf16, fp16 or fp32 [rows,H] -> [T,H] of its type;
     pairs without a row (inv_perm < 0) add nothing."""
-    rows, H = _require_dense("moe_permute_backward", "grad_rows", grad_rows)
-    k, pairs = int(top_k), inv_perm.numel()
-    _require(k >= 1 and pairs % k == 0, "moe_permute_backward: inv_perm must hold top_k entries per token")
-    _require_vector("moe_permute_backward", "inv_perm", inv_perm, torch.int32, (pairs,), grad_rows)
-    T = pairs // k
-    out = grad_rows.new_empty((T, H))
-    _call(grad_rows, _lib.lsg_moe_permute_backward, grad_rows.data_ptr(), _CODE[grad_rows.dtype],
-          inv_perm.data_ptr(), rows, T, k, H, out.data_ptr())
-    return out
+    return _host.moe_permute_backward(grad_rows, inv_perm, top_k)
 
 
 def moe_unpermute_backward(grad_out, y, inv_perm, topk_weights, expert_offsets=None):
@@ -1015,39 +894,11 @@ def moe_unpermute_backward(grad_out, y, inv_perm, topk_weights, expert_offsets=N
     grad_out [T,H] and y [rows,H] bf16, fp16 or fp32, alike; grad_weights fp32 [T,k].  With
     expert_offsets (int32, as moe_permutation returns them) the rows behind the last expert's are
     cleared in grad_y; without them, rows that no pair names are uninitialised."""
-    op = "moe_unpermute_backward"
-    T, H = _require_dense(op, "grad_out", grad_out)
-    rows, h = _require_dense(op, "y", y)
-    if y.dtype is not grad_out.dtype or h != H or y.get_device() != grad_out.get_device():
-        raise RuntimeError(f"{op}: grad_out and y must have the same dtype, device and H")
-    _require(topk_weights.dim() == 2, "moe_unpermute_backward: topk_weights must be [T, k]")
-    k = topk_weights.size(1)
-    _require_vector(op, "topk_weights", topk_weights, torch.float32, (T, k), y)
-    _require_vector(op, "inv_perm", inv_perm, torch.int32, (T * k,), y)
-    if expert_offsets is not None:
-        _require(expert_offsets.dim() == 1 and expert_offsets.numel() >= 2, f"{op}: expert_offsets must be [E + 1]")
-        _require_vector(op, "expert_offsets", expert_offsets, torch.int32, expert_offsets.shape, y)
-    grad_y = torch.empty_like(y)
-    grad_w = torch.empty_like(topk_weights)
-    _call(y, _lib.lsg_moe_unpermute_backward, grad_out.data_ptr(), y.data_ptr(), _CODE[y.dtype],
-          inv_perm.data_ptr(), topk_weights.data_ptr(), expert_offsets.data_ptr() if expert_offsets is not None else None,
-          expert_offsets.numel() - 1 if expert_offsets is not None else 0, rows, T, k, H, grad_y.data_ptr(),
-          grad_w.data_ptr())
-    return grad_y, grad_w
+    return _host.moe_unpermute_backward(grad_out, y, inv_perm, topk_weights, expert_offsets)
 
 
 def moe_route_backward(topk_idx, topk_weights, grad_weights, num_experts):
     """Gradient of moe_route by its logits: fp32 [T,E] from the weights' gradient fp32 [T,k].  The
     weights are the softmax over the chosen logits, so grad_logits[t, topk_idx[t,s]] =
     w[t,s] * (grad_weights[t,s] - sum_r w[t,r] grad_weights[t,r]), and 0 elsewhere."""
-    op = "moe_route_backward"
-    if topk_idx.dtype is not torch.int32 or topk_idx.get_device() < 0 or topk_idx.dim() != 2 or not topk_idx.is_contiguous():
-        raise RuntimeError(f"{op}: topk_idx must be contiguous int32 [T, k] on CUDA")
-    T, k = topk_idx.shape
-    _require_vector(op, "topk_weights", topk_weights, torch.float32, (T, k), topk_idx)
-    _require_vector(op, "grad_weights", grad_weights, torch.float32, (T, k), topk_idx)
-    E = int(num_experts)
-    out = topk_weights.new_empty((T, E))
-    _call(topk_idx, _lib.lsg_moe_route_backward, topk_idx.data_ptr(), topk_weights.data_ptr(),
-          grad_weights.data_ptr(), T, E, k, out.data_ptr())
-    return out
+    return _host.moe_route_backward(topk_idx, topk_weights, grad_weights, num_experts)

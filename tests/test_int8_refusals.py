@@ -136,8 +136,10 @@ def test_moe_gradient_refusals(capi):
 
 
 def test_operators_refuse_cpu_tensors(capi):
-    torch = pytest.importorskip("torch")
+    import torch
     from layerstormgemmkernels_b200 import ops
+    from layerstormgemmkernels_b200.torch_ext import build_ext
+    build_ext.build_ops()
     x = torch.zeros(4, 64, dtype=torch.bfloat16)
     q = torch.zeros(8, 64, dtype=torch.int8)
     s = torch.ones(8)
