@@ -13,7 +13,8 @@ namespace lsg {
 
 namespace {
 
-int check(const char* op, int N, int K, const void* A, long long lda, const void* B, long long ldb, const void* D, int dt) {
+int check(const char* op, int K, const void* A, long long lda, const void* B, long long ldb, const void* D, int dt,
+          const float* sa, const float* sb) {
     if (dt != LSG_DTYPE_BF16 && dt != LSG_DTYPE_F16 && dt != LSG_DTYPE_F32)
         return fail(LSG_ERR_UNSUPPORTED, "%s: output dtype must be bf16, fp16 or f32", op);
     if (K < 1 || K > kInt8MaxK)
@@ -22,8 +23,9 @@ int check(const char* op, int N, int K, const void* A, long long lda, const void
     if (!A || !B || !D) return fail(LSG_ERR_INVALID, "%s: null pointer", op);
     if (((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) || lda % 16 || ldb % 16)
         return fail(LSG_ERR_ALIGNMENT, "%s: operand rows must start on 16-byte boundaries", op);
-    if (reinterpret_cast<uintptr_t>(D) & (dt == LSG_DTYPE_F32 ? 3 : 1))
-        return fail(LSG_ERR_ALIGNMENT, "%s: the output is not aligned to its type", op);
+    if ((reinterpret_cast<uintptr_t>(D) & (dt == LSG_DTYPE_F32 ? 3 : 1)) ||
+        ((reinterpret_cast<uintptr_t>(sa) | reinterpret_cast<uintptr_t>(sb)) & 3))
+        return fail(LSG_ERR_ALIGNMENT, "%s: the output or the scales are not aligned to their type", op);
     return LSG_OK;
 }
 
@@ -47,7 +49,7 @@ extern "C" int lsg_int8_gemm(const lsg_int8_gemm_params* p, void* stream) {
     if (!p) return fail(LSG_ERR_INVALID, "int8_gemm: null params");
     if (p->M < 0 || p->N < 0) return fail(LSG_ERR_INVALID, "int8_gemm: negative shape");
     if (p->M == 0 || p->N == 0) return LSG_OK;
-    const int rc = check("int8_gemm", p->N, p->K, p->A, p->lda, p->B, p->ldb, p->D, p->output_dtype);
+    const int rc = check("int8_gemm", p->K, p->A, p->lda, p->B, p->ldb, p->D, p->output_dtype, p->scale_A, p->scale_B);
     if (rc != LSG_OK) return rc;
     if (!p->scale_A || !p->scale_B) return fail(LSG_ERR_INVALID, "int8_gemm: null pointer");
     Int8Gemm a = {};
@@ -74,9 +76,10 @@ extern "C" int lsg_int8_gemm_from_bf16(const lsg_int8_gemm_params* p, int input_
     if (p->lda < p->K) return fail(LSG_ERR_INVALID, "int8_gemm_from_bf16: a row stride is smaller than K");
     // the activations may lie anywhere: the product reads their codes
     const long long ldq = pad16(p->K > 0 ? p->K : 0);
-    int rc = check("int8_gemm_from_bf16", p->N, p->K, p->B, ldq, p->B, p->ldb, p->D, p->output_dtype);
+    int rc = check("int8_gemm_from_bf16", p->K, p->B, ldq, p->B, p->ldb, p->D, p->output_dtype, nullptr, p->scale_B);
     if (rc != LSG_OK) return rc;
     if (!p->A || !p->scale_B) return fail(LSG_ERR_INVALID, "int8_gemm_from_bf16: null pointer");
+    if (reinterpret_cast<uintptr_t>(p->A) & 1) return fail(LSG_ERR_ALIGNMENT, "int8_gemm_from_bf16: the input is not aligned to its type");
     const size_t need = lsg_int8_gemm_from_bf16_workspace_bytes(p->M, p->K);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(LSG_ERR_WORKSPACE, "int8_gemm_from_bf16: workspace too small (have %zu, need %zu)",
@@ -105,7 +108,8 @@ extern "C" int lsg_int8_grouped_gemm(const lsg_int8_grouped_gemm_params* p, int 
     if (p->num_experts < 0 || total_tokens < 0 || p->N < 0) return fail(LSG_ERR_INVALID, "int8_grouped_gemm: negative shape");
     if (p->num_experts > 1024) return fail(LSG_ERR_INVALID, "int8_grouped_gemm: at most 1024 experts (E=%d)", p->num_experts);
     if (p->num_experts == 0 || total_tokens == 0 || p->N == 0) return LSG_OK;
-    const int rc = check("int8_grouped_gemm", p->N, p->K, p->A_base, p->lda, p->B_base, p->ldb, p->D_base, p->output_dtype);
+    const int rc = check("int8_grouped_gemm", p->K, p->A_base, p->lda, p->B_base, p->ldb, p->D_base, p->output_dtype,
+                         p->scale_A_base, p->scale_B_base);
     if (rc != LSG_OK) return rc;
     if (!p->scale_A_base || !p->scale_B_base || !p->expert_offsets)
         return fail(LSG_ERR_INVALID, "int8_grouped_gemm: null pointer");
@@ -169,8 +173,10 @@ extern "C" int lsg_int8_moe_ffn(const lsg_int8_moe_ffn_params* p, void* workspac
     if (reinterpret_cast<uintptr_t>(workspace) & 255)
         return fail(LSG_ERR_ALIGNMENT, "int8_moe_ffn: workspace must be 256-byte aligned");
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    int rc = check("int8_moe_ffn", 2 * I, H, ws, f.ldh, p->gate_up, H, ws, LSG_DTYPE_F32);
-    if (rc == LSG_OK) rc = check("int8_moe_ffn", H, I, ws, f.ldi, p->down, I, p->D, p->output_dtype);
+    int rc = check("int8_moe_ffn", H, ws, f.ldh, p->gate_up, H, ws, LSG_DTYPE_F32, p->gate_up_scales, nullptr);
+    if (rc == LSG_OK) rc = check("int8_moe_ffn", I, ws, f.ldi, p->down, I, p->D, p->output_dtype, p->down_scales, nullptr);
+    if (rc == LSG_OK && (reinterpret_cast<uintptr_t>(p->hidden) & 1))
+        rc = fail(LSG_ERR_ALIGNMENT, "int8_moe_ffn: hidden is not aligned to its type");
     if (rc != LSG_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     int8_t* codes = reinterpret_cast<int8_t*>(ws + f.codes);

@@ -145,7 +145,7 @@ int8_gemv_kernel(const Int8Gemm a, int ldq, int slots, unsigned int* status, lon
             // give up, but not before the copies behind this one have landed
             for (int j = 1; j < slots && i + j < pieces; ++j) {
                 const int other = (slot + j) % slots;
-                mbar_wait_bounded(&full[other][warp], (lap + (slot + j >= slots ? 1 : 0)) & 1, status, kDevWaitFull, 2000u, limit);
+                mbar_wait_bounded(&full[other][warp], (lap + (slot + j >= slots ? 1 : 0)) & 1, status, kDevWaitFull);
             }
             return;
         }

@@ -71,8 +71,10 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// Release at CTA scope: what the arrival hands over are tensor-memory reads that have completed.  At cluster
+// scope it would wait for the epilogue's stores to global memory (a quarter of the time of short-K tiles).
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // cta_group::2: the barrier may be the other CTA's of the pair.
@@ -384,7 +386,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             if (CG == 1 || rank == 0)
                 for (int i = 0; i < a.stages; ++i) {
                     const uint32_t n = lap + (i < s ? 1 : 0);   // times stage i was filled
-                    if (n > 0) mbar_wait_bounded(&full[i], (n - 1) & 1, a.status, kDevWaitFull, 2000u, a.limit);
+                    if (n > 0) mbar_wait_bounded(&full[i], (n - 1) & 1, a.status, kDevWaitFull);
                 }
         }
     } else if (warp == kEpiWarps + 1) {
@@ -506,6 +508,16 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                         else store_column(static_cast<float*>(a.D) + at, a.N, v, count);
                     }
                 };
+                // the accumulator is free for the next tile but one when its last piece is in registers
+                auto hand_back = [&] {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (elect_one()) {
+                        if (CG == 2) arrive_remote(map_to_rank(smem_u32(&acc_empty[ab]), 0));
+                        else mbar_arrive(&acc_empty[ab]);
+                    }
+                    __syncwarp();
+                };
                 // two pieces in registers: one is read while the other is worked on
                 uint32_t r0[16], r1[16];
                 int c = group * 16;
@@ -513,22 +525,22 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                     tmem_ld16(src + c, r0);
                     tmem_ld_wait(r0);
                 }
+                if (c + kPieces >= t.rows) hand_back();
                 while (c < t.rows) {
                     if (c + kPieces < t.rows) tmem_ld16(src + c + kPieces, r1);
                     piece(r0, c);
-                    if (c + kPieces >= t.rows) break;
+                    c += kPieces;
+                    if (c >= t.rows) break;
                     tmem_ld_wait(r1);
-                    if (c + 2 * kPieces < t.rows) tmem_ld16(src + c + 2 * kPieces, r0);
-                    piece(r1, c + kPieces);
-                    if (c + 2 * kPieces < t.rows) tmem_ld_wait(r0);
-                    c += 2 * kPieces;
+                    if (c + kPieces < t.rows) tmem_ld16(src + c + kPieces, r0);
+                    else hand_back();
+                    piece(r1, c);
+                    c += kPieces;
+                    if (c >= t.rows) break;
+                    tmem_ld_wait(r0);
+                    if (c + kPieces >= t.rows) hand_back();
                 }
-                tc_fence_before();
                 __syncwarp();
-                if (elect_one()) {
-                    if (CG == 2) arrive_remote(map_to_rank(smem_u32(&acc_empty[ab]), 0));
-                    else mbar_arrive(&acc_empty[ab]);
-                }
                 ab ^= 1;
                 acc_lap += ab == 0;
             }
@@ -651,6 +663,7 @@ int round_up(int v, int step) { return (v + step - 1) / step * step; }
 // the row quantizer launched right in front.  That kernel lets this one start only after its own wait,
 // so everything launched before it has ended: offsets are read and weights loaded while it still runs.
 int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
+    if (g.M > 0x7fffffff - 512 || g.N > 0x7fffffff - 512) return fail(LSG_ERR_UNSUPPORTED, "int8 product: too many rows");
     MmaArgs a = {};
     a.D = g.D; a.out_dtype = g.out_dtype; a.sA = g.scale_A; a.sB = g.scale_B; a.offsets = g.expert_offsets;
     a.M = g.M; a.N = g.N; a.E = g.E; a.kblocks = (g.K + kKB - 1) / kKB;

@@ -232,8 +232,8 @@ int launch_rows(const RowQuantArgs& a, long long rows, cudaStream_t s) {
 }
 
 // Shape and pointer checks shared by the entries; `ld` in values, ldq in bytes.
-int check_rows(const char* op, int dtype, bool f32_ok, long long rows, int K, long long ld, const void* codes,
-               long long ldq) {
+int check_rows(const char* op, int dtype, bool f32_ok, long long rows, int K, uintptr_t x, long long ld, const void* codes,
+               long long ldq, const float* scales) {
     if (dtype != LSG_DTYPE_BF16 && dtype != LSG_DTYPE_F16 && !(f32_ok && dtype == LSG_DTYPE_F32))
         return fail(LSG_ERR_UNSUPPORTED, "%s: input must be bf16 or fp16%s", op, f32_ok ? " or f32" : "");
     if (rows < 0 || K < 0) return fail(LSG_ERR_INVALID, "%s: negative shape", op);
@@ -241,6 +241,8 @@ int check_rows(const char* op, int dtype, bool f32_ok, long long rows, int K, lo
     if (ld < K || ldq < K) return fail(LSG_ERR_INVALID, "%s: a row stride is smaller than the row", op);
     if (ldq % 16 != 0 || (reinterpret_cast<uintptr_t>(codes) & 15))
         return fail(LSG_ERR_ALIGNMENT, "%s: code rows must start on 16-byte boundaries", op);
+    if ((x & (dtype == LSG_DTYPE_F32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(scales) & 3))
+        return fail(LSG_ERR_ALIGNMENT, "%s: a buffer is not aligned to its type", op);
     return LSG_OK;
 }
 
@@ -269,7 +271,7 @@ using namespace lsg;
 
 extern "C" int lsg_dynamic_int8_quant(const void* x, long long ldx, int dtype, void* codes, long long ldq, float* scales,
                                       long long rows, int K, void* stream) {
-    const int rc = check_rows("dynamic_int8_quant", dtype, false, rows, K, ldx, codes, ldq);
+    const int rc = check_rows("dynamic_int8_quant", dtype, false, rows, K, reinterpret_cast<uintptr_t>(x), ldx, codes, ldq, scales);
     if (rc != LSG_OK) return rc;
     if (rows == 0) return LSG_OK;
     if (!scales || (K > 0 && (!x || !codes))) return fail(LSG_ERR_INVALID, "dynamic_int8_quant: null pointer");
@@ -279,7 +281,8 @@ extern "C" int lsg_dynamic_int8_quant(const void* x, long long ldx, int dtype, v
 
 extern "C" int lsg_silu_mul_int8_quant(const void* gate, long long ldg, const void* up, long long ldu, int dtype,
                                        void* codes, long long ldq, float* scales, long long rows, int K, void* stream) {
-    int rc = check_rows("silu_mul_int8_quant", dtype, true, rows, K, ldg < ldu ? ldg : ldu, codes, ldq);
+    int rc = check_rows("silu_mul_int8_quant", dtype, true, rows, K, reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(up),
+                        ldg < ldu ? ldg : ldu, codes, ldq, scales);
     if (rc != LSG_OK) return rc;
     if (rows == 0) return LSG_OK;
     if (!scales || (K > 0 && (!gate || !up || !codes))) return fail(LSG_ERR_INVALID, "silu_mul_int8_quant: null pointer");
@@ -289,7 +292,7 @@ extern "C" int lsg_silu_mul_int8_quant(const void* gate, long long ldg, const vo
 
 extern "C" int lsg_moe_permute_int8(const void* hidden, long long ld, int dtype, const int32_t* inv_perm, int num_tokens,
                                     int top_k, int H, void* codes, long long ldq, float* scales, void* stream) {
-    int rc = check_rows("moe_permute_int8", dtype, false, num_tokens, H, ld, codes, ldq);
+    int rc = check_rows("moe_permute_int8", dtype, false, num_tokens, H, reinterpret_cast<uintptr_t>(hidden), ld, codes, ldq, scales);
     if (rc != LSG_OK) return rc;
     if (top_k < 1 || static_cast<long long>(num_tokens) * top_k > 0x7fffffffll)
         return fail(LSG_ERR_INVALID, "moe_permute_int8: need top_k >= 1 and at most 2^31 - 1 pairs");

@@ -334,13 +334,16 @@ int unpermute_backward(const void* grad_out, const void* y, const int32_t* inv, 
     return LSG_BY_SLOTS(launch_unpermute_backward, 1, grad_out, y, inv, w, used, rows, tokens, k, H, grad_y, grad_w, s);
 }
 
-int check_moe(const char* op, int dtype, int tokens, int k, int H) {
+int check_moe(const char* op, int dtype, int tokens, int k, int H, const void* a, const void* b, const void* c = nullptr) {
     if (dtype != LSG_DTYPE_BF16 && dtype != LSG_DTYPE_F16 && dtype != LSG_DTYPE_F32)
         return fail(LSG_ERR_UNSUPPORTED, "%s: dtype must be bf16, fp16 or f32", op);
     if (tokens < 0 || H < 0) return fail(LSG_ERR_INVALID, "%s: negative shape", op);
     if (k < 1 || k > kMaxSlots) return fail(LSG_ERR_INVALID, "%s: need 1 <= top_k <= %d (k=%d)", op, kMaxSlots, k);
     if (static_cast<long long>(tokens) * k > 0x7fffffffll)
         return fail(LSG_ERR_INVALID, "%s: more than 2^31 - 1 pairs", op);
+    const uintptr_t size = dtype == LSG_DTYPE_F32 ? 4 : 2;
+    if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & (size - 1)) != 0)
+        return fail(LSG_ERR_ALIGNMENT, "%s: a buffer is not aligned to its type", op);
     return LSG_OK;
 }
 
@@ -355,7 +358,7 @@ using namespace lsg;
 
 extern "C" int lsg_moe_permute_dtype(const void* hidden, int dtype, const int32_t* perm, int rows, int num_tokens,
                                      int top_k, int H, void* out, void* stream) {
-    const int rc = check_moe("moe_permute", dtype, num_tokens, top_k, H);
+    const int rc = check_moe("moe_permute", dtype, num_tokens, top_k, H, hidden, out);
     if (rc != LSG_OK) return rc;
     if (rows <= 0 || H == 0) return rows < 0 ? fail(LSG_ERR_INVALID, "moe_permute: negative shape") : LSG_OK;
     if (!hidden || !perm || !out) return fail(LSG_ERR_INVALID, "moe_permute: null pointer");
@@ -364,7 +367,7 @@ extern "C" int lsg_moe_permute_dtype(const void* hidden, int dtype, const int32_
 
 extern "C" int lsg_moe_unpermute_dtype(const void* y, int dtype, const int32_t* inv_perm, const float* topk_weights, int rows,
                                        int num_tokens, int top_k, int H, void* out, void* stream) {
-    const int rc = check_moe("moe_unpermute", dtype, num_tokens, top_k, H);
+    const int rc = check_moe("moe_unpermute", dtype, num_tokens, top_k, H, y, out);
     if (rc != LSG_OK) return rc;
     if (rows < 0) return fail(LSG_ERR_INVALID, "moe_unpermute: negative shape");
     if (num_tokens == 0 || H == 0) return LSG_OK;
@@ -374,7 +377,7 @@ extern "C" int lsg_moe_unpermute_dtype(const void* y, int dtype, const int32_t* 
 
 extern "C" int lsg_moe_permute_backward(const void* grad_rows, int dtype, const int32_t* inv_perm, int rows, int num_tokens,
                                         int top_k, int H, void* grad_hidden, void* stream) {
-    const int rc = check_moe("moe_permute_backward", dtype, num_tokens, top_k, H);
+    const int rc = check_moe("moe_permute_backward", dtype, num_tokens, top_k, H, grad_rows, grad_hidden);
     if (rc != LSG_OK) return rc;
     if (rows < 0) return fail(LSG_ERR_INVALID, "moe_permute_backward: negative shape");
     if (num_tokens == 0 || H == 0) return LSG_OK;
@@ -387,7 +390,7 @@ extern "C" int lsg_moe_permute_backward(const void* grad_rows, int dtype, const 
 extern "C" int lsg_moe_unpermute_backward(const void* grad_out, const void* y, int dtype, const int32_t* inv_perm,
                                           const float* topk_weights, const int32_t* expert_offsets, int num_experts, int rows,
                                           int num_tokens, int top_k, int H, void* grad_y, float* grad_weights, void* stream) {
-    const int rc = check_moe("moe_unpermute_backward", dtype, num_tokens, top_k, H);
+    const int rc = check_moe("moe_unpermute_backward", dtype, num_tokens, top_k, H, grad_out, y, grad_y);
     if (rc != LSG_OK) return rc;
     if (rows < 0) return fail(LSG_ERR_INVALID, "moe_unpermute_backward: negative shape");
     if (rows > static_cast<long long>(num_tokens) * top_k)

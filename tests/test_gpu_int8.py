@@ -130,8 +130,8 @@ def test_weight_quant(ops, dtype):
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("M,K", [(1, 16), (3, 77), (9, 768), (5, 2056), (4, 14336), (2, 16400)])
 def test_silu_mul_quant(ops, dtype, M, K):
-    """silu(g) * u in fp32 is at most 2^-20 (relative) off: expf two ulp, an addition, a division and a
-    product half an ulp each, 3.5 * 2^-23.  A code is the nearest integer to a quotient of at most 127
+    """silu(g) * u in fp32 is at most 2^-20 (relative) off: expf and the quotient two ulp each, an addition
+    and a product half an ulp, 5 * 2^-23.  A code is the nearest integer to a quotient of at most 127
     with the errors of value and maximum, so |code - quotient| <= 0.5 + 127 * 2^-19."""
     g = torch.Generator().manual_seed(M + K)
     both = (torch.randn(M, 2 * K, generator=g) * 2).to(dtype)
@@ -160,7 +160,7 @@ def test_silu_mul_far_gates(ops):
 # -----------------------------------------------------------------------------------------
 # Products
 # -----------------------------------------------------------------------------------------
-DENSE = [(1, 1, 1), (1, 7, 16), (1, 128, 4096), (2, 1000, 1008), (3, 257, 333), (4, 64, 64), (5, 129, 2048), (8, 1024, 14336),
+DENSE = [(1, 1, 1), (1, 7, 16), (1, 128, 4096), (2, 1000, 1008), (3, 257, 333), (4, 64, 64), (3, 40, 1), (9, 17, 7), (20, 300, 15), (260, 9500, 40), (5, 129, 2048), (8, 1024, 14336),
          (9, 300, 4096), (16, 515, 1040), (17, 4099, 512), (31, 128, 144), (33, 96, 4000), (64, 640, 2064), (65, 1, 4096),
          (77, 2048, 7168), (127, 255, 100), (128, 256, 128), (129, 257, 2304), (200, 3000, 1024), (256, 512, 4096),
          (257, 1025, 513), (300, 4096, 1024), (511, 130, 2000), (1000, 777, 1552), (1024, 2048, 2048),
@@ -414,6 +414,88 @@ def test_two_streams_at_once(ops, M):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(d, want[i]) for d in got[i])
+
+
+@pytest.mark.parametrize("M", [1, 2, 8, 60, 300])
+def test_weights_made_right_before(ops, M):
+    """The weight is quantized by the launch in front of the product, into memory that held the weight of
+    the call before: nothing of the product may read it earlier than that launch has ended."""
+    g = torch.Generator().manual_seed(M)
+    N, K = 9600, 512
+    x = torch.randn(M, K, generator=g).to(BF16).cuda()
+    hidden_codes, hidden_scales = ops.dynamic_int8_quant(x)
+    src = [(torch.randn(N, K, generator=g) * 0.02).to(BF16).cuda() for _ in range(3)]
+    want = []
+    for w in src:
+        codes, scales = ops.weight_int8_quant(w)
+        torch.cuda.synchronize()
+        want.append(ops.int8_gemm_from_bf16(x, codes, scales))
+        torch.cuda.synchronize()
+        del codes, scales
+    got = []
+    for i in range(12):
+        codes, scales = ops.weight_int8_quant(src[i % 3])
+        got.append(ops.int8_gemm(hidden_codes, codes, hidden_scales, scales, M, N, K, "bf16"))
+        codes, scales = ops.weight_int8_quant(src[i % 3])
+        got.append(ops.int8_gemm_from_bf16(x, codes, scales))
+        del codes, scales
+    torch.cuda.synchronize()
+    for i, d in enumerate(got):
+        assert torch.equal(d, want[(i // 2) % 3]), i
+
+
+@pytest.mark.parametrize("T", [3, 400])
+def test_experts_on_two_streams(ops, T):
+    g = torch.Generator().manual_seed(T)
+    E, k, H, I = 8, 2, 512, 256
+    gate_up, gus, down, ds = experts(g, E, H, I)
+    sets = []
+    for _ in range(2):
+        hidden = torch.randn(T, H, generator=g).to(BF16).cuda()
+        idx, _ = ops.moe_route(torch.randn(T, E, generator=g).cuda(), k)
+        offs, _, inv = ops.moe_permutation(idx, E)
+        sets.append((hidden, offs, inv))
+    want = [ops.int8_moe_ffn(h, o, i, k, gate_up, gus, down, ds) for h, o, i in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(10):
+        for j, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                h, o, i = sets[j]
+                got[j].append(ops.int8_moe_ffn(h, o, i, k, gate_up, gus, down, ds))
+    torch.cuda.synchronize()
+    for j in range(2):
+        assert all(torch.equal(d, want[j]) for d in got[j])
+
+
+def test_offsets_that_fall(ops):
+    """Offsets are taken as a rising sequence inside [0, T]: what falls or lies outside makes experts empty
+    and never reaches past the rows."""
+    g = torch.Generator().manual_seed(21)
+    A, B = rand_codes(g, 64, 256), torch.randint(-127, 128, (4, 96, 256), generator=g, dtype=torch.int8).cuda()
+    one, sb = torch.ones(64, device="cuda"), torch.ones(4, 96, device="cuda")
+    D = torch.full((64, 96), -1.0, device="cuda")
+    ops.int8_grouped_gemm(A, B, D, one, sb, torch.tensor([-3, 20, 5, 30, 1 << 30], dtype=torch.int32, device="cuda"), 96, 256, "fp32")
+    for e, (a, b) in enumerate(((0, 20), (20, 20), (20, 30), (30, 64))):
+        assert torch.equal(D[a:b].double(), A[a:b].double() @ B[e].double().t())
+
+
+@pytest.mark.parametrize("E", [1, 300, 1024])
+def test_many_experts(ops, E):
+    g = torch.Generator().manual_seed(E)
+    counts = torch.randint(0, 4, (E,), generator=g).tolist()
+    counts[E // 2] = 37
+    T, N, K = sum(counts), 64, 128
+    A, B = rand_codes(g, T, K), torch.randint(-127, 128, (E, N, K), generator=g, dtype=torch.int8).cuda()
+    sa, sb = torch.rand(T, generator=g).cuda(), torch.rand(E, N, generator=g).cuda()
+    offs = offsets_of(counts)
+    D = torch.empty(T, N, device="cuda")
+    ops.int8_grouped_gemm(A, B, D, sa, sb, offs.cuda(), N, K, "fp32")
+    expert = torch.repeat_interleave(torch.arange(E), torch.tensor(counts)).cuda()
+    acc = torch.bmm(B[expert].double(), A.double().unsqueeze(-1)).squeeze(-1)
+    ref = acc * sa.double().unsqueeze(1) * sb.double()[expert]
+    assert bool(((D.double() - ref).abs() <= 4 * 2.0 ** -24 * ref.abs()).all())
 
 
 def test_refused_on_cuda(ops):

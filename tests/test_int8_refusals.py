@@ -24,6 +24,7 @@ def gemm(capi, **kw):
     (dict(scale_A=None), ValueError, "null"), (dict(scale_B=None), ValueError, "null"), (dict(D=None), ValueError, "null"),
     (dict(A=P + 8), RuntimeError, "16-byte"), (dict(B=P + 1), RuntimeError, "16-byte"), (dict(lda=72), RuntimeError, "16-byte"),
     (dict(ldb=65), RuntimeError, "16-byte"), (dict(D=P + 1), RuntimeError, "aligned"), (dict(D=P + 2, output_dtype=1), RuntimeError, "aligned"),
+    (dict(scale_A=P + 2), RuntimeError, "aligned"), (dict(scale_B=P + 1), RuntimeError, "aligned"),
     (dict(output_dtype=3), RuntimeError, "bf16, fp16 or f32")])
 def test_gemm_refusals(capi, kw, error, text):
     with pytest.raises(error, match=text):
@@ -49,7 +50,7 @@ def test_gemm_from_bf16_refusals(capi):
     for kw, error, text in ((dict(dtype=1), RuntimeError, "bf16 or fp16"), (dict(ws=None), RuntimeError, "workspace"),
                             (dict(size=need - 1), RuntimeError, "workspace"), (dict(ws=P + 16), RuntimeError, "256-byte"),
                             (dict(lda=63), ValueError, "stride"), (dict(K=0), ValueError, "1 <= K"), (dict(A=None), ValueError, "null"),
-                            (dict(ldb=72), RuntimeError, "16-byte")):
+                            (dict(ldb=72), RuntimeError, "16-byte"), (dict(A=P + 1), RuntimeError, "aligned")):
         with pytest.raises(error, match=text):
             call(**kw)
 
@@ -60,7 +61,8 @@ def test_quantizer_refusals(capi):
     for kw, error, text in ((dict(dtype=1), RuntimeError, "bf16 or fp16"), (dict(rows=-1), ValueError, "negative"),
                             (dict(rows=1 << 31), ValueError, "rows"), (dict(ldx=63), ValueError, "stride"),
                             (dict(ldq=48), ValueError, "stride"), (dict(ldq=72), RuntimeError, "16-byte"),
-                            (dict(codes=P + 4), RuntimeError, "16-byte"), (dict(x=None), ValueError, "null"),
+                            (dict(codes=P + 4), RuntimeError, "16-byte"), (dict(x=P + 1), RuntimeError, "aligned"),
+                            (dict(scales=P + 2), RuntimeError, "aligned"), (dict(x=None), ValueError, "null"),
                             (dict(scales=None), ValueError, "null")):
         with pytest.raises(error, match=text):
             quant(**kw)
@@ -124,6 +126,8 @@ def test_moe_gradient_refusals(capi):
             (L.lsg_moe_unpermute_backward, (P, P, 0, P, P, P, 0, 8, 4, 2, 64, P, P, None), ValueError, "num_experts"),
             (L.lsg_moe_unpermute_backward, (P, None, 0, P, P, None, 0, 8, 4, 2, 64, P, P, None), ValueError, "null"),
             (L.lsg_moe_unpermute_backward, (P, P, 0, P, P, None, 0, 8, 4, 2, -64, P, P, None), ValueError, "negative"),
+            (L.lsg_moe_permute_backward, (P + 2, 1, P, 8, 4, 2, 64, P, None), RuntimeError, "aligned"),
+            (L.lsg_moe_unpermute_backward, (P, P + 1, 0, P, P, None, 0, 8, 4, 2, 64, P, P, None), RuntimeError, "aligned"),
             (L.lsg_moe_route_backward, (P, P, P, 4, 2000, 2, P, None), ValueError, "E <= 1024"),
             (L.lsg_moe_route_backward, (P, P, P, 4, 2, 3, P, None), ValueError, "top_k"),
             (L.lsg_moe_route_backward, (P, P, None, 4, 8, 2, P, None), ValueError, "null"),
