@@ -28,7 +28,7 @@ int int8_gemm(const Int8Gemm& a, bool early, cudaStream_t s);
 // A few rows on a streaming mat-vec (int8_gemv.cu): whether a call of these sizes goes there, and the
 // call, with A as codes (x_dtype < 0) or as bf16 / fp16 activations that it quantizes on the way (lda in
 // values, scale_A unused).
-bool int8_gemv_takes(int M, int K);
+bool int8_gemv_takes(int M, int N, int K);
 int int8_gemv(const Int8Gemm& a, int x_dtype, cudaStream_t s);
 // On the tensor cores (int8_mma.cu).  swiglu: B is [E, 2 N, K], gate rows in front of up rows, and D
 // fp32 silu(gate) * up.  early: the launch in front on the stream is int8_quant_rows, which writes A.

@@ -32,7 +32,7 @@ int check(const char* op, int K, const void* A, long long lda, const void* B, lo
 }  // namespace
 
 int int8_gemm(const Int8Gemm& a, bool early, cudaStream_t s) {
-    if (!a.expert_offsets && int8_gemv_takes(a.M, a.K)) return int8_gemv(a, -1, s);
+    if (!a.expert_offsets && int8_gemv_takes(a.M, a.N, a.K)) return int8_gemv(a, -1, s);
     return int8_mma(a, false, early, s);
 }
 
@@ -62,7 +62,7 @@ extern "C" int lsg_int8_gemm(const lsg_int8_gemm_params* p, void* stream) {
 }
 
 extern "C" size_t lsg_int8_gemm_from_bf16_workspace_bytes(int M, int K) {
-    if (M <= 0 || K <= 0 || int8_gemv_takes(M, K)) return 0;
+    if (M <= 0 || K <= 0 || (M == 1 && int8_gemv_takes(1, 1, K))) return 0;   // quantized inside the mat-vec
     return a256(static_cast<size_t>(M) * pad16(K)) + a256(static_cast<size_t>(M) * 4);
 }
 
@@ -91,7 +91,7 @@ extern "C" int lsg_int8_gemm_from_bf16(const lsg_int8_gemm_params* p, int input_
     a.B = static_cast<const int8_t*>(p->B); a.ldb = p->ldb;
     a.D = p->D; a.out_dtype = p->output_dtype; a.scale_B = p->scale_B;
     a.M = p->M; a.N = p->N; a.K = p->K; a.E = 1;
-    if (need == 0) {
+    if (int8_gemv_takes(p->M, p->N, p->K)) {
         a.A = static_cast<const int8_t*>(p->A); a.lda = p->lda;
         return int8_gemv(a, input_dtype, s);
     }

@@ -10,7 +10,7 @@
 // scale is rounded, so quotients next to a half-way point fall on either side of it.
 //
 // The activation silu(g) * u of silu_mul stays in fp32 up to its code (rounding it to bf16 first
-// moves one value in fifteen by a code).
+// moves one code in eighty).
 //
 // Memory bound: one CTA per row, the row held in registers between the maximum and the codes, so
 // that every input byte is read once.  Rows that are not whole 16-byte pieces, or longer than

@@ -845,7 +845,7 @@ def _require_rows_of(op, t, others):
 def moe_permute(hidden, perm, top_k):
     """out[row] = hidden[perm[row] // top_k], bf16, fp16 or fp32 [T,H] -> [rows,H]."""
     rows, H = perm.numel(), hidden.size(1)
-    if hidden.dtype != torch.bfloat16:
+    if hidden.dtype != torch.bfloat16 or H % 8:      # lsg_moe_permute copies whole 16-byte pieces of bf16
         _require_rows_of("moe_permute", hidden, [("perm", perm, torch.int32, (rows,))])
         with torch.cuda.device(hidden.device):
             out = torch.empty((rows, H), dtype=hidden.dtype, device=hidden.device)
@@ -862,7 +862,7 @@ def moe_unpermute(y, inv_perm, topk_weights):
     without a row (inv_perm < 0) add nothing."""
     T, k = topk_weights.shape
     H = y.size(1)
-    if y.dtype != torch.bfloat16:
+    if y.dtype != torch.bfloat16 or H % 2:           # lsg_moe_unpermute takes bf16 in pairs
         _require_rows_of("moe_unpermute", y, [("inv_perm", inv_perm, torch.int32, (T * k,)),
                                               ("topk_weights", topk_weights, torch.float32, (T, k))])
         with torch.cuda.device(y.device):
