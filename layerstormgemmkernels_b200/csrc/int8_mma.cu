@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace lsg {
 
@@ -38,6 +39,7 @@ namespace {
 constexpr int kRows = 128;                   // weight rows of a CTA
 constexpr int kKB = 128;                     // bytes of K in a stage
 constexpr int kABytes = kRows * kKB;
+template <bool WIDE> constexpr int kPairBlocks = WIDE ? 2 : 1;   // K blocks of a pair's stage
 constexpr int kEpiGroups = 2;               // of four warps: 128 lanes of tensor memory
 constexpr int kEpiWarps = 4 * kEpiGroups;
 constexpr int kPieces = 16 * kEpiGroups;     // columns from one piece of a warp to its next
@@ -92,16 +94,16 @@ __device__ __forceinline__ void tma_5d(void* dst, const CUtensorMap* map, int x,
             : "memory");
 }
 template <int CG>
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     if constexpr (CG == 2)
         asm volatile(
-            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-            ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar)
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+            ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
             : "memory");
     else
         asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-            ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar)
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+            ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
             : "memory");
 }
 template <int CG>
@@ -221,12 +223,12 @@ __device__ __forceinline__ Tile tile_of(const MmaArgs& a, const int* cum, const 
     return t;
 }
 
-template <int CG, bool SWIGLU, int SPLIT>
+template <int CG, bool SWIGLU, int SPLIT, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1)
 int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const MmaArgs a) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int sub = CG == 2 ? 1 : a.sub;
+    const int sub = CG == 2 ? kPairBlocks<WIDE> : a.sub;
     const int stage_bytes = sub * a.block_bytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + a.stages * stage_bytes);
     uint64_t* empty = full + kMaxStages;
@@ -333,18 +335,24 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         int s = 0;
         uint32_t lap = 0;
         bool ok = true;
-        const int blocks_all = CG == 2 ? 1 : sub;
+        
+        const uint32_t full_at = CG == 2 ? map_to_rank(smem_u32(full), 0) : smem_u32(full);   // the leader's barriers
         // the weights of stage i, K blocks kb.., and the bytes that its barrier waits for
         auto load_weights = [&](int i, int kb, const Tile& t, int n_cta, int blocks) {
             uint8_t* dst = smem + i * stage_bytes;
-            const uint32_t bar = CG == 2 ? map_to_rank(smem_u32(&full[i]), 0) : smem_u32(&full[i]);
+            const uint32_t bar = full_at + 8 * i;
             // the leader's barrier counts the bytes of both CTAs
-            if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[i], CG * blocks * (kABytes + a.tn * kKB));
-            for (int j = 0; j < blocks; ++j) {
-                if constexpr (SWIGLU)
-                    tma_5d<CG>(dst + j * a.block_bytes, &tmW, (kb + j) * kKB, 0, 0, n_cta * (kRows / 32), t.expert, bar);
-                else
-                    tma_5d<CG>(dst + j * a.block_bytes, &tmW, (kb + j) * kKB, n_cta * kRows, t.expert, 0, 0, bar);
+            if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[i], CG * (WIDE ? sub : blocks) * (kABytes + a.tn * kKB));
+            if constexpr (WIDE) {
+                if constexpr (SWIGLU) tma_5d<CG>(dst, &tmW, 0, 0, 2 * t.expert, n_cta * (kRows / 32), kb, bar);
+                else tma_5d<CG>(dst, &tmW, 0, n_cta * kRows, t.expert, kb, 0, bar);
+            } else {
+                for (int j = 0; j < blocks; ++j) {
+                    if constexpr (SWIGLU)
+                        tma_5d<CG>(dst + j * kABytes, &tmW, (kb + j) * kKB, 0, 0, n_cta * (kRows / 32), t.expert, bar);
+                    else
+                        tma_5d<CG>(dst + j * kABytes, &tmW, (kb + j) * kKB, n_cta * kRows, t.expert, 0, 0, bar);
+                }
             }
         };
         int ahead = 0;   // stages whose weights are under way before the kernel in front has ended
@@ -352,8 +360,8 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             if (first < total) {
                 const Tile t = tile_of(a, cum, start, first, kStep);
                 const int n_cta = t.n * CG + (CG == 2 ? static_cast<int>(rank) : 0);
-                for (int kb = kb0; kb < kb1 && ahead < a.stages; kb += blocks_all, ++ahead)
-                    if (elect_one()) load_weights(ahead, kb, t, n_cta, CG == 2 ? 1 : min(sub, kb1 - kb));
+                for (int kb = kb0; kb < kb1 && ahead < a.stages; kb += sub, ++ahead)
+                    if (elect_one()) load_weights(ahead, kb, t, n_cta, min(sub, kb1 - kb));
                 __syncwarp();
             }
             pdl_wait_prior();
@@ -367,11 +375,15 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], (lap - 1) & 1, a.status, kDevWaitEmpty, 2000u, a.limit));
                 if (!ok) break;
                 if (elect_one()) {
-                    const int blocks = CG == 2 ? 1 : min(sub, kb1 - kb);
+                    const int blocks = min(sub, kb1 - kb);
                     if (lap > 0 || s >= ahead) load_weights(s, kb, t, n_cta, blocks);
-                    uint8_t* dst = smem + s * stage_bytes + kABytes;
-                    const uint32_t bar = CG == 2 ? map_to_rank(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
-                    for (int j = 0; j < blocks; ++j) tma_2d<CG>(dst + j * a.block_bytes, &tmX, (kb + j) * kKB, x_row, bar);
+                    uint8_t* dst = smem + s * stage_bytes + sub * kABytes;
+                    const uint32_t bar = full_at + 8 * s;
+                    if constexpr (WIDE) {
+                        tma_3d<CG>(dst, &tmX, 0, x_row, kb, bar);
+                    } else {
+                        for (int j = 0; j < blocks; ++j) tma_3d<CG>(dst + j * a.tn * kKB, &tmX, (kb + j) * kKB, x_row, 0, bar);
+                    }
                 }
                 __syncwarp();
                 if (++s == a.stages) {
@@ -408,11 +420,12 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[s], lap & 1, a.status, kDevWaitFull, 2000u, a.limit));
                     if (!ok) break;
                     tc_fence_after();
-                    const int blocks = CG == 2 ? 1 : min(sub, kb1 - kb);
+                    const int blocks = min(sub, kb1 - kb);
                     if (elect_one()) {
                         for (int j = 0; j < blocks; ++j) {
-                            const uint32_t at = smem_u32(smem + s * stage_bytes + j * a.block_bytes);
-                            const uint64_t adesc = smem_desc_sw128(at), bdesc = smem_desc_sw128(at + kABytes);
+                            const uint32_t at = smem_u32(smem + s * stage_bytes);
+                            const uint64_t adesc = smem_desc_sw128(at + j * kABytes);
+                            const uint64_t bdesc = smem_desc_sw128(at + sub * kABytes + j * a.tn * kKB);
 #pragma unroll
                             for (int k = 0; k < kKB / 32; ++k)
                                 mma_i8<CG>(d, adesc + 2 * k, bdesc + 2 * k, idesc, (kb + j > kb0 || k != 0) ? 1u : 0u);
@@ -623,34 +636,55 @@ int encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims,
     return LSG_OK;
 }
 
-// The weight [E, N, K] (or [E, 2 N, K], gate rows in front of up rows): boxes of 128 rows.
-int weight_map(CUtensorMap* map, const Int8Gemm& g, bool swiglu) {
-    const cuuint64_t ld = static_cast<cuuint64_t>(g.ldb);
+// The weight [E, N, K] (or [E, 2 N, K], gate rows in front of up rows): boxes of 128 rows by 128 bytes, or by
+// `blocks` times 128 bytes, block after block (0: K is not a multiple of 128, and reads as zeros behind it).
+int weight_map(CUtensorMap* map, const Int8Gemm& g, bool swiglu, int blocks) {
+    const cuuint64_t ld = static_cast<cuuint64_t>(g.ldb), n = static_cast<cuuint64_t>(g.N), e = static_cast<cuuint64_t>(g.E);
+    const cuuint64_t k = static_cast<cuuint64_t>(g.K), kb = k / kKB;
+    if (swiglu && blocks) {
+        const cuuint64_t dims[5] = {kKB, 16, 2 * e, n / 16, kb};
+        const cuuint64_t strides[4] = {ld, ld * n, ld * 16, kKB};
+        const cuuint32_t box[5] = {kKB, 16, 2, 4, static_cast<cuuint32_t>(blocks)};
+        return encode(map, 5, g.B, dims, strides, box);
+    }
     if (swiglu) {
-        const cuuint64_t n = static_cast<cuuint64_t>(g.N);
-        const cuuint64_t dims[5] = {static_cast<cuuint64_t>(g.K), 16, 2, n / 16, static_cast<cuuint64_t>(g.E)};
+        const cuuint64_t dims[5] = {k, 16, 2, n / 16, e};
         const cuuint64_t strides[4] = {ld, ld * n, ld * 16, ld * n * 2};
         const cuuint32_t box[5] = {kKB, 16, 2, 4, 1};
         return encode(map, 5, g.B, dims, strides, box);
     }
-    const cuuint64_t dims[5] = {static_cast<cuuint64_t>(g.K), static_cast<cuuint64_t>(g.N), static_cast<cuuint64_t>(g.E), 1, 1};
-    const cuuint64_t all = ld * static_cast<cuuint64_t>(g.N);
-    const cuuint64_t strides[4] = {ld, all, all, all};
+    if (blocks) {
+        const cuuint64_t dims[5] = {kKB, n, e, kb, 1};
+        const cuuint64_t strides[4] = {ld, ld * n, kKB, ld * n};
+        const cuuint32_t box[5] = {kKB, kRows, 1, static_cast<cuuint32_t>(blocks), 1};
+        return encode(map, 5, g.B, dims, strides, box);
+    }
+    const cuuint64_t dims[5] = {k, n, e, 1, 1};
+    const cuuint64_t strides[4] = {ld, ld * n, ld * n, ld * n};
     const cuuint32_t box[5] = {kKB, kRows, 1, 1, 1};
     return encode(map, 5, g.B, dims, strides, box);
 }
 
-template <int CG, bool SWIGLU, int SPLIT>
+// The tokens [M, K]: boxes of `rows` by 128 bytes, or as above.
+int token_map(CUtensorMap* map, const Int8Gemm& g, int rows, int blocks) {
+    const cuuint64_t ld = static_cast<cuuint64_t>(g.lda), m = static_cast<cuuint64_t>(g.M), k = static_cast<cuuint64_t>(g.K);
+    const cuuint64_t dims[3] = {blocks ? kKB : k, m, blocks ? k / kKB : 1};
+    const cuuint64_t strides[2] = {ld, blocks ? kKB : ld * m};
+    const cuuint32_t box[3] = {kKB, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(blocks ? blocks : 1)};
+    return encode(map, 3, g.A, dims, strides, box);
+}
+
+template <int CG, bool SWIGLU, int SPLIT, bool WIDE>
 int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const MmaArgs& a, int grid, int cluster, cudaStream_t s) {
     static std::atomic<bool> configured[64];
     int dev = 0;
     LSG_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_relaxed)) {
-        LSG_CUDA_TRY(cudaFuncSetAttribute(int8_mma_kernel<CG, SWIGLU, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        LSG_CUDA_TRY(cudaFuncSetAttribute(int8_mma_kernel<CG, SWIGLU, SPLIT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_relaxed);
     }
     const size_t smem = static_cast<size_t>(a.stages) * a.sub * a.block_bytes + 1024 + kTailBytes;
-    LSG_CUDA_TRY(launch_clusters(int8_mma_kernel<CG, SWIGLU, SPLIT>, cluster, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, s,
+    LSG_CUDA_TRY(launch_clusters(int8_mma_kernel<CG, SWIGLU, SPLIT, WIDE>, cluster, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem, s,
                                  true, tmW, tmX, a));
     return LSG_OK;
 }
@@ -664,6 +698,8 @@ int round_up(int v, int step) { return (v + step - 1) / step * step; }
 // so everything launched before it has ended: offsets are read and weights loaded while it still runs.
 int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
     if (g.M > 0x7fffffff - 512 || g.N > 0x7fffffff - 512) return fail(LSG_ERR_UNSUPPORTED, "int8 product: too many rows");
+    // K a multiple of 128: one copy loads all K blocks of a stage (experts of 4096 tokens 1319 -> 1295 us)
+    const bool wide = g.K % kKB == 0;
     MmaArgs a = {};
     a.D = g.D; a.out_dtype = g.out_dtype; a.sA = g.scale_A; a.sB = g.scale_B; a.offsets = g.expert_offsets;
     a.M = g.M; a.N = g.N; a.E = g.E; a.kblocks = (g.K + kKB - 1) / kKB;
@@ -707,7 +743,7 @@ int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
     // Up to 128 tokens: two to four K blocks a stage, so that what is asked of a weight row at a time is 256
     // to 512 bytes (256 tokens, 8 experts of 4096 / 14336: 278 us with stages of 56 KB, 261 with 74 KB, 272
     // with 110 KB; 128 x 14336 x 4096 20.6 with one block, then 18.3, 16.2, 18.2).
-    a.sub = pair ? 1 : std::min(4, std::max(1, 74 * 1024 / a.block_bytes));
+    a.sub = pair ? (wide ? kPairBlocks<true> : kPairBlocks<false>) : std::min(4, std::max(1, 74 * 1024 / a.block_bytes));
     a.stages = kSmemMax / (a.sub * a.block_bytes) < kMaxStages ? kSmemMax / (a.sub * a.block_bytes) : kMaxStages;
     int cols = 64;
     while (cols < 2 * tile) cols *= 2;
@@ -716,23 +752,25 @@ int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
     if (tiles > 0x7fffffffll) return fail(LSG_ERR_UNSUPPORTED, "int8 product: too many tiles");
 
     CUtensorMap tmW, tmX;
-    int rc = weight_map(&tmW, g, swiglu);
+    int rc = weight_map(&tmW, g, swiglu, wide ? a.sub : 0);
     if (rc != LSG_OK) return rc;
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(g.K), static_cast<cuuint64_t>(g.M)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(g.lda)};
-    const cuuint32_t box[2] = {kKB, static_cast<cuuint32_t>(a.tn)};
-    rc = encode(&tmX, 2, g.A, dims, strides, box);
+    rc = token_map(&tmX, g, a.tn, wide ? a.sub : 0);
     if (rc != LSG_OK) return rc;
 
-    if (pair) {
-        const int grid = 2 * static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
-        return swiglu ? launch<2, true, 1>(tmW, tmX, a, grid, 2, s) : launch<2, false, 1>(tmW, tmX, a, grid, 2, s);
-    }
-    if (split == 8) return launch<1, false, 8>(tmW, tmX, a, static_cast<int>(tiles) * 8, 8, s);
-    if (split == 4) return launch<1, false, 4>(tmW, tmX, a, static_cast<int>(tiles) * 4, 4, s);
-    if (split == 2) return launch<1, false, 2>(tmW, tmX, a, static_cast<int>(tiles) * 2, 2, s);
-    const int grid = static_cast<int>(tiles < sms ? tiles : sms);
-    return swiglu ? launch<1, true, 1>(tmW, tmX, a, grid, 1, s) : launch<1, false, 1>(tmW, tmX, a, grid, 1, s);
+    const int count = static_cast<int>(tiles);
+    const auto go = [&](auto w) {
+        constexpr bool W = decltype(w)::value;
+        if (pair) {
+            const int grid = 2 * std::min(count, sms / 2);
+            return swiglu ? launch<2, true, 1, W>(tmW, tmX, a, grid, 2, s) : launch<2, false, 1, W>(tmW, tmX, a, grid, 2, s);
+        }
+        if (split == 8) return launch<1, false, 8, W>(tmW, tmX, a, count * 8, 8, s);
+        if (split == 4) return launch<1, false, 4, W>(tmW, tmX, a, count * 4, 4, s);
+        if (split == 2) return launch<1, false, 2, W>(tmW, tmX, a, count * 2, 2, s);
+        const int grid = std::min(count, sms);
+        return swiglu ? launch<1, true, 1, W>(tmW, tmX, a, grid, 1, s) : launch<1, false, 1, W>(tmW, tmX, a, grid, 1, s);
+    };
+    return wide ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace lsg
