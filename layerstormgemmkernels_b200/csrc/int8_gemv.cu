@@ -5,7 +5,8 @@
 // per SM from the first microsecond on), and forms the exact int32 sums with dp4a against the activation
 // codes in shared memory.  Activations that come as bf16 or fp16 are quantized by every CTA for itself
 // while its first weights arrive (the arithmetic of the row quantizer, the same codes and scales): one
-// launch instead of two.
+// launch instead of two.  1 x 4096 x 4096 takes 5.0 us (two launches 6.7), 14336 x 4096 12.4 (4.8 TB/s with
+// launch and tail), 16384 x 16384 45 (5.9 TB/s).  Loads into registers instead of the ring: 14.2 for the second.
 #include "common.cuh"
 #include "host.h"
 #include "int8.cuh"

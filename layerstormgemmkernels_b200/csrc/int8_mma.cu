@@ -8,7 +8,7 @@
 //
 //   first warps epilogue: warp w owns tensor-memory lanes 32 (w % 4).. and the pieces of 16 columns
 //               (tokens) w / 4, w / 4 + groups, ..
-//   next warp   TMA producer: 128 weight rows and the tile's tokens, 128 or 256 bytes of K a stage
+//   next warp   TMA producer: 128 weight rows and the tile's tokens, one to four K blocks of 128 bytes a stage
 //   last warp   MMA issuer: 4 instructions (K = 32 each) for 128 bytes of K
 //
 // Three forms of the same kernel:
@@ -21,6 +21,14 @@
 // five-dimensional box of the stacked weight puts them there), a shuffle brings g and u together and
 // silu(g) * u is stored in fp32: the quantizer that follows reads 4 bytes instead of 8.
 // Persistent except for split; every wait is time-limited.
+//
+// What bounds it.  Large products: the tensor pipe, busy nine tenths of the time (4096 x 14336 x 4096 in 153 us
+// as a burst, 3.1 Pop/s; 180 us when the power limit has taken the clock to 1.5 GHz), with operands coming
+// out of L2 at 12 TB/s: single CTAs, which load half as much again, take 36 us for 2048 x 4096 x 4096 where
+// pairs take 31.  The two wide dimensions are 256 because tensor memory holds two accumulators of 256
+// columns.  Few tokens: the weight bytes (64 tokens through 128 experts 5.2 to 5.7 TB/s).
+// A few dense tiles: 2 us for adding the partial sums, which splitting saves several times over (77 x 4096 x
+// 14336: 16.6 us with four CTAs a tile, 31 with one).
 #include "common.cuh"
 #include "host.h"
 #include "int8.cuh"
@@ -728,7 +736,7 @@ int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
     int split = 1;
     if (!pair && !swiglu && !g.expert_offsets) {
         static const int ways[3] = {8, 4, 2};
-        static const int slots[3] = {15, 33, 74};               // clusters of that size that are resident
+        static const int slots[3] = {15, 33, 74};               // clusters of that size that are resident on a B200
         for (int i = 0; i < 3; ++i)
             if (units * cta_tiles <= slots[i] && a.kblocks >= 2 * ways[i]) {
                 split = ways[i];
