@@ -14,7 +14,6 @@
 #include "common.cuh"
 #include "host.h"
 
-#include <algorithm>
 #include <type_traits>
 
 namespace lsg {
@@ -249,9 +248,9 @@ moe_unpermute_backward_kernel(const Piece<T, P>* __restrict__ grad_out, const Pi
     }
 }
 
-// One warp per token.  The chosen experts' gradients are formed by lanes 0..k-1; every lane then
-// writes the experts lane, lane + 32, ..., summing the slots that name the expert (routing names an
-// expert once; a caller's own indices may name it twice).
+// One warp per token.  Lanes 0..k-1 form the chosen experts' gradients, each with the other slots that name
+// its expert added in order (routing names an expert once; a caller's own indices may name it twice); the
+// row is cleared by whole warps and the k values go over it.
 __global__ void __launch_bounds__(256)
 moe_route_backward_kernel(const int32_t* __restrict__ idx, const float* __restrict__ w, const float* __restrict__ grad_w,
                           int T, int E, int k, float* __restrict__ grad_logits) {
@@ -263,28 +262,38 @@ moe_route_backward_kernel(const int32_t* __restrict__ idx, const float* __restri
     const float wl = lane < k ? w[t * k + lane] : 0.0f;
     const float gl = lane < k ? grad_w[t * k + lane] : 0.0f;
     const int el = lane < k ? idx[t * k + lane] : -1;
+    float* row = grad_logits + t * E;
+    if ((reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+        for (int e = lane; e < E / 4; e += 32) reinterpret_cast<float4*>(row)[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (lane < (E & 3)) row[(E & ~3) + lane] = 0.0f;
+    } else {
+        for (int e = lane; e < E; e += 32) row[e] = 0.0f;
+    }
     float dot = wl * gl;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
     const float d = wl * (gl - dot);
-    for (int e = lane; e < ((E + 31) & ~31); e += 32) {
-        float v = 0.0f;
-        for (int s = 0; s < k; ++s) {
-            const int es = __shfl_sync(0xffffffffu, el, s);
-            const float ds = __shfl_sync(0xffffffffu, d, s);
-            if (es == e) v += ds;
-        }
-        if (e < E) grad_logits[t * E + e] = v;
+    float sum = 0.0f;
+    for (int s = 0; s < k; ++s) {
+        const int es = __shfl_sync(0xffffffffu, el, s);
+        const float ds = __shfl_sync(0xffffffffu, d, s);
+        if (es == el) sum += ds;
     }
+    __syncwarp();   // the zeros are written before the values
+    if (el >= 0 && el < E) row[el] = sum;
 }
 
-int threads_for(int per_row) { return per_row >= 256 ? 256 : (per_row < 1 ? 32 : (per_row + 31) / 32 * 32); }
+// Threads of a token's CTA, at most `most`: the row's pieces in as few rounds, evenly.
+int threads_for(int per_row, int most = 256) {
+    const int rounds = (per_row + most - 1) / most;
+    return rounds < 1 ? 32 : ((per_row + rounds - 1) / rounds + 31) / 32 * 32;
+}
 
 bool whole_pieces(int H, size_t size, uintptr_t at) { return (static_cast<size_t>(H) * size) % 16 == 0 && (at & 15) == 0; }
 
 template <typename T, int P, int K>
 int launch_sum(const void* y, const int32_t* inv, const float* w, int rows, int tokens, int k, int per_row, void* out, cudaStream_t s) {
-    LSG_CUDA_TRY(launch_kernel(moe_sum_slots_kernel<T, P, K>, dim3(static_cast<unsigned>(tokens)), dim3(threads_for(per_row)), 0, s,
+    LSG_CUDA_TRY(launch_kernel(moe_sum_slots_kernel<T, P, K>, dim3(static_cast<unsigned>(tokens)), dim3(threads_for(per_row, tokens >= 2048 ? 128 : 256)), 0, s,
                                true, static_cast<const Piece<T, P>*>(y), inv, w, rows, k, per_row, static_cast<Piece<T, P>*>(out)));
     return LSG_OK;
 }
@@ -292,7 +301,7 @@ template <typename T, int P, int K>
 int launch_unpermute_backward(const void* grad_out, const void* y, const int32_t* inv, const float* w, const int32_t* used, int rows,
                               int tokens, int k, int per_row, void* grad_y, float* grad_w, cudaStream_t s) {
     LSG_CUDA_TRY(launch_kernel(moe_unpermute_backward_kernel<T, P, K>, dim3(static_cast<unsigned>(tokens)),
-                               dim3(std::min(tokens >= 2048 ? 64 : 256, threads_for(per_row))), 0, s, true, static_cast<const Piece<T, P>*>(grad_out),
+                               dim3(threads_for(per_row, tokens >= 2048 ? 64 : 256)), 0, s, true, static_cast<const Piece<T, P>*>(grad_out),
                                static_cast<const Piece<T, P>*>(y), inv, w, used, rows, k, per_row,
                                static_cast<Piece<T, P>*>(grad_y), grad_w));
     return LSG_OK;
