@@ -699,6 +699,57 @@ int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const MmaArgs& a, int
 
 int round_up(int v, int step) { return (v + step - 1) / step * step; }
 
+struct Plan {
+    int tile;       // tokens of a tile
+    bool pair;
+    int split;
+};
+
+// One product: the tile, the form and the cut of K of the least estimated time, in SM cycles.  A K block of a
+// tile takes what the tensor pipe needs (2 cycles a token, nine tenths of the time) or what its operands need to
+// arrive, whichever is longer: 68 bytes a cycle out of L2 in single CTAs, 58 in pairs, weight rows that only this
+// tile of tokens reads 48, as they come from memory.  All weights take the memory's 3300 bytes a cycle once.
+// Behind the last K block come the epilogue (13 cycles a token) and, where K is cut, adding the partial sums
+// (2200 and 37 a token); what does not fit the stages at once waits for memory once more (1000).
+// Against one rule per row count (even tiles of up to 256 tokens, cut when fewer than half the SMs have one):
+// 1001 x 1024 x 4096 12.9 -> 9.7 us, 512 x 4096 x 4096 15.2 -> 11.5, 600 x 2000 x 1024 9.0 -> 5.5, 1500 x 4096 x
+// 4096 25.6 -> 22.3.
+Plan plan_dense(int M, int N, int kblocks, int sms) {
+    const long long ctas = (N + kRows - 1) / kRows;
+    const long long bytes = static_cast<long long>(N) * kblocks * kKB;
+    static const int slots[4] = {0, 74, 33, 15};            // clusters of 2, 4, 8 CTAs that are resident on a B200
+    Plan best = {256, false, 1};
+    long long least = -1;
+    const auto consider = [&](int tile, bool pair, int split, long long units, long long active, long long rounds) {
+        const int from = units == 1 ? 48 : (pair ? 58 : (units == 2 ? 58 : 68));
+        const long long kbs = (kblocks + split - 1) / split;
+        const long long mma = tile * 2 * 10 / 9, load = kABytes / from + (pair ? tile * 64 / 58 : tile * 128 / 68);
+        const long long stream = bytes / std::min(3300ll, 48 * std::min(active, static_cast<long long>(sms)));
+        const long long laps = rounds * kbs * (kABytes + (pair ? tile * 64 : tile * 128)) / (216 * 1024);
+        const long long t = std::max(rounds * kbs * std::max(mma, load), stream) + tile * 13 +
+                            (split > 1 ? 2200 + tile * 37 : 0) + (laps > 0 ? 1000 : 0);
+        if (least < 0 || t < least) {
+            least = t;
+            best = {tile, pair, split};
+        }
+    };
+    int last = 0;
+    for (long long units = (static_cast<long long>(M) + 255) / 256, tries = 0; tries < 32; ++tries, ++units) {
+        const int tile = round_up(static_cast<int>((M + units - 1) / units), 16);
+        if (tile == last) continue;
+        last = tile;
+        const long long n = (M + tile - 1) / tile;
+        consider(tile, false, 1, n, n * ctas, (n * ctas + sms - 1) / sms);
+        for (int c = 1; c < 4; ++c)
+            if (n * ctas <= slots[c] && kblocks >= (2 << c)) consider(tile, false, 1 << c, n, n * ctas << c, 1);
+        const int even = round_up(tile, 32);
+        const long long m = (M + even - 1) / even, pairs = m * ((ctas + 1) / 2);
+        if (tile >= 32) consider(even, true, 1, m, 2 * pairs, (pairs + sms / 2 - 1) / (sms / 2));
+        if (tile <= 32) break;
+    }
+    return best;
+}
+
 }  // namespace
 
 // D = A B^T with both scales; swiglu: B is [E, 2 N, K] and D fp32 silu(gate) * up.  early: A comes from
@@ -717,33 +768,22 @@ int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
     const int sms = sm_count();
     const int per_cta = swiglu ? kRows / 2 : kRows;             // output columns of a CTA
     const int cta_tiles = (g.N + per_cta - 1) / per_cta;
-    // tokens of a tile: even shares of at most 256; by the average of the experts where rows are grouped
-    const long long share = g.expert_offsets ? (static_cast<long long>(g.M) + g.E - 1) / g.E : g.M;
-    int tile;
+    Plan plan;
     if (g.expert_offsets) {
-        // 1.4 times the average, so that most experts are one tile: 1024 tokens, 128 experts of 2048 / 768,
-        // top 8 (64 rows each): 148.7 us with 96, 154 with 128; 2048 tokens 188 with 160, 194 with 256
-        const long long most = share + share * 2 / 5;
-        tile = most >= 256 ? 256 : (most > 64 ? round_up(static_cast<int>(most), 32) : round_up(static_cast<int>(most), 16));
+        // 1.4 times the average rows of an expert, so that most experts are one tile: 1024 tokens, 128 experts of
+        // 2048 / 768, top 8 (64 rows each): 148.7 us with 96, 154 with 128; 2048 tokens 188 with 160, 194 with 256.
+        // Pairs from 96 tokens on (256 tokens, 8 experts of 4096 / 14336: 266.7 us with pairs, 274 without).
+        const long long share = (static_cast<long long>(g.M) + g.E - 1) / g.E, most = share + share * 2 / 5;
+        plan.tile = most >= 256 ? 256 : (most > 64 ? round_up(static_cast<int>(most), 32) : round_up(static_cast<int>(most), 16));
+        plan.split = 1;
+        plan.pair = plan.tile > 64 && (g.M / plan.tile + static_cast<long long>(std::min(g.E, g.M))) * cta_tiles >= sms / 2;
     } else {
-        const int units = (g.M + 255) / 256;
-        tile = round_up((g.M + units - 1) / units, 16);
+        plan = plan_dense(g.M, g.N, a.kblocks, sms);
     }
-    const long long units = g.expert_offsets ? g.M / tile + static_cast<long long>(g.E < g.M ? g.E : g.M) : (g.M + tile - 1) / tile;
-    // Pairs halve what a CTA loads of the tokens.  Experts take them from 96 tokens on (256 tokens, 8 experts of
-    // 4096 / 14336: 266.7 us with pairs, 274 without), one product above 128.
-    const bool pair = tile > (g.expert_offsets ? 64 : 128) && units * cta_tiles >= sms / 2;
-    int split = 1;
-    if (!pair && !swiglu && !g.expert_offsets) {
-        static const int ways[3] = {8, 4, 2};
-        static const int slots[3] = {15, 33, 74};               // clusters of that size that are resident on a B200
-        for (int i = 0; i < 3; ++i)
-            if (units * cta_tiles <= slots[i] && a.kblocks >= 2 * ways[i]) {
-                split = ways[i];
-                break;
-            }
-    }
-    if (pair) tile = round_up(tile, 32);
+    const int tile = plan.tile, split = plan.split;
+    const bool pair = plan.pair;
+    const long long units = g.expert_offsets ? g.M / tile + static_cast<long long>(std::min(g.E, g.M))
+                                             : (static_cast<long long>(g.M) + tile - 1) / tile;
     a.tile = tile;
     a.tn = pair ? tile / 2 : tile;
     a.n_tiles = pair ? (cta_tiles + 1) / 2 : cta_tiles;

@@ -180,6 +180,24 @@ def test_gemm(ops, M, N, K, kind):
     check_product(D, acc, sa, sb, kind)
 
 
+# Sizes whose estimates choose tiles of 16 to 256 tokens, in single CTAs, in pairs and with K cut among two,
+# four and eight CTAs; the rows and channels end inside a tile.
+FORMS = [(15, 14337, 272), (16, 6000, 2048), (18, 13, 2050), (19, 2001, 2064), (17, 6003, 4096), (20, 130, 30), (31, 14336, 48),
+         (45, 1008, 4100), (33, 4099, 4096), (47, 14333, 528), (49, 14336, 1040), (63, 14335, 2048), (79, 14336, 520),
+         (81, 14339, 528), (95, 14336, 1040), (99, 2005, 4096), (97, 14336, 530), (113, 14337, 1056), (130, 2000, 4090),
+         (129, 14336, 528), (161, 2003, 4096), (190, 14331, 528), (223, 14336, 544), (250, 14336, 513), (1780, 130, 4096),
+         (3001, 129, 2048), (2100, 600, 144)]
+
+
+@pytest.mark.parametrize("M,N,K", FORMS)
+def test_gemm_forms_of_tiles(ops, M, N, K):
+    g = torch.Generator().manual_seed(M + N + K)
+    A, B = rand_codes(g, M, K), rand_codes(g, N, K)
+    sa, sb = (torch.rand(M, generator=g) + 0.1).cuda(), (torch.rand(N, generator=g) + 0.1).cuda()
+    D = ops.int8_gemm(A, B, sa, sb, M, N, K, "fp32")
+    check_product(D, A.double() @ B.double().t(), sa, sb, "fp32")
+
+
 @pytest.mark.parametrize("M", [1, 4, 16, 40, 300])
 def test_gemm_extreme_codes_and_longest_k(ops, M):
     """-128 in every place at the longest K: sums of 128 * 128 * 131056 = 2^31 - 2^18."""
