@@ -184,18 +184,24 @@ extern "C" int lsg_int8_moe_ffn(const lsg_int8_moe_ffn_params* p, void* workspac
     float* h = reinterpret_cast<float*>(ws + f.h);
     int8_t* act = reinterpret_cast<int8_t*>(ws + f.act);
     float* act_scales = reinterpret_cast<float*>(ws + f.act_scales);
-    rc = int8_quant_rows(p->hidden, p->ld_hidden, p->input_dtype, codes, f.ldh, scales, p->num_tokens, H, p->inv_perm, p->top_k, rows, s);
-    if (rc != LSG_OK) return rc;
     Int8Gemm a = {};
     a.A = codes; a.lda = f.ldh; a.B = static_cast<const int8_t*>(p->gate_up); a.ldb = H;
     a.D = h; a.out_dtype = LSG_DTYPE_F32; a.scale_A = scales; a.scale_B = p->gate_up_scales;
     a.M = rows; a.N = I; a.K = H; a.E = p->num_experts; a.expert_offsets = p->expert_offsets;
+    Int8Gemm b = a;
+    b.A = act; b.lda = f.ldi; b.B = static_cast<const int8_t*>(p->down); b.ldb = I;
+    b.D = p->D; b.out_dtype = p->output_dtype; b.scale_A = act_scales; b.scale_B = p->down_scales;
+    b.N = H; b.K = I;
+    if (int8_moe_gemv_takes(p->num_tokens, rows, H, I)) {
+        a.A = static_cast<const int8_t*>(p->hidden); a.lda = p->ld_hidden;
+        b.A = reinterpret_cast<const int8_t*>(h); b.lda = I;
+        return int8_moe_gemv(a, p->input_dtype, p->inv_perm, p->top_k, b, s);
+    }
+    rc = int8_quant_rows(p->hidden, p->ld_hidden, p->input_dtype, codes, f.ldh, scales, p->num_tokens, H, p->inv_perm, p->top_k, rows, s);
+    if (rc != LSG_OK) return rc;
     rc = int8_mma(a, true, true, s);
     if (rc != LSG_OK) return rc;
     rc = int8_quant_rows(h, I, LSG_DTYPE_F32, act, f.ldi, act_scales, rows, I, nullptr, 1, 0, s);
     if (rc != LSG_OK) return rc;
-    a.A = act; a.lda = f.ldi; a.B = static_cast<const int8_t*>(p->down); a.ldb = I;
-    a.D = p->D; a.out_dtype = p->output_dtype; a.scale_A = act_scales; a.scale_B = p->down_scales;
-    a.N = H; a.K = I;
-    return int8_gemm(a, true, s);
+    return int8_gemm(b, true, s);
 }

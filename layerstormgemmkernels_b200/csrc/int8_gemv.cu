@@ -1,4 +1,4 @@
-// The 8-bit integer product for up to four token rows: a streaming mat-vec.
+// The 8-bit integer product for one or two token rows: a streaming mat-vec.
 //
 // Bound by the weight bytes, N * K once.  One CTA of 16 warps per SM; every warp streams its own weight
 // rows, in pieces of up to 4 KB by bulk copies into a private ring of up to three slots (192 KB under way

@@ -1,0 +1,309 @@
+// The 8-bit expert block for up to eight rows (one token with its experts, or a few): two streaming mat-vecs.
+//
+//   h[r] = silu(g) * u,  (g, u) = codes(hidden[token of r]) . gate_up[expert of r]      fp32
+//   D[r] = codes(h[r]) . down[expert of r]
+//
+// Bound by the weight bytes of the rows' experts, read once per row.  Jobs of two weight rows (a gate and its up
+// row, or two channels of down) go round the SMs; a warp streams those of its jobs by bulk copies of 1 KB into a
+// ring of 6 KB of its own and forms exact int32 sums with dp4a, so the bits are those of the tensor-core route.
+// Every CTA quantizes the activations for itself while its first weights arrive: two launches instead of four.
+// A CTA holds under half of an SM's shared memory and registers, so those of the second product start under the
+// first one and have up to 14 MB of their weights in shared memory when h is there.
+// One token, with routing and combining, 2 experts of 2048 / 2048: 11.3 us (four launches 17.4), 8 of 1024 / 512: 10.6
+// (14.5), 8 of 2048 / 768: 18.0 (19.5); 4 tokens, 2 experts of 1024 / 1024 each: 12.8 (15.0).  Tried: copies of
+// 512 bytes (18.6 for the third), one weight row a job (20), the jobs of a CTA side by side, which needs the codes
+// of fewer rows (19.0; 2 experts of 4096 / 8192 52 instead of 44), more than 48 registers (19.4; 54).
+#include "common.cuh"
+#include "host.h"
+#include "int8.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace lsg {
+
+namespace {
+
+constexpr int kRows = 8;                   // rows (pairs of a token and an expert) at most
+constexpr int kWarps = 16;
+constexpr int kThreads = kWarps * 32;
+constexpr int kBlock = 2;                  // weight rows of a job: a gate and an up row, or two channels
+constexpr int kPiece = 1024;               // bytes of a weight row in a slot at most
+constexpr int kSlots = 3;
+constexpr int kSlotBytes = kBlock * kPiece;
+constexpr int kRing = kSlots * kSlotBytes; // of a warp
+constexpr int kCodes = 16384;              // bytes of codes at most (two CTAs on an SM)
+
+struct Args {
+    Int8Gemm g;              // A: hidden [tokens, K] or h [M, K]; N: output channels; B: [E, N or 2 N, K]
+    const int32_t* inv;      // row of a pair (first product)
+    int top_k, tokens;       // rows of A
+    unsigned int* status;
+    long long limit;
+};
+
+// One row of activations and this thread's place in it: the warps are shared out evenly among the rows.
+template <typename T>
+struct RowPart {
+    static constexpr int kVecs = Int8In<T>::kVecs;
+    const T* row;
+    int m, share, t, step;
+    bool have, whole;
+
+    __device__ __forceinline__ RowPart(const Int8Gemm& g, int rows) {
+        share = kWarps;
+        while (share > 1 && share * rows > kWarps) share >>= 1;
+        const int warp = threadIdx.x >> 5;
+        m = warp / share;
+        t = (warp % share) * 32 + (threadIdx.x & 31);
+        step = share * 32;
+        have = m < rows;
+        row = reinterpret_cast<const T*>(g.A) + (have ? m : 0) * g.lda;
+        whole = ((reinterpret_cast<uintptr_t>(g.A) | static_cast<uintptr_t>(g.lda * sizeof(T))) & 15) == 0;
+    }
+    __device__ __forceinline__ void load(int v, uint4 (&raw)[kVecs]) const {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) raw[i] = reinterpret_cast<const uint4*>(row)[v * kVecs + i];
+    }
+    // this thread's part of the row's largest magnitude (as bits)
+    __device__ __forceinline__ uint32_t top(int K) const {
+        uint32_t most = 0;
+        if (have && whole) {
+#pragma unroll 2
+            for (int v = t; v < K / 8; v += step) {
+                uint4 raw[kVecs];
+                load(v, raw);
+                most = Int8In<T>::top(most, raw);
+            }
+            most = Int8In<T>::top_bits(most);
+        } else if (have) {
+            for (int k = t; k < K; k += step) most = max(most, __float_as_uint(fabsf(Int8In<T>::get(row, k))));
+        }
+        return most;
+    }
+    __device__ __forceinline__ void codes(int K, const RowScale& r, int8_t* q) const {
+        if (have && whole) {
+#pragma unroll 2
+            for (int v = t; v < K / 8; v += step) {
+                uint4 raw[kVecs];
+                load(v, raw);
+                float f[8];
+                Int8In<T>::unpack(raw, f);
+                reinterpret_cast<uint2*>(q)[v] = code8<T>(f, r);
+            }
+        } else if (have) {
+            for (int k = t; k < K; k += step) q[k] = static_cast<int8_t>(code1<T>(Int8In<T>::get(row, k), r));
+        }
+    }
+};
+
+// X: bf16 or fp16, the first product (hidden rows, silu(g) * u in fp32); float, the second one (rows of h).
+// K is a multiple of 16.
+template <typename X>
+__global__ void __launch_bounds__(kThreads, 2) int8_moe_gemv_kernel(const Args a) {
+    constexpr bool kFirst = sizeof(X) == 2;
+    constexpr int kOuts = kFirst ? kBlock / 2 : kBlock;   // output channels of a job
+    extern __shared__ __align__(128) uint8_t smem[];   // [kWarps][kSlots][kBlock][kPiece], then codes [tokens][K]
+    __shared__ uint64_t full[kWarps][kSlots];
+    __shared__ float scale[kRows];
+    __shared__ uint32_t part[kWarps];
+    __shared__ int expert_of[kRows], source_of[kRows];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int M = a.g.M, N = a.g.N, K = a.g.K;
+    uint8_t* ring = smem + warp * kRing;
+    int8_t* codes = reinterpret_cast<int8_t*>(smem + kWarps * kRing);
+
+    if (lane == 0) {
+        for (int s = 0; s < kSlots; ++s) mbar_init(&full[warp][s], 1);
+        mbar_fence_init();
+    }
+    // The first product waits here, then lets the second one start: that one finds offsets and weights in
+    // place (all launches before the first product have ended) and waits for h alone.
+    const RowPart<X> mine_of(a.g, a.tokens);
+    if (kFirst) {
+        pdl_wait_prior();
+        pdl_launch_dependents();
+    }
+    // Warp r: the expert of row r.  Offsets are taken as a rising sequence: the first expert that ends behind r.
+    if (warp < M) {
+        const int below = __ldg(a.g.expert_offsets);
+        int pair = 0;
+        if constexpr (kFirst) pair = __ldg(a.inv + min(lane, M - 1));
+        int found = a.g.E;
+        for (int e0 = 0; e0 < a.g.E && found == a.g.E; e0 += 128) {
+            int end[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) end[i] = __ldg(a.g.expert_offsets + min(e0 + i * 32 + lane, a.g.E - 1) + 1);
+#pragma unroll
+            for (int i = 3; i >= 0; --i)
+                if (e0 + i * 32 + lane < a.g.E && end[i] > warp) found = e0 + i * 32 + lane;
+            found = __reduce_min_sync(0xffffffffu, found);
+        }
+        if constexpr (kFirst) {
+            const uint32_t hits = __ballot_sync(0xffffffffu, lane < M && pair == warp);
+            pair = hits ? __ffs(hits) - 1 : 0;
+        }
+        if (lane == 0) {
+            expert_of[warp] = found < a.g.E && below <= warp ? found : -1;
+            source_of[warp] = kFirst ? pair / a.top_k : warp;
+        }
+    }
+    if (kFirst) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, mine_of.top(K));
+        if (lane == 0) part[warp] = top;
+    }
+    __syncthreads();
+    // rows with an expert lie side by side
+    const uint32_t live = __ballot_sync(0xffffffffu, lane < M && expert_of[min(lane, M - 1)] >= 0);
+    const int row0 = live ? __ffs(live) - 1 : 0, across = N / kOuts, jobs = __popc(live) * across;
+    const int first = warp * gridDim.x + blockIdx.x, stride = kWarps * gridDim.x;   // round the SMs
+    const int mine = first < jobs ? (jobs - 1 - first) / stride + 1 : 0;
+    const int per_job = (K + kPiece - 1) / kPiece, pieces = mine * per_job;
+    const int rows_on = stride / across, on = stride - rows_on * across;      // a step from job to job
+
+    struct Place {
+        int row, block, c;
+    };
+    Place p = {row0 + first / across, first % across, 0};
+    auto next = [&](Place& at) {
+        if (++at.c < per_job) return;
+        at.c = 0;
+        at.row += rows_on;
+        at.block += on;
+        if (at.block >= across) {
+            at.block -= across;
+            ++at.row;
+        }
+    };
+    // lane i < kBlock: its weight row of a job, among those of all experts
+    auto weight_row = [&](const Place& at) {
+        const int base = at.block * kOuts;
+        if (kFirst) return static_cast<long long>(expert_of[at.row]) * 2 * N + (lane / kOuts) * N + base + lane % kOuts;
+        return static_cast<long long>(expert_of[at.row]) * N + base + lane;
+    };
+    auto copy = [&](const Place& at, int slot) {
+        const int bytes = min(kPiece, K - at.c * kPiece);
+        if (lane == 0) mbar_arrive_expect_tx(&full[warp][slot], bytes * kBlock);
+        __syncwarp();
+        if (lane < kBlock)
+            bulk_g2s(ring + slot * kSlotBytes + lane * kPiece, a.g.B + weight_row(at) * K + at.c * kPiece, bytes,
+                     &full[warp][slot]);
+    };
+    Place ahead = p;
+    for (int i = 0; i < min(kSlots, pieces); ++i) {
+        copy(ahead, i);
+        next(ahead);
+    }
+    float sb = pieces > 0 && lane < kBlock ? __ldg(a.g.scale_B + weight_row(p)) : 0.0f;
+    if (!kFirst) {
+        pdl_wait_prior();
+        pdl_launch_dependents();
+        const uint32_t top = __reduce_max_sync(0xffffffffu, mine_of.top(K));
+        if (lane == 0) part[warp] = top;
+        __syncthreads();
+    }
+    {
+        const int m = mine_of.m;
+        const uint32_t theirs = lane < mine_of.share ? part[min(m * mine_of.share + lane, kWarps - 1)] : 0u;
+        const RowScale r = row_scale(__reduce_max_sync(0xffffffffu, theirs));
+        if (mine_of.have && mine_of.t == 0) scale[m] = r.scale;
+        mine_of.codes(K, r, codes + m * K);
+    }
+    __syncthreads();
+
+    int acc[kBlock], slot = 0;
+    uint32_t lap = 0;
+#pragma unroll
+    for (int j = 0; j < kBlock; ++j) acc[j] = 0;
+    for (int i = 0; i < pieces; ++i) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][slot], lap & 1, a.status, kDevWaitFull, 2000u, a.limit))) {
+            // give up, but not before the copies behind this one have landed
+            for (int j = 1; j < kSlots && i + j < pieces; ++j) {
+                const int other = (slot + j) % kSlots;
+                mbar_wait_bounded(&full[warp][other], (lap + (slot + j >= kSlots ? 1 : 0)) & 1, a.status, kDevWaitFull);
+            }
+            return;
+        }
+        const int source = source_of[p.row];
+        const int bytes = min(kPiece, K - p.c * kPiece);
+        const int8_t* x = codes + source * K + p.c * kPiece;
+        const uint8_t* w = ring + slot * kSlotBytes;
+#pragma unroll
+        for (int part_k = 0; part_k < kPiece; part_k += 512) {
+            const int k = part_k + lane * 16;
+            if (k < bytes) {
+                const int4 xv = *reinterpret_cast<const int4*>(x + k);
+#pragma unroll
+                for (int j = 0; j < kBlock; ++j) {
+                    const int4 wv = *reinterpret_cast<const int4*>(w + j * kPiece + k);
+                    acc[j] = dp4a_ss(wv.x, xv.x, dp4a_ss(wv.y, xv.y, dp4a_ss(wv.z, xv.z, dp4a_ss(wv.w, xv.w, acc[j]))));
+                }
+            }
+        }
+        __syncwarp();
+        if (i + kSlots < pieces) {
+            copy(ahead, slot);
+            next(ahead);
+        }
+        if (++slot == kSlots) {
+            slot = 0;
+            ++lap;
+        }
+        const Place done = p;
+        next(p);
+        if (p.c == 0) {
+            // lane j: weight row j of the job
+            int sum = 0;
+#pragma unroll
+            for (int j = 0; j < kBlock; ++j) {
+                const int all = __reduce_add_sync(0xffffffffu, acc[j]);
+                if (lane == j) sum = all;
+                acc[j] = 0;
+            }
+            float v = __fmul_rn(__fmul_rn(static_cast<float>(sum), scale[source]), sb);
+            if (kFirst) v = silu_mul(v, __shfl_down_sync(0xffffffffu, v, kOuts));
+            if (lane < kOuts) store_out(a.g.D, a.g.out_dtype, static_cast<size_t>(done.row) * N + done.block * kOuts + lane, v);
+            if (i + 1 < pieces && lane < kBlock) sb = __ldg(a.g.scale_B + weight_row(p));
+        }
+    }
+}
+
+template <typename X>
+int launch(Args a, cudaStream_t s) {
+    static std::atomic<bool> configured[64];
+    int dev = 0;
+    LSG_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_relaxed)) {
+        LSG_CUDA_TRY(cudaFuncSetAttribute(int8_moe_gemv_kernel<X>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          kWarps * kRing + kCodes));
+        if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_relaxed);
+    }
+    const long long jobs = static_cast<long long>(a.g.M) * a.g.N / (sizeof(X) == 2 ? kBlock / 2 : kBlock);
+    const int ctas = static_cast<int>(std::min<long long>(sm_count(), jobs));
+    a.status = device_status_word();
+    a.limit = wait_limit_cycles();
+    const size_t smem = kWarps * kRing + static_cast<size_t>(a.tokens) * a.g.K;
+    LSG_CUDA_TRY(launch_kernel(int8_moe_gemv_kernel<X>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, s, true, a));
+    return LSG_OK;
+}
+
+}  // namespace
+
+bool int8_moe_gemv_takes(int tokens, int rows, int H, int I) {
+    return rows <= kRows && static_cast<long long>(tokens) * H <= kCodes && static_cast<long long>(rows) * I <= kCodes;
+}
+
+int int8_moe_gemv(const Int8Gemm& first, int x_dtype, const int32_t* inv, int top_k, const Int8Gemm& second, cudaStream_t s) {
+    Args a = {};
+    a.g = first;
+    a.inv = inv;
+    a.top_k = top_k;
+    a.tokens = first.M / top_k;
+    const int rc = x_dtype == LSG_DTYPE_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
+    if (rc != LSG_OK) return rc;
+    a.g = second;
+    a.tokens = second.M;
+    return launch<float>(a, s);
+}
+
+}  // namespace lsg

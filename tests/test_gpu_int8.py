@@ -363,6 +363,67 @@ def test_moe_ffn(ops, T, E, k, H, I, kind):
         assert not bool(out[3].any())
 
 
+def four_steps(ops, hidden, offs, inv, k, gate_up, gus, down, ds, kind, fill):
+    """int8_moe_ffn from its four public steps; rows without an expert hold `fill`."""
+    rows, I, H = hidden.size(0) * k, down.size(2), hidden.size(1)
+    codes, scales = ops.moe_permute_int8(hidden, inv, k)
+    gu = torch.zeros(rows, 2 * I, device="cuda")
+    ops.int8_grouped_gemm(codes, gate_up, gu, scales, gus, offs, 2 * I, H, "fp32")
+    act, act_scales = ops.silu_mul_int8_quant(gu[:, :I], gu[:, I:])
+    D = torch.full((rows, H), fill, device="cuda", dtype={"bf16": BF16, "fp16": FP16, "fp32": FP32}[kind])
+    return ops.int8_grouped_gemm(act, down, D, act_scales, ds, offs, H, I, kind)
+
+
+@pytest.mark.parametrize("kind,dtype", [("bf16", BF16), ("fp16", FP16), ("fp32", BF16)])
+@pytest.mark.parametrize("T,E,k,H,I", [(1, 1, 1, 16, 16), (1, 3, 1, 1040, 16), (1, 128, 8, 2048, 768), (1, 7, 3, 48, 5456),
+                                       (2, 5, 4, 528, 1040), (3, 4, 2, 1024, 2032), (4, 1024, 2, 272, 512), (8, 6, 1, 2048, 2048),
+                                       (1, 4, 2, 16384, 48), (7, 2, 1, 16, 1024), (2, 300, 4, 1008, 80), (8, 2, 1, 2064, 16),
+                                       (9, 4, 1, 64, 64), (1, 9, 8, 64, 2064)])
+def test_moe_ffn_few_rows(ops, T, E, k, H, I, kind, dtype):
+    """Up to eight rows, on both sides of the sizes that the streaming form takes: the bits of the four
+    steps, from hidden rows that start on any 2 bytes, with an infinite and a zero token among them, and
+    again (a fresh run changes nothing)."""
+    g = torch.Generator().manual_seed(T + E + H + I)
+    base = torch.randn(T + 2, H + 7, generator=g).to(dtype).cuda()
+    hidden = base[1:T + 1, 3:H + 3]
+    if T > 3:
+        hidden[1, H // 2] = math.inf
+        hidden[2] = 0
+    gate_up, gus, down, ds = experts(g, E, H, I)
+    idx = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)]).int().cuda()
+    for at in (hidden, hidden.contiguous()):
+        offs, perm, inv = ops.moe_permutation(idx, E)
+        rows = ops.int8_moe_ffn(at, offs, inv, k, gate_up, gus, down, ds, kind)
+        D = four_steps(ops, at, offs, inv, k, gate_up, gus, down, ds, kind, 0.0)
+        used = int(offs[-1])
+        assert used == T * k and torch.equal(rows.nan_to_num(7.0, 8.0, 9.0), D.nan_to_num(7.0, 8.0, 9.0))
+        assert bool(rows.isnan().any()) == (T > 3)
+        assert torch.equal(rows.nan_to_num(7.0), ops.int8_moe_ffn(at, offs, inv, k, gate_up, gus, down, ds, kind).nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("gone", [(), (0,), (1, 3), (0, 1, 2, 3)])
+def test_moe_ffn_few_rows_without_an_expert(ops, gone):
+    """Pairs that no expert here takes (padding, another rank's) leave the rows behind the last one out;
+    the combination skips them."""
+    g = torch.Generator().manual_seed(5)
+    T, E, k, H, I = 4, 6, 2, 256, 96
+    hidden = torch.randn(T, H, generator=g).to(BF16).cuda()
+    gate_up, gus, down, ds = experts(g, E, H, I)
+    idx, w = ops.moe_route(torch.randn(T, E, generator=g).cuda(), k)
+    whole_offs, _, whole_inv = ops.moe_permutation(idx, E)
+    whole = ops.moe_unpermute(ops.int8_moe_ffn(hidden, whole_offs, whole_inv, k, gate_up, gus, down, ds), whole_inv, w)
+    for t in gone:
+        idx[t] = E if t % 2 else -1
+    offs, perm, inv = ops.moe_permutation(idx, E)
+    rows = ops.int8_moe_ffn(hidden, offs, inv, k, gate_up, gus, down, ds)
+    out = ops.moe_unpermute(rows, inv, w)
+    for t in range(T):
+        if t in gone:
+            assert not bool(out[t].any())
+        else:
+            assert torch.equal(out[t], whole[t])
+
+
 def test_dense_and_grouped_agree(ops):
     """One expert with all rows is the dense product, bit for bit."""
     g = torch.Generator().manual_seed(11)
