@@ -7,12 +7,12 @@
 // row, or two channels of down) go round the SMs; a warp streams those of its jobs by bulk copies of 1 KB into a
 // ring of 6 KB of its own and forms exact int32 sums with dp4a, so the bits are those of the tensor-core route.
 // Every CTA quantizes the activations for itself while its first weights arrive: two launches instead of four.
-// A CTA holds under half of an SM's shared memory and registers, so those of the second product start under the
-// first one and have up to 14 MB of their weights in shared memory when h is there.
-// One token, with routing and combining, 2 experts of 2048 / 2048: 11.3 us (four launches 17.4), 8 of 1024 / 512: 10.6
-// (14.5), 8 of 2048 / 768: 18.0 (19.5); 4 tokens, 2 experts of 1024 / 1024 each: 12.8 (15.0).  Tried: copies of
-// 512 bytes (18.6 for the third), one weight row a job (20), the jobs of a CTA side by side, which needs the codes
-// of fewer rows (19.0; 2 experts of 4096 / 8192 52 instead of 44), more than 48 registers (19.4; 54).
+// CTAs of the second product start beside those of the first one and have up to 14 MB of their weights in shared
+// memory when h is there.
+// One token, with routing and combining, 2 experts of 2048 / 2048: 11.3 us (four launches 17.4), 8 of 1024 / 512: 10.5
+// (14.5), 8 of 2048 / 768: 16.6 (19.5), 8 of 4096 / 1536: 37 (41); 4 tokens, 2 experts of 1024 / 1024 each: 12.4 (15.0).
+// Tried: copies of 512 bytes (18.6 for the third), one weight row a job (20), the jobs of a CTA side by side, which
+// needs the codes of fewer rows (19.0; 2 experts of 4096 / 8192 52 instead of 42), a scale loaded for each job (17.9).
 #include "common.cuh"
 #include "host.h"
 #include "int8.cuh"
@@ -32,7 +32,13 @@ constexpr int kPiece = 1024;               // bytes of a weight row in a slot at
 constexpr int kSlots = 3;
 constexpr int kSlotBytes = kBlock * kPiece;
 constexpr int kRing = kSlots * kSlotBytes; // of a warp
-constexpr int kCodes = 16384;              // bytes of codes at most (two CTAs on an SM)
+// Shared memory of a CTA of the second product: over half of an SM's, under what a CTA of the first leaves.  So every SM
+// takes one of them while the first product runs; where two fit, SMs that are done early take two.  48 registers for
+// the same reason: one token, 2 experts of 4096 / 8192 42 us, with up to 64 registers 48, and 54 where two fit as well.
+constexpr int kAlone = 116 * 1024;
+constexpr int kCodes = 16384;              // bytes of codes at most
+
+static_assert(kWarps * kRing + kCodes <= kAlone);
 
 struct Args {
     Int8Gemm g;              // A: hidden [tokens, K] or h [M, K]; N: output channels; B: [E, N or 2 N, K]
@@ -100,7 +106,7 @@ struct RowPart {
 // X: bf16 or fp16, the first product (hidden rows, silu(g) * u in fp32); float, the second one (rows of h).
 // K is a multiple of 16.
 template <typename X>
-__global__ void __launch_bounds__(kThreads, 2) int8_moe_gemv_kernel(const Args a) {
+__global__ void __maxnreg__(48) int8_moe_gemv_kernel(const Args a) {
     constexpr bool kFirst = sizeof(X) == 2;
     constexpr int kOuts = kFirst ? kBlock / 2 : kBlock;   // output channels of a job
     extern __shared__ __align__(128) uint8_t smem[];   // [kWarps][kSlots][kBlock][kPiece], then codes [tokens][K]
@@ -194,7 +200,15 @@ __global__ void __launch_bounds__(kThreads, 2) int8_moe_gemv_kernel(const Args a
         copy(ahead, i);
         next(ahead);
     }
-    float sb = pieces > 0 && lane < kBlock ? __ldg(a.g.scale_B + weight_row(p)) : 0.0f;
+    // lane i: the scale of weight row i % kBlock of this warp's job i / kBlock (of 16; a load per job would be waited for)
+    auto channel_scales = [&](int job) {
+        const int at = first + (job + lane / kBlock) * stride, on = lane % kBlock;
+        if (at >= jobs) return 0.0f;
+        const int row = at / across, base = (at - row * across) * kOuts;
+        const long long w = static_cast<long long>(expert_of[row0 + row]) * (N * (kBlock / kOuts));
+        return __ldg(a.g.scale_B + w + (on / kOuts) * N + base + on % kOuts);
+    };
+    float sb = channel_scales(0);
     if (!kFirst) {
         pdl_wait_prior();
         pdl_launch_dependents();
@@ -211,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 2) int8_moe_gemv_kernel(const Args a
     }
     __syncthreads();
 
-    int acc[kBlock], slot = 0;
+    int acc[kBlock], slot = 0, job = 0;
     uint32_t lap = 0;
 #pragma unroll
     for (int j = 0; j < kBlock; ++j) acc[j] = 0;
@@ -260,10 +274,11 @@ __global__ void __launch_bounds__(kThreads, 2) int8_moe_gemv_kernel(const Args a
                 if (lane == j) sum = all;
                 acc[j] = 0;
             }
-            float v = __fmul_rn(__fmul_rn(static_cast<float>(sum), scale[source]), sb);
+            const float sb_own = __shfl_sync(0xffffffffu, sb, (job & (32 / kBlock - 1)) * kBlock + (lane & (kBlock - 1)));
+            float v = __fmul_rn(__fmul_rn(static_cast<float>(sum), scale[source]), sb_own);
             if (kFirst) v = silu_mul(v, __shfl_down_sync(0xffffffffu, v, kOuts));
             if (lane < kOuts) store_out(a.g.D, a.g.out_dtype, static_cast<size_t>(done.row) * N + done.block * kOuts + lane, v);
-            if (i + 1 < pieces && lane < kBlock) sb = __ldg(a.g.scale_B + weight_row(p));
+            if ((++job & (32 / kBlock - 1)) == 0) sb = channel_scales(job);
         }
     }
 }
@@ -275,14 +290,15 @@ int launch(Args a, cudaStream_t s) {
     LSG_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_relaxed)) {
         LSG_CUDA_TRY(cudaFuncSetAttribute(int8_moe_gemv_kernel<X>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          kWarps * kRing + kCodes));
+                                          kAlone));
         if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_relaxed);
     }
     const long long jobs = static_cast<long long>(a.g.M) * a.g.N / (sizeof(X) == 2 ? kBlock / 2 : kBlock);
     const int ctas = static_cast<int>(std::min<long long>(sm_count(), jobs));
     a.status = device_status_word();
     a.limit = wait_limit_cycles();
-    const size_t smem = kWarps * kRing + static_cast<size_t>(a.tokens) * a.g.K;
+    size_t smem = kWarps * kRing + static_cast<size_t>(a.tokens) * a.g.K;
+    if (sizeof(X) == 4) smem = std::max(smem, static_cast<size_t>(kAlone));
     LSG_CUDA_TRY(launch_kernel(int8_moe_gemv_kernel<X>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, s, true, a));
     return LSG_OK;
 }
