@@ -523,6 +523,40 @@ def test_weights_made_right_before(ops, M):
         assert torch.equal(d, want[(i // 2) % 3]), i
 
 
+@pytest.mark.parametrize("T,k", [(1, 8), (2, 4), (3, 2), (5, 2)])
+def test_experts_one_layer_behind_the_other(ops, T, k):
+    """Layers in one pair of weight buffers: offsets, scales and weights are written right in front of each
+    call, whose result is the next one's input; with a wait between all launches every layer's bits are the same.
+    (silu(g) * u is about quadratic in its input: without a norm the last layers' values fall below bf16's range, so
+    what counts is the first ones'.)"""
+    g = torch.Generator().manual_seed(T)
+    E, H, I = 16, 1024, 512
+    layers = [experts(g, E, H, I) for _ in range(3)]
+    x = torch.randn(T, H, generator=g).to(BF16).cuda()
+    logits = [torch.randn(T, E, generator=g).cuda() for _ in range(3)]
+    now = [torch.empty_like(t) for t in layers[0]]
+
+    def run(wait):
+        h, every = x.clone(), []
+        for n in range(9):
+            idx, w = ops.moe_route(logits[(n + n // 3) % 3], k)
+            offs, _, inv = ops.moe_permutation(idx, E)
+            for t, src in zip(now, layers[n % 3]):
+                t.copy_(src)
+            wait()
+            rows = ops.int8_moe_ffn(h, offs, inv, k, *now)
+            wait()
+            h = ops.moe_unpermute(rows, inv, w)
+            wait()
+            every += [rows, h]
+        return every
+
+    want = run(torch.cuda.synchronize)
+    assert all(bool(d.isfinite().all()) for d in want) and all(bool(d.any()) for d in want[:6])
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(run(lambda: None), want))
+
+
 @pytest.mark.parametrize("T", [3, 400])
 def test_experts_on_two_streams(ops, T):
     g = torch.Generator().manual_seed(T)
