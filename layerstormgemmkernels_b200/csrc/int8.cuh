@@ -32,7 +32,7 @@ bool int8_gemv_takes(int M, int N, int K);
 int int8_gemv(const Int8Gemm& a, int x_dtype, cudaStream_t s);
 // The expert block for a few rows on streaming mat-vecs (int8_moe_gemv.cu): whether these sizes go there, and both
 // products.  first: A the hidden rows (lda in values), B [E, 2 N, K], D fp32 h [M, N]; second: A is h.
-bool int8_moe_gemv_takes(int tokens, int rows, int H, int I);
+bool int8_moe_gemv_takes(int tokens, int top_k, int E, int H, int I);
 int int8_moe_gemv(const Int8Gemm& first, int x_dtype, const int32_t* inv, int top_k, const Int8Gemm& second, cudaStream_t s);
 // On the tensor cores (int8_mma.cu).  swiglu: B is [E, 2 N, K], gate rows in front of up rows, and D
 // fp32 silu(gate) * up.  early: the launch in front on the stream is int8_quant_rows, which writes A.

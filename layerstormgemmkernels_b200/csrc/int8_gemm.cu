@@ -192,7 +192,7 @@ extern "C" int lsg_int8_moe_ffn(const lsg_int8_moe_ffn_params* p, void* workspac
     b.A = act; b.lda = f.ldi; b.B = static_cast<const int8_t*>(p->down); b.ldb = I;
     b.D = p->D; b.out_dtype = p->output_dtype; b.scale_A = act_scales; b.scale_B = p->down_scales;
     b.N = H; b.K = I;
-    if (int8_moe_gemv_takes(p->num_tokens, rows, H, I)) {
+    if (int8_moe_gemv_takes(p->num_tokens, p->top_k, p->num_experts, H, I)) {
         a.A = static_cast<const int8_t*>(p->hidden); a.lda = p->ld_hidden;
         b.A = reinterpret_cast<const int8_t*>(h); b.lda = I;
         return int8_moe_gemv(a, p->input_dtype, p->inv_perm, p->top_k, b, s);
