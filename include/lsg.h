@@ -765,6 +765,10 @@ LSG_API int lsg_moe_permute_dtype(const void* hidden, int dtype, const int32_t* 
                                   int H, void* out, void* stream);
 LSG_API int lsg_moe_unpermute_dtype(const void* y, int dtype, const int32_t* inv_perm, const float* topk_weights, int rows,
                                     int num_tokens, int top_k, int H, void* out, void* stream);
+/* lsg_moe_unpermute_dtype with an output of its own type: bf16 or fp16 from f32 rows (one rounding
+ * between the experts and the output), or the rows' type. */
+LSG_API int lsg_moe_unpermute_to(const void* y, int dtype, const int32_t* inv_perm, const float* topk_weights, int rows,
+                                 int num_tokens, int top_k, int H, void* out, int out_dtype, void* stream);
 
 /* Gradients of the three steps (dtype: bf16, fp16 or f32 for rows and tokens, fp32 for weights and
  * logits; top_k <= 16; sums in fp32 in a fixed order, no atomics).

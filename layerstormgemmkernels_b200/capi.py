@@ -208,6 +208,7 @@ def _load():
         "lsg_int8_moe_ffn": (ci, [ctypes.POINTER(Int8MoeFfnParams), vp, sz, vp]),
         "lsg_moe_permute_dtype": (ci, [vp, ci, vp, ci, ci, ci, ci, vp, vp]),
         "lsg_moe_unpermute_dtype": (ci, [vp, ci, vp, vp, ci, ci, ci, ci, vp, vp]),
+        "lsg_moe_unpermute_to": (ci, [vp, ci, vp, vp, ci, ci, ci, ci, vp, ci, vp]),
         "lsg_moe_permute_backward": (ci, [vp, ci, vp, ci, ci, ci, ci, vp, vp]),
         "lsg_moe_unpermute_backward": (ci, [vp, vp, ci, vp, vp, vp, ci, ci, ci, ci, ci, vp, vp, vp]),
         "lsg_moe_route_backward": (ci, [vp, vp, vp, ci, ci, ci, vp, vp]),

@@ -93,11 +93,20 @@ __device__ __forceinline__ void slot_rows(const int32_t* inv, size_t at, int row
         if (row[s] >= rows) row[s] = -1;
     }
 }
-// out[t] = sum over slots, in order, of (w ? w[t,s] : 1) * y[inv[t,s]]; k <= K.
-template <typename T, int P, int K>
+// Four values of a 16-bit type, rounded from fp32 and stored as one: 16 bytes of fp32 rows leave as 8.
+template <typename O>
+__device__ __forceinline__ void store4(O* p, const float (&f)[4]) {
+    alignas(8) O v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = from_f<O>(f[i]);
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+}
+
+// out[t] = sum over slots, in order, of (w ? w[t,s] : 1) * y[inv[t,s]], rounded once to O; k <= K.
+template <typename T, typename O, int P, int K>
 __global__ void __launch_bounds__(256)
 moe_sum_slots_kernel(const Piece<T, P>* __restrict__ y, const int32_t* __restrict__ inv, const float* __restrict__ w,
-                     int rows, int k, int per_row, Piece<T, P>* __restrict__ out) {
+                     int rows, int k, int per_row, O* __restrict__ out) {
     pdl_launch_dependents();
     pdl_wait_prior();
     const size_t t = blockIdx.x;
@@ -122,7 +131,6 @@ moe_sum_slots_kernel(const Piece<T, P>* __restrict__ y, const int32_t* __restric
         for (int u = 0; u < U; ++u) {
             const int c = c0 + u * blockDim.x;
             if (c >= per_row) break;
-            Piece<T, P> o;
             float acc[P];
 #pragma unroll
             for (int i = 0; i < P; ++i) acc[i] = 0.0f;
@@ -133,8 +141,13 @@ moe_sum_slots_kernel(const Piece<T, P>* __restrict__ y, const int32_t* __restric
 #pragma unroll
                 for (int i = 0; i < P; ++i) acc[i] = fmaf(ws[s], f[i], acc[i]);
             }
-            o.set(acc);
-            out[t * per_row + c] = o;
+            if constexpr (P > 1 && !std::is_same<T, O>::value) {
+                store4(out + (t * per_row + c) * P, acc);
+            } else {
+                Piece<O, P> o;
+                o.set(acc);
+                reinterpret_cast<Piece<O, P>*>(out)[t * per_row + c] = o;
+            }
         }
     }
 }
@@ -291,10 +304,10 @@ int threads_for(int per_row, int most = 256) {
 
 bool whole_pieces(int H, size_t size, uintptr_t at) { return (static_cast<size_t>(H) * size) % 16 == 0 && (at & 15) == 0; }
 
-template <typename T, int P, int K>
-int launch_sum(const void* y, const int32_t* inv, const float* w, int rows, int tokens, int k, int per_row, void* out, cudaStream_t s) {
-    LSG_CUDA_TRY(launch_kernel(moe_sum_slots_kernel<T, P, K>, dim3(static_cast<unsigned>(tokens)), dim3(threads_for(per_row, tokens >= 2048 ? 128 : 256)), 0, s,
-                               true, static_cast<const Piece<T, P>*>(y), inv, w, rows, k, per_row, static_cast<Piece<T, P>*>(out)));
+template <typename T, int P, int K, typename O>
+int launch_sum(const void* y, const int32_t* inv, const float* w, int rows, int tokens, int k, int per_row, O* out, cudaStream_t s) {
+    LSG_CUDA_TRY(launch_kernel(moe_sum_slots_kernel<T, O, P, K>, dim3(static_cast<unsigned>(tokens)), dim3(threads_for(per_row, tokens >= 2048 ? 128 : 256)), 0, s,
+                               true, static_cast<const Piece<T, P>*>(y), inv, w, rows, k, per_row, out));
     return LSG_OK;
 }
 template <typename T, int P, int K>
@@ -312,13 +325,15 @@ int launch_unpermute_backward(const void* grad_out, const void* y, const int32_t
     (k <= 2 ? fn<T, P, 2>(__VA_ARGS__)                                                                 \
             : (k <= 4 ? fn<T, P, 4>(__VA_ARGS__) : (k <= 8 ? fn<T, P, 8>(__VA_ARGS__) : fn<T, P, 16>(__VA_ARGS__))))
 
-template <typename T>
+// O: what the sums are rounded to, the rows' own type or 16 bits from fp32 rows.
+template <typename T, typename O = T>
 int sum_slots(const void* y, const int32_t* inv, const float* w, int rows, int tokens, int k, int H, void* out,
               cudaStream_t s) {
     constexpr int P = 16 / sizeof(T);
+    O* o = static_cast<O*>(out);
     if (whole_pieces(H, sizeof(T), reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)))
-        return LSG_BY_SLOTS(launch_sum, P, y, inv, w, rows, tokens, k, H / P, out, s);
-    return LSG_BY_SLOTS(launch_sum, 1, y, inv, w, rows, tokens, k, H, out, s);
+        return LSG_BY_SLOTS(launch_sum, P, y, inv, w, rows, tokens, k, H / P, o, s);
+    return LSG_BY_SLOTS(launch_sum, 1, y, inv, w, rows, tokens, k, H, o, s);
 }
 
 template <typename T>
@@ -382,6 +397,24 @@ extern "C" int lsg_moe_unpermute_dtype(const void* y, int dtype, const int32_t* 
     if (num_tokens == 0 || H == 0) return LSG_OK;
     if ((rows > 0 && !y) || !inv_perm || !topk_weights || !out) return fail(LSG_ERR_INVALID, "moe_unpermute: null pointer");
     return LSG_BY_DTYPE(sum_slots)(y, inv_perm, topk_weights, rows, num_tokens, top_k, H, out, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lsg_moe_unpermute_to(const void* y, int dtype, const int32_t* inv_perm, const float* topk_weights, int rows,
+                                    int num_tokens, int top_k, int H, void* out, int out_dtype, void* stream) {
+    if (out_dtype == dtype)
+        return lsg_moe_unpermute_dtype(y, dtype, inv_perm, topk_weights, rows, num_tokens, top_k, H, out, stream);
+    if (dtype != LSG_DTYPE_F32 || (out_dtype != LSG_DTYPE_BF16 && out_dtype != LSG_DTYPE_F16))
+        return fail(LSG_ERR_UNSUPPORTED, "moe_unpermute: the output is of the rows' type, or bf16 or fp16 from f32 rows");
+    int rc = check_moe("moe_unpermute", dtype, num_tokens, top_k, H, y, nullptr);
+    if (rc == LSG_OK) rc = check_moe("moe_unpermute", out_dtype, num_tokens, top_k, H, out, nullptr);
+    if (rc != LSG_OK) return rc;
+    if (rows < 0) return fail(LSG_ERR_INVALID, "moe_unpermute: negative shape");
+    if (num_tokens == 0 || H == 0) return LSG_OK;
+    if ((rows > 0 && !y) || !inv_perm || !topk_weights || !out) return fail(LSG_ERR_INVALID, "moe_unpermute: null pointer");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (out_dtype == LSG_DTYPE_F16)
+        return sum_slots<float, __half>(y, inv_perm, topk_weights, rows, num_tokens, top_k, H, out, s);
+    return sum_slots<float, __nv_bfloat16>(y, inv_perm, topk_weights, rows, num_tokens, top_k, H, out, s);
 }
 
 extern "C" int lsg_moe_permute_backward(const void* grad_rows, int dtype, const int32_t* inv_perm, int rows, int num_tokens,

@@ -857,18 +857,24 @@ def moe_permute(hidden, perm, top_k):
     return out
 
 
-def moe_unpermute(y, inv_perm, topk_weights):
+def moe_unpermute(y, inv_perm, topk_weights, output_dtype=None):
     """out[t] = sum over slots of topk_weights[t,s] * y[inv_perm[t*k+s]], bf16, fp16 or fp32; pairs
-    without a row (inv_perm < 0) add nothing."""
+    without a row (inv_perm < 0) add nothing.
+
+    The sum is rounded once to the rows' type; fp32 rows also go to output_dtype 'bf16' or 'fp16', so
+    that experts' rows kept in fp32 leave with one rounding (bf16 rows make it two)."""
     T, k = topk_weights.shape
     H = y.size(1)
-    if y.dtype != torch.bfloat16 or H % 2:           # lsg_moe_unpermute takes bf16 in pairs
+    to = y.dtype
+    if output_dtype is not None:
+        to = torch.float32 if output_dtype in ("fp32", "float32") else _parse_output_dtype(output_dtype)[1]
+    if y.dtype != torch.bfloat16 or H % 2 or to != y.dtype:      # lsg_moe_unpermute takes bf16 in pairs
         _require_rows_of("moe_unpermute", y, [("inv_perm", inv_perm, torch.int32, (T * k,)),
                                               ("topk_weights", topk_weights, torch.float32, (T, k))])
         with torch.cuda.device(y.device):
-            out = torch.empty((T, H), dtype=y.dtype, device=y.device)
-            capi.check(_lib.lsg_moe_unpermute_dtype(y.data_ptr(), _CODE[y.dtype], inv_perm.data_ptr(),
-                                                    topk_weights.data_ptr(), y.size(0), T, k, H, out.data_ptr(), _stream()))
+            out = torch.empty((T, H), dtype=to, device=y.device)
+            capi.check(_lib.lsg_moe_unpermute_to(y.data_ptr(), _CODE[y.dtype], inv_perm.data_ptr(), topk_weights.data_ptr(),
+                                                 y.size(0), T, k, H, out.data_ptr(), _CODE[to], _stream()))
         return out
     out = y.new_empty((T, H), dtype=torch.bfloat16)
     capi.check(_lib.lsg_moe_unpermute(y.data_ptr(), inv_perm.data_ptr(), topk_weights.data_ptr(), T, k, H,

@@ -1,0 +1,79 @@
+"""GPU tests of the ways of rows to the experts and back: what the combination rounds, and rows that start
+anywhere.
+
+Tolerances, with u = 2^-24: a sum of k products in fp32 is off by at most (k + 1) u times the sum of the
+magnitudes, and storing it adds half a step of the type (bf16 2^-8, fp16 2^-11 of the value; fp16 below
+its normal range 2^-25)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+HALF_STEP = {BF16: 2.0 ** -8, FP16: 2.0 ** -11, FP32: U}
+NAME = {BF16: "bf16", FP16: "fp16", FP32: "fp32"}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from layerstormgemmkernels_b200 import ops as _ops
+    return _ops
+
+
+def routed(ops, T, E, k, seed):
+    g = torch.Generator().manual_seed(seed)
+    idx, w = ops.moe_route(torch.randn(T, E, generator=g).cuda(), k)
+    if T > 4:
+        idx[1] = -1                      # a token that no expert takes
+        idx[2, 0] = E                    # an expert that is not there
+    offs, perm, inv = ops.moe_permutation(idx, E)
+    return g, w, offs, perm, inv
+
+
+def check_sum(out, y, inv, w):
+    iv, (T, k) = inv.cpu().long().view(w.shape), w.shape
+    part = torch.where((iv >= 0).unsqueeze(-1), y.cpu().double()[iv.clamp_min(0)], torch.zeros(1, dtype=torch.float64))
+    part = part * w.cpu().double().unsqueeze(-1)
+    want = part.sum(1)
+    tol = (k + 1) * U * part.abs().sum(1) * (1 + 2.0 ** -7) + HALF_STEP[out.dtype] * want.abs() + (2.0 ** -25 if out.dtype == FP16 else 0)
+    assert bool(((out.cpu().double() - want).abs() <= tol).all())
+
+
+# -----------------------------------------------------------------------------------------
+# One rounding from fp32 rows to a 16-bit output
+# -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("to", [BF16, FP16])
+@pytest.mark.parametrize("T,E,k,H", [(1, 4, 1, 4), (1, 128, 8, 2048), (5, 4, 4, 33), (7, 6, 3, 1), (33, 60, 4, 1001), (130, 8, 2, 4096),
+                                     (64, 16, 16, 260), (2100, 16, 6, 512)])
+def test_fp32_rows_leave_with_one_rounding(ops, T, E, k, H, to):
+    """The fp32 combination's bits, rounded once; rows that start 4 bytes off too."""
+    g, w, offs, perm, inv = routed(ops, T, E, k, T + H)
+    flat = torch.randn(T * k * H + 1, generator=g).cuda()
+    for y in (flat[:-1].view(T * k, H), flat[1:].view(T * k, H)):
+        out = ops.moe_unpermute(y, inv, w, NAME[to])
+        assert out.dtype == to and torch.equal(out, ops.moe_unpermute(y, inv, w).to(to))
+        check_sum(out, y, inv, w)
+        assert torch.equal(ops.moe_unpermute(y, inv, w, "fp32"), ops.moe_unpermute(y, inv, w))
+
+
+def test_experts_rows_in_fp32(ops):
+    """Experts' rows in fp32 and a bf16 output: off by one rounding, at most half a step of bf16, from the
+    combination in 64 bits of the rows that the block formed."""
+    g = torch.Generator().manual_seed(3)
+    T, E, k, H, I = 50, 8, 2, 512, 256
+    hidden = torch.randn(T, H, generator=g).to(BF16).cuda()
+    gate_up, gus = ops.weight_int8_quant((torch.randn(E, 2 * I, H, generator=g) * 0.05).to(BF16).cuda())
+    down, ds = ops.weight_int8_quant((torch.randn(E, H, I, generator=g) * 0.05).to(BF16).cuda())
+    idx, w = ops.moe_route(torch.randn(T, E, generator=g).cuda(), k)
+    offs, _, inv = ops.moe_permutation(idx, E)
+    rows = ops.int8_moe_ffn(hidden, offs, inv, k, gate_up, gus, down, ds, "fp32")
+    check_sum(ops.moe_unpermute(rows, inv, w, "bf16"), rows, inv, w)
+
+
+def test_output_types_that_are_refused(ops):
+    y, inv, w = torch.randn(8, 16, device="cuda"), torch.arange(8, dtype=torch.int32, device="cuda"), torch.ones(4, 2, device="cuda")
+    for bad in (lambda: ops.moe_unpermute(y.half(), inv, w, "bf16"), lambda: ops.moe_unpermute(y.bfloat16(), inv, w, "fp32"),
+                lambda: ops.moe_unpermute(y, inv, w, "int8")):
+        with pytest.raises(RuntimeError):
+            bad()

@@ -155,3 +155,17 @@ def test_operators_refuse_cpu_tensors(capi):
                 lambda: ops.moe_route_backward(inv.view(4, 2), s.view(4, 2), s.view(4, 2), 8)):
         with pytest.raises(RuntimeError, match="CUDA"):
             bad()
+
+
+def test_unpermute_output_type_refusals(capi):
+    f = capi.lib.lsg_moe_unpermute_to
+    for args, error, text in (((P, 0, P, P, 8, 4, 2, 64, P, 2, None), RuntimeError, "rows' type"),
+                              ((P, 1, P, P, 8, 4, 2, 64, P, 9, None), RuntimeError, "rows' type"),
+                              ((P, 1, P, P, 8, 4, 17, 64, P, 0, None), ValueError, "top_k"),
+                              ((P + 2, 1, P, P, 8, 4, 2, 64, P, 0, None), RuntimeError, "aligned"),
+                              ((P, 1, P, P, 8, 4, 2, 64, P + 1, 0, None), RuntimeError, "aligned"),
+                              ((P, 1, None, P, 8, 4, 2, 64, P, 0, None), ValueError, "null"),
+                              ((P, 1, P, P, -1, 4, 2, 64, P, 0, None), ValueError, "negative")):
+        with pytest.raises(error, match=text):
+            capi.check(f(*args))
+    assert f(None, 1, None, None, 0, 0, 2, 64, None, 0, None) == 0
