@@ -750,12 +750,13 @@ LSG_API int lsg_ep_return_rows_group(const void* y_bf16, const int32_t* dst_star
  * No counterpart in the reference. */
 LSG_API int lsg_ep_barrier(void* const* flag_ptrs, int rank, int world, int mode, void* stream);
 
-/* out[row,:] = hidden[perm[row] / top_k, :]   (bf16, H multiple of 8). */
+/* out[row,:] = hidden[perm[row] / top_k, :]   (bf16, H multiple of 8, 16-byte aligned buffers). */
 LSG_API int lsg_moe_permute(const void* hidden_bf16, const int32_t* perm, int rows, int top_k, int H,
                             void* out_bf16, void* stream);
 
 /* out[t,:] = sum over slots s (in order) of topk_weights[t,s] * y[inv_perm[t*k+s], :],
- * fp32 fused multiply-adds, rounded to bf16; pairs without a row (inv_perm < 0) add nothing. */
+ * fp32 fused multiply-adds, rounded to bf16; pairs without a row (inv_perm < 0) add nothing.
+ * H even, y and out on 4-byte boundaries. */
 LSG_API int lsg_moe_unpermute(const void* y_bf16, const int32_t* inv_perm, const float* topk_weights,
                               int num_tokens, int top_k, int H, void* out_bf16, void* stream);
 

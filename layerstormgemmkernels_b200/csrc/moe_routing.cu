@@ -489,7 +489,8 @@ extern "C" int lsg_moe_permutation(const int32_t* topk_idx, int num_tokens, int 
 
 extern "C" int lsg_moe_permute(const void* hidden_bf16, const int32_t* perm, int rows, int top_k, int H,
                                void* out_bf16, void* stream) {
-    if (rows <= 0) return LSG_OK;
+    if (H < 0) return fail(LSG_ERR_INVALID, "moe_permute: negative shape");
+    if (rows <= 0 || H == 0) return LSG_OK;
     if (!hidden_bf16 || !perm || !out_bf16) return fail(LSG_ERR_INVALID, "moe_permute: null pointer");
     if (H % 8 != 0 || (reinterpret_cast<uintptr_t>(hidden_bf16) & 15) || (reinterpret_cast<uintptr_t>(out_bf16) & 15))
         return fail(LSG_ERR_ALIGNMENT, "moe_permute: H must be a multiple of 8 and buffers 16-byte aligned");
@@ -503,9 +504,12 @@ extern "C" int lsg_moe_permute(const void* hidden_bf16, const int32_t* perm, int
 
 extern "C" int lsg_moe_unpermute(const void* y_bf16, const int32_t* inv_perm, const float* topk_weights,
                                  int num_tokens, int top_k, int H, void* out_bf16, void* stream) {
-    if (num_tokens <= 0) return LSG_OK;
+    if (H < 0) return fail(LSG_ERR_INVALID, "moe_unpermute: negative shape");
+    if (num_tokens <= 0 || H == 0) return LSG_OK;
     if (!y_bf16 || !inv_perm || !topk_weights || !out_bf16) return fail(LSG_ERR_INVALID, "moe_unpermute: null pointer");
     if (H % 2 != 0) return fail(LSG_ERR_INVALID, "moe_unpermute: H must be even");
+    if ((reinterpret_cast<uintptr_t>(y_bf16) | reinterpret_cast<uintptr_t>(out_bf16)) & 3)
+        return fail(LSG_ERR_ALIGNMENT, "moe_unpermute: rows are read in pairs of bf16, on 4-byte boundaries");
     if (H % 8 == 0 && top_k <= 8 && ((reinterpret_cast<uintptr_t>(y_bf16) | reinterpret_cast<uintptr_t>(out_bf16)) & 15) == 0) {
         const int vpr = H / 8;
         const int threads = vpr >= 256 ? 256 : ((vpr + 31) / 32) * 32;

@@ -830,31 +830,9 @@ def ep_expert_order(recv_counts, world, experts_per_rank, rows):
     return offs, order[:rows], inv[:rows]
 
 
-_CODE = {torch.bfloat16: capi.DTYPE_BF16, torch.float16: capi.DTYPE_F16, torch.float32: capi.DTYPE_F32}
-
-
-def _require_rows_of(op, t, others):
-    # t: the rows; others: (name, tensor, dtype, shape) that go with them
-    _require(t.is_cuda and t.dtype in _CODE and t.dim() == 2 and t.is_contiguous(),
-             f"{op}: rows must be contiguous BF16, FP16 or FP32 [rows, H] on CUDA")
-    for name, o, dtype, shape in others:
-        _require(o.device == t.device and o.dtype == dtype and o.is_contiguous() and tuple(o.shape) == shape,
-                 f"{op}: {name} must be contiguous {dtype} {shape} on the rows' device")
-
-
 def moe_permute(hidden, perm, top_k):
     """out[row] = hidden[perm[row] // top_k], bf16, fp16 or fp32 [T,H] -> [rows,H]."""
-    rows, H = perm.numel(), hidden.size(1)
-    if hidden.dtype != torch.bfloat16 or H % 8:      # lsg_moe_permute copies whole 16-byte pieces of bf16
-        _require_rows_of("moe_permute", hidden, [("perm", perm, torch.int32, (rows,))])
-        with torch.cuda.device(hidden.device):
-            out = torch.empty((rows, H), dtype=hidden.dtype, device=hidden.device)
-            capi.check(_lib.lsg_moe_permute_dtype(hidden.data_ptr(), _CODE[hidden.dtype], perm.data_ptr(), rows,
-                                                  hidden.size(0), int(top_k), H, out.data_ptr(), _stream()))
-        return out
-    out = hidden.new_empty((rows, H), dtype=torch.bfloat16)
-    capi.check(_lib.lsg_moe_permute(hidden.data_ptr(), perm.data_ptr(), rows, int(top_k), H, out.data_ptr(), _stream()))
-    return out
+    return _host.moe_permute(hidden, perm, top_k)
 
 
 def moe_unpermute(y, inv_perm, topk_weights, output_dtype=None):
@@ -863,23 +841,7 @@ def moe_unpermute(y, inv_perm, topk_weights, output_dtype=None):
 
     The sum is rounded once to the rows' type; fp32 rows also go to output_dtype 'bf16' or 'fp16', so
     that experts' rows kept in fp32 leave with one rounding (bf16 rows make it two)."""
-    T, k = topk_weights.shape
-    H = y.size(1)
-    to = y.dtype
-    if output_dtype is not None:
-        to = torch.float32 if output_dtype in ("fp32", "float32") else _parse_output_dtype(output_dtype)[1]
-    if y.dtype != torch.bfloat16 or H % 2 or to != y.dtype:      # lsg_moe_unpermute takes bf16 in pairs
-        _require_rows_of("moe_unpermute", y, [("inv_perm", inv_perm, torch.int32, (T * k,)),
-                                              ("topk_weights", topk_weights, torch.float32, (T, k))])
-        with torch.cuda.device(y.device):
-            out = torch.empty((T, H), dtype=to, device=y.device)
-            capi.check(_lib.lsg_moe_unpermute_to(y.data_ptr(), _CODE[y.dtype], inv_perm.data_ptr(), topk_weights.data_ptr(),
-                                                 y.size(0), T, k, H, out.data_ptr(), _CODE[to], _stream()))
-        return out
-    out = y.new_empty((T, H), dtype=torch.bfloat16)
-    capi.check(_lib.lsg_moe_unpermute(y.data_ptr(), inv_perm.data_ptr(), topk_weights.data_ptr(), T, k, H,
-                                      out.data_ptr(), _stream()))
-    return out
+    return _host.moe_unpermute(y, inv_perm, topk_weights, output_dtype)
 
 
 # ---------------------------------------------------------------------------

@@ -1,5 +1,5 @@
 // PyTorch extension module `lsg_torch_ops`: the host side of the eager operators of the 8-bit integer
-// family and of the MoE gradients (layerstormgemmkernels_b200/ops.py documents them) over the C ABI of
+// family, of the rows' ways to the experts and back, and of the MoE gradients (layerstormgemmkernels_b200/ops.py documents them) over the C ABI of
 // liblsg_b200.so.  Calls of these operators at decode sizes cost their host work; argument checks,
 // allocation and the call through ctypes take about 9 us, here they take about half.
 // torch supplies tensors, the caching allocator and the current stream of the inputs' device.
@@ -63,6 +63,12 @@ void need_dense(const char* op, const char* name, const Tensor& t) {
     if (!is_float(t) || !t.is_cuda() || t.dim() != 2 || !t.is_contiguous())
         refuse(op, std::string(name) + " must be contiguous BF16, FP16 or FP32 [rows, H] on CUDA");
 }
+// int32 indices or fp32 weights of `n` pairs, in any shape
+void need_pairs(const char* op, const char* name, const Tensor& t, at::ScalarType type, int64_t n, const Tensor& like) {
+    if (t.scalar_type() != type || t.device() != like.device() || !t.is_contiguous() || t.numel() != n)
+        refuse(op, std::string(name) + " must be " + std::to_string(n) + " contiguous values of " + c10::toString(type) + " on the rows' device");
+}
+bool lies_on(const Tensor& t, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
 // Sizes that the C ABI takes as int.
 int as_int(const char* op, int64_t v) {
     if (v < 0 || v > 0x7fffffff) refuse(op, "a size is outside 0 .. 2^31 - 1");
@@ -233,6 +239,45 @@ Tensor int8_moe_ffn(const Tensor& hidden, const Tensor& expert_offsets, const Te
     return D;
 }
 
+Tensor moe_permute(const Tensor& hidden, const Tensor& perm, int64_t top_k) {
+    const char* op = "moe_permute";
+    need_dense(op, "rows", hidden);
+    const int64_t rows = perm.numel(), T = hidden.size(0), H = hidden.size(1);
+    need_pairs(op, "perm", perm, at::kInt, rows, hidden);
+    if (top_k < 1) refuse(op, "top_k must be positive");
+    On on(hidden);
+    Tensor out = empty({rows, H}, hidden.scalar_type(), hidden);
+    const int32_t* p = static_cast<const int32_t*>(perm.data_ptr());
+    // bf16 in whole 16-byte pieces: a thread a piece (4096 x 8 rows of 768 13.9 us, 34.7 with a CTA a row)
+    if (hidden.scalar_type() == at::kBFloat16 && H % 8 == 0 && lies_on(hidden, 16))
+        check(lsg_moe_permute(hidden.data_ptr(), p, as_int(op, rows), as_int(op, top_k), as_int(op, H), out.data_ptr(), on.stream));
+    else
+        check(lsg_moe_permute_dtype(hidden.data_ptr(), code_of(hidden.scalar_type()), p, as_int(op, rows), as_int(op, T),
+                                    as_int(op, top_k), as_int(op, H), out.data_ptr(), on.stream));
+    return out;
+}
+
+Tensor moe_unpermute(const Tensor& y, const Tensor& inv_perm, const Tensor& topk_weights, const c10::optional<std::string>& output_dtype) {
+    const char* op = "moe_unpermute";
+    need_dense(op, "rows", y);
+    if (topk_weights.dim() != 2) refuse(op, "topk_weights must be [T, k]");
+    const int64_t T = topk_weights.size(0), k = topk_weights.size(1), rows = y.size(0), H = y.size(1);
+    need_pairs(op, "topk_weights", topk_weights, at::kFloat, T * k, y);
+    need_pairs(op, "inv_perm", inv_perm, at::kInt, T * k, y);
+    const at::ScalarType from = y.scalar_type(), to = output_dtype.has_value() ? out_type(*output_dtype) : from;
+    On on(y);
+    Tensor out = empty({T, H}, to, y);
+    const int32_t* inv = static_cast<const int32_t*>(inv_perm.data_ptr());
+    const float* w = static_cast<const float*>(topk_weights.data_ptr());
+    // bf16 in pairs has any number of slots, and 512 x 6 rows of 2048 take 2.7 us (3.8 by slots)
+    if (from == at::kBFloat16 && to == from && H % 2 == 0 && lies_on(y, 4))
+        check(lsg_moe_unpermute(y.data_ptr(), inv, w, as_int(op, T), as_int(op, k), as_int(op, H), out.data_ptr(), on.stream));
+    else
+        check(lsg_moe_unpermute_to(y.data_ptr(), code_of(from), inv, w, as_int(op, rows), as_int(op, T), as_int(op, k), as_int(op, H),
+                                   out.data_ptr(), code_of(to), on.stream));
+    return out;
+}
+
 Tensor moe_permute_backward(const Tensor& grad_rows, const Tensor& inv_perm, int64_t top_k) {
     const char* op = "moe_permute_backward";
     need_dense(op, "grad_rows", grad_rows);
@@ -293,7 +338,7 @@ Tensor moe_route_backward(const Tensor& topk_idx, const Tensor& topk_weights, co
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    m.doc() = "Host side of the eager 8-bit integer and MoE gradient operators; documented in layerstormgemmkernels_b200.ops.";
+    m.doc() = "Host side of the eager 8-bit integer, MoE row and MoE gradient operators; documented in layerstormgemmkernels_b200.ops.";
     m.def("dynamic_int8_quant", &dynamic_int8_quant);
     m.def("silu_mul_int8_quant", &silu_mul_int8_quant);
     m.def("int8_gemm", &int8_gemm);
@@ -301,6 +346,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("int8_grouped_gemm", &int8_grouped_gemm);
     m.def("moe_permute_int8", &moe_permute_int8);
     m.def("int8_moe_ffn", &int8_moe_ffn);
+    m.def("moe_permute", &moe_permute);
+    m.def("moe_unpermute", &moe_unpermute);
     m.def("moe_permute_backward", &moe_permute_backward);
     m.def("moe_unpermute_backward", &moe_unpermute_backward);
     m.def("moe_route_backward", &moe_route_backward);

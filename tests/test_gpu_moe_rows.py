@@ -77,3 +77,47 @@ def test_output_types_that_are_refused(ops):
                 lambda: ops.moe_unpermute(y, inv, w, "int8")):
         with pytest.raises(RuntimeError):
             bad()
+
+
+# -----------------------------------------------------------------------------------------
+# Rows of every type from any address; what no type takes
+# -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("T,E,k,H", [(1, 4, 1, 2), (5, 4, 4, 34), (33, 60, 4, 1002), (40, 8, 2, 2048), (17, 30, 12, 264)])
+def test_rows_from_any_address(ops, T, E, k, H, dtype):
+    """Rows that start one to eight values off an aligned buffer give the bits of an aligned copy."""
+    g, w, offs, perm, inv = routed(ops, T, E, k, T + H)
+    xs, ys = torch.randn(T * H + 8, generator=g).to(dtype).cuda(), torch.randn(T * k * H + 8, generator=g).to(dtype).cuda()
+    for off in (0, 1, 2, 3, 4, 8):
+        x, y = xs[off:off + T * H].view(T, H), ys[off:off + T * k * H].view(T * k, H)
+        n = int(offs[-1])
+        assert torch.equal(ops.moe_permute(x, perm, k)[:n], x[(perm[:n] // k).long()])
+        out = ops.moe_unpermute(y, inv, w)
+        assert torch.equal(out, ops.moe_unpermute(y.clone(), inv, w))
+        check_sum(out, y, inv, w)
+        assert torch.equal(out, ops.moe_unpermute(y, inv.view(T, k), w))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_rows_without_values_or_tokens(ops, dtype):
+    perm, w = torch.arange(6, dtype=torch.int32, device="cuda"), torch.ones(3, 2, device="cuda")
+    assert ops.moe_permute(torch.zeros(3, 0, dtype=dtype, device="cuda"), perm, 2).shape == (6, 0)
+    assert ops.moe_unpermute(torch.zeros(6, 0, dtype=dtype, device="cuda"), perm, w).shape == (3, 0)
+    assert ops.moe_permute(torch.zeros(0, 8, dtype=dtype, device="cuda"), perm[:0], 2).shape == (0, 8)
+    assert ops.moe_unpermute(torch.zeros(0, 8, dtype=dtype, device="cuda"), perm[:0], w[:0]).shape == (0, 8)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_rows_refused(ops, dtype):
+    """Every type alike: layouts, index and weight types and sizes that the kernels do not read."""
+    x, y = torch.zeros(4, 16, dtype=dtype, device="cuda"), torch.zeros(8, 16, dtype=dtype, device="cuda")
+    inv, w = torch.arange(8, dtype=torch.int32, device="cuda"), torch.ones(4, 2, device="cuda")
+    for bad in (lambda: ops.moe_permute(x.t(), inv, 2), lambda: ops.moe_permute(x[:, :8], inv, 2), lambda: ops.moe_permute(x, inv.long(), 2),
+                lambda: ops.moe_permute(x, inv.cpu(), 2), lambda: ops.moe_permute(x, inv[::2], 2),
+                lambda: ops.moe_unpermute(y.t(), inv, w), lambda: ops.moe_unpermute(y[:, :8], inv, w),
+                lambda: ops.moe_unpermute(y, inv.long(), w), lambda: ops.moe_unpermute(y, inv[:7], w),
+                lambda: ops.moe_unpermute(y, inv, w.half()), lambda: ops.moe_unpermute(y, inv, w.to(dtype).double()),
+                lambda: ops.moe_unpermute(y, inv, torch.ones(2, 4, device="cuda").t()), lambda: ops.moe_unpermute(y, inv.cpu(), w),
+                lambda: ops.moe_unpermute(y, inv, w.cpu())):
+        with pytest.raises(RuntimeError, match="must be"):
+            bad()

@@ -169,3 +169,27 @@ def test_unpermute_output_type_refusals(capi):
         with pytest.raises(error, match=text):
             capi.check(f(*args))
     assert f(None, 1, None, None, 0, 0, 2, 64, None, 0, None) == 0
+
+
+def test_bf16_rows_that_the_row_entries_refuse(capi):
+    """Rows off the boundaries that the bf16 entries read on; rows without values are nothing to do."""
+    L = capi.lib
+    for fn, args, error, text in ((L.lsg_moe_unpermute, (P + 2, P, P, 4, 2, 64, P, None), RuntimeError, "4-byte"),
+                                  (L.lsg_moe_unpermute, (P, P, P, 4, 2, 6, P + 2, None), RuntimeError, "4-byte"),
+                                  (L.lsg_moe_unpermute, (P, P, P, 4, 2, -2, P, None), ValueError, "negative"),
+                                  (L.lsg_moe_permute, (P + 8, P, 8, 2, 64, P, None), RuntimeError, "16-byte"),
+                                  (L.lsg_moe_permute, (P, P, 8, 2, -8, P, None), ValueError, "negative")):
+        with pytest.raises(error, match=text):
+            capi.check(fn(*args))
+    assert L.lsg_moe_permute(P, P, 8, 2, 0, P, None) == 0 and L.lsg_moe_unpermute(P, P, P, 4, 2, 0, P, None) == 0
+
+
+def test_row_operators_refuse_cpu_tensors(capi):
+    import torch
+    from layerstormgemmkernels_b200 import ops
+    inv, w = torch.zeros(8, dtype=torch.int32), torch.ones(4, 2)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        for bad in (lambda: ops.moe_permute(torch.zeros(4, 64, dtype=dtype), inv, 2),
+                    lambda: ops.moe_unpermute(torch.zeros(8, 64, dtype=dtype), inv, w)):
+            with pytest.raises(RuntimeError, match="rows must be contiguous BF16"):
+                bad()
