@@ -20,7 +20,9 @@
 // SwiGLU: of every 32 lanes 16 are gate rows and 16 the up rows of the same channels (one
 // five-dimensional box of the stacked weight puts them there), a shuffle brings g and u together and
 // silu(g) * u is stored in fp32: the quantizer that follows reads 4 bytes instead of 8.
-// Persistent except for split; every wait is time-limited.
+// Persistent except for split; every wait is time-limited.  A CTA whose wait runs out records it, tells the other CTA
+// of its pair and leaves its loops; what it and its pair have under way (copies into the stages, MMAs) is waited for
+// behind the closing barrier, so that nothing lands in shared or tensor memory that has been handed on.
 //
 // What bounds it.  Large products: the tensor pipe, busy nine tenths of the time (4096 x 14336 x 4096 in 153 us
 // as a burst, 3.1 Pop/s; 180 us when the power limit has taken the clock to 1.5 GHz), with operands coming
@@ -80,6 +82,18 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
     uint32_t r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
+}
+__device__ __forceinline__ uint32_t load_remote(uint32_t cluster_addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_remote(uint32_t cluster_addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+// Takes bytes that no copy will bring off a barrier's count.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 // Release at CTA scope: what the arrival hands over are tensor-memory reads that have completed.  At cluster
 // scope it would wait for the epilogue's stores to global memory (a quarter of the time of short-K tiles).
@@ -242,9 +256,11 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     uint64_t* empty = full + kMaxStages;
     uint64_t* acc_full = empty + kMaxStages;   // [2]
     uint64_t* acc_empty = acc_full + 2;        // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint64_t* drained = acc_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* scan = reinterpret_cast<int*>(tmem_slot + 2);                           // [16]
+    uint32_t* filled = tmem_slot + 18;                                           // stages filled; with weights at least
     float* scales = reinterpret_cast<float*>(smem + a.stages * stage_bytes + 512);   // [epilogue warps][2][16] of the tokens
     int* cum = reinterpret_cast<int*>(smem + a.stages * stage_bytes + 512 + kEpiWarps * 128);   // [E + 1] tiles of tokens before expert e
     int* start = cum + 1025;                                                      // [E + 1] first row
@@ -263,6 +279,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             mbar_init(&acc_full[i], 1);
             mbar_init(&acc_empty[i], kEpiWarps * CG);
         }
+        mbar_init(drained, 1);
         *abort_flag = 0;
         mbar_fence_init();
     }
@@ -338,12 +355,16 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     const int kb0 = SPLIT > 1 ? static_cast<int>(a.kblocks * rank / SPLIT) : 0;
     const int kb1 = SPLIT > 1 ? static_cast<int>(a.kblocks * (rank + 1) / SPLIT) : a.kblocks;
 
+    // before the closing barrier: behind it both CTAs of a pair find their flag set
+    auto give_up = [&] {
+        *abort_flag = 1;
+        if constexpr (CG == 2) store_remote(map_to_rank(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1), 1);
+    };
     if (warp == kEpiWarps) {
         // ------------------------------ TMA producer ------------------------------
         int s = 0;
         uint32_t lap = 0;
         bool ok = true;
-        
         const uint32_t full_at = CG == 2 ? map_to_rank(smem_u32(full), 0) : smem_u32(full);   // the leader's barriers
         // the weights of stage i, K blocks kb.., and the bytes that its barrier waits for
         auto load_weights = [&](int i, int kb, const Tile& t, int n_cta, int blocks) {
@@ -400,14 +421,10 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 }
             }
         }
-        if (!ok) {
-            *abort_flag = 1;
-            // copies in flight land before the CTA ends
-            if (CG == 1 || rank == 0)
-                for (int i = 0; i < a.stages; ++i) {
-                    const uint32_t n = lap + (i < s ? 1 : 0);   // times stage i was filled
-                    if (n > 0) mbar_wait_bounded(&full[i], (n - 1) & 1, a.status, kDevWaitFull);
-                }
+        if (!ok) give_up();
+        if (lane == 0) {
+            filled[0] = lap * a.stages + s;
+            filled[1] = max(filled[0], static_cast<uint32_t>(ahead));
         }
     } else if (warp == kEpiWarps + 1) {
         // ------------------------------ MMA issuer --------------------------------
@@ -450,7 +467,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 ab ^= 1;
                 acc_lap += ab == 0;
             }
-            if (!ok) *abort_flag = 1;
+            if (!ok) give_up();
         }
     } else {
         // ------------------------------ epilogue ---------------------------------
@@ -566,8 +583,40 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 acc_lap += ab == 0;
             }
         }
-        if (!ok) *abort_flag = 1;
+        if (!ok) give_up();
     }
+
+    // Behind the closing barrier of a CTA (pair) that gave up: the issuer waits for its MMAs, the producer for every
+    // stage's last copies.  The leader's barriers count both CTAs' bytes, and one of the two may have gone a stage
+    // further: the leader arms what it has not yet, and takes off what was never asked for.
+    auto drain = [&] {
+        const bool leads = CG == 1 || rank == 0;
+        if (warp == kEpiWarps + 1) {
+            if (leads && elect_one()) commit<CG>(drained);
+            __syncwarp();
+            mbar_wait_bounded(drained, 0, a.status, kDevWaitMma);
+        } else if (leads && warp == kEpiWarps && lane == 0) {
+            const uint32_t f0 = filled[0], w0 = filled[1];
+            uint32_t f1 = f0, w1 = w0;
+            if constexpr (CG == 2) {
+                const uint32_t theirs = map_to_rank(smem_u32(filled), 1);
+                f1 = load_remote(theirs);
+                w1 = load_remote(theirs + 4);
+            }
+            const uint32_t stages = a.stages, end = max(w0, w1), per_tile = (kb1 - kb0 + sub - 1) / sub;
+            for (uint32_t f = end > stages ? end - stages : 0; f < end; ++f) {
+                uint64_t* bar = &full[f % stages];
+                const uint32_t blocks = WIDE ? sub : min(sub, kb1 - kb0 - static_cast<int>(f % per_tile) * sub);
+                const uint32_t weights = blocks * kABytes, tokens = blocks * a.tn * kKB;
+                uint32_t never = (f >= w0 ? weights : 0) + (f >= f0 ? tokens : 0);
+                if (CG == 2) never += (f >= w1 ? weights : 0) + (f >= f1 ? tokens : 0);
+                if (f >= w0) mbar_arrive_expect_tx(bar, CG * (weights + tokens));
+                if (never > 0) mbar_complete_tx(bar, never);
+                mbar_wait_bounded(bar, (f / stages) & 1, a.status, kDevWaitFull);
+            }
+        }
+        __syncwarp();
+    };
 
     tc_fence_before();
     __syncwarp();
@@ -584,6 +633,7 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         const size_t size = a.out_dtype == LSG_DTYPE_F32 ? 4 : 2;
         const bool whole = n + 3 < a.N && (a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.D) & (4 * size - 1)) == 0;
         cluster_sync();
+        if (*abort_flag) drain();
         for (int c0 = static_cast<int>(rank) + SPLIT * warp; c0 < t.rows; c0 += U * kApart) {
             float4 p[U][SPLIT];
             float sa[U];
@@ -624,8 +674,13 @@ int8_mma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         cluster_sync();      // nobody leaves while its sums are read
     } else if constexpr (CG == 2) {
         cluster_sync();
+        if (*abort_flag) {
+            drain();
+            cluster_sync();      // the leader has waited for the other CTA's copies
+        }
     } else {
         __syncthreads();
+        if (*abort_flag) drain();
     }
     if (warp == kEpiWarps + 1) {
         tc_fence_after();
