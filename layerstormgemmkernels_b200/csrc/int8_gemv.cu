@@ -143,8 +143,8 @@ int8_gemv_kernel(const Int8Gemm a, int ldq, int slots, unsigned int* status, lon
     for (int m = 0; m < MR; ++m) acc[m] = 0;
     for (int i = 0; i < pieces; ++i) {
         if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[slot][warp], lap & 1, status, kDevWaitFull, 2000u, limit))) {
-            // give up, but not before the copies behind this one have landed
-            for (int j = 1; j < slots && i + j < pieces; ++j) {
+            // give up, but not before this copy and the ones behind it have landed
+            for (int j = 0; j < slots && i + j < pieces; ++j) {
                 const int other = (slot + j) % slots;
                 mbar_wait_bounded(&full[other][warp], (lap + (slot + j >= slots ? 1 : 0)) & 1, status, kDevWaitFull);
             }

@@ -231,8 +231,8 @@ __global__ void __maxnreg__(48) int8_moe_gemv_kernel(const Args a) {
     for (int j = 0; j < kBlock; ++j) acc[j] = 0;
     for (int i = 0; i < pieces; ++i) {
         if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][slot], lap & 1, a.status, kDevWaitFull, 2000u, a.limit))) {
-            // give up, but not before the copies behind this one have landed
-            for (int j = 1; j < kSlots && i + j < pieces; ++j) {
+            // give up, but not before this copy and the ones behind it have landed
+            for (int j = 0; j < kSlots && i + j < pieces; ++j) {
                 const int other = (slot + j) % kSlots;
                 mbar_wait_bounded(&full[warp][other], (lap + (slot + j >= kSlots ? 1 : 0)) & 1, a.status, kDevWaitFull);
             }

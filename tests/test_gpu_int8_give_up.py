@@ -67,3 +67,29 @@ def test_gate_and_up(ops, rows, I):
     offs = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
     inv = torch.arange(rows, dtype=torch.int32, device="cuda")
     gives_up_and_goes_on(lambda: ops.int8_moe_ffn(hidden, offs, inv, 1, gate_up, gus, down, ds, "fp32"))
+
+
+def test_streaming_forms_with_a_short_limit(ops):
+    """One row, and one token's experts: their waits are for copies of a few KB and end long before any limit.
+    Whatever a limit of one cycle does, the call returns and the next ones give the same bits."""
+    from layerstormgemmkernels_b200 import capi
+    x = torch.randn(1, 8192, generator=torch.Generator(device="cuda").manual_seed(8), device="cuda").to(BF16)
+    w, ws = codes(16384, 8192, 9), torch.ones(16384, device="cuda")
+    gate_up, down = codes(8 * 2048, 8192, 10).view(8, 2048, 8192), codes(8 * 8192, 1024, 11).view(8, 8192, 1024)
+    gus, ds = torch.full((8, 2048), 1e-5, device="cuda"), torch.ones(8, 8192, device="cuda")
+    offs = torch.arange(9, dtype=torch.int32, device="cuda").clamp_max(8)
+    inv = torch.arange(8, dtype=torch.int32, device="cuda")
+
+    def call():
+        return torch.cat([ops.int8_gemm_from_bf16(x, w, ws, "fp32").flatten(),
+                          ops.int8_moe_ffn(x, offs, inv, 8, gate_up, gus, down, ds, "fp32").flatten()])
+    want = call()
+    for _ in range(10):
+        capi.check(capi.lib.lsg_set_wait_limit_cycles(1))
+        try:
+            got = call()
+            if capi.device_status() == 0:
+                assert torch.equal(got, want)
+        finally:
+            capi.check(capi.lib.lsg_set_wait_limit_cycles(0))
+        assert torch.equal(call(), want) and capi.device_status() == 0
