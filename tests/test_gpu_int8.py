@@ -629,3 +629,20 @@ def test_refused_on_cuda(ops):
                 lambda: ops.weight_int8_quant(torch.zeros(2, 3, 20, dtype=BF16, device="cuda"))):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("top", [-20.0, -86.0, -87.4, -88.5, -89.0, -91.0])
+def test_silu_mul_of_gates_far_below_zero(ops, top):
+    """Rows whose gates are all far below zero, with values of `up` that bring silu(g) * u back to the size of
+    ordinary activations: nothing of them is lost.  e^(-|g| / 2) is off by two ulp at most and counts twice
+    (8 * 2^-24); the products with it, the sum, the reciprocal and the two products behind it add 2^-24 each:
+    14 * 2^-24 in all, below 2^-20."""
+    g = torch.Generator().manual_seed(7)
+    gate = top - torch.rand(3, 512, generator=g)
+    up = torch.randn(3, 512, generator=g) * math.exp(-top - 10)
+    h = gate.double() * torch.sigmoid(gate.double()) * up.double()
+    a = h.abs().amax(1)
+    codes, scales = ops.silu_mul_int8_quant(gate.cuda(), up.cuda())
+    assert bool(((scales.cpu().double() - a / 127).abs() <= a / 127 * 2.0 ** -19).all())
+    off = (codes.cpu().double() - h * 127 / a.unsqueeze(1)).abs().max()
+    assert off <= 0.5 + 127 * 2.0 ** -19, off
