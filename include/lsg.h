@@ -587,8 +587,9 @@ LSG_API int lsg_nvfp4_reformat_scales(const float* src, void* dst, int rows, int
  * weight.  Rows that are whole 16-byte pieces of at most 16384 values are read once. */
 LSG_API int lsg_dynamic_int8_quant(const void* x, long long ldx, int dtype, void* codes, long long ldq, float* scales,
                                    long long rows, int K, void* stream);
-/* The same of silu(gate) * up, formed in fp32 and not rounded in between; gate, up: bf16, fp16 or
- * f32 with row strides ldg, ldu (the halves of one [rows, 2 K] matrix, say). */
+/* The same of silu(gate) * up, formed in fp32 (off by at most 14 * 2^-24 of itself) and not rounded in
+ * between: the codes are the ones of the fp32 values' unrounded quotients.  gate, up: bf16, fp16 or f32
+ * with row strides ldg, ldu (the halves of one [rows, 2 K] matrix, say). */
 LSG_API int lsg_silu_mul_int8_quant(const void* gate, long long ldg, const void* up, long long ldu, int dtype,
                                     void* codes, long long ldq, float* scales, long long rows, int K, void* stream);
 /* The same of a token matrix, written to the rows of its (token, slot) pairs: the codes and scale of

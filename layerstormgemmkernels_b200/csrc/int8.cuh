@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace lsg {
 
 // |sum| <= 128 * 128 * K < 2^31, and K rounded up to 16 stays in the range
@@ -146,7 +148,7 @@ template <> struct Int8In<__half> {
 };
 template <> struct Int8In<float> {
     static constexpr int kVecs = 2;
-    static constexpr bool kOneFma = true;
+    static constexpr bool kOneFma = true;    // and a look at whether it fell next to half-way
     static __device__ __forceinline__ float get(const void* p, size_t i) { return static_cast<const float*>(p)[i]; }
     static __device__ __forceinline__ void unpack(const uint4* v, float (&f)[8]) {
         const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
@@ -170,7 +172,9 @@ constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an in
 // 2^-(15 + d) from the quotient; a quotient can be half-way only when a is 127 times a power of two,
 // where c is exact, or when it is 63.5 (127 is prime), where c on the upper side takes it to 64, the
 // even neighbour.  fp16 has other half-way cases (a = 381, x = 1.5): it forms the correctly rounded
-// quotient from the exact 127 x instead.  Rows below 2^-100 are moved up so that c stays finite.
+// quotient from the exact 127 x instead.  fp32 values (of silu(g) u) have quotients as near half-way as 2^-33: where
+// x c comes within 2^-16 above half-way (one value in 65536) two products and their rounding errors decide (settle).
+// Rows below 2^-100 are moved up so that c stays finite.
 struct RowScale {
     float scale, c, den, rcp;
     bool dead;   // all zero, or not finite: codes are 0
@@ -198,12 +202,52 @@ __device__ __forceinline__ uint32_t code_bits(float x, const RowScale& r) {
         return __float_as_uint(fmaf(x, r.c, kMagic));
     }
 }
+// fp32: |x| c less the code's magnitude n.  Only from -1/2 to 2^-16 above it can n be one too large (c is 127 / a
+// rounded up, so |x| c is never below the quotient).
+constexpr float kDoubt = -0.5f + 0x1.1p-16f;
+__device__ __forceinline__ float above_code(float x, uint32_t bits, const RowScale& r) {
+    const float f = fmaf(x, r.c, kMagic - __uint_as_float(bits));
+    return __uint_as_float(__float_as_uint(f) ^ (__float_as_uint(x) & 0x80000000u));
+}
+// The code in doubt: n, or n - 1 where 127 |x| / a is below n - 1/2 (or at it, and n is odd), that is by the sign of
+// 254 |x| - (2 n - 1) a.  In units of 1 / 256 the products stay in range; their difference is exact, since they lie
+// within a factor of two, and so are both products' rounding errors and the difference of these (at most 17 bits).
+__device__ __forceinline__ uint32_t settle(float x, uint32_t bits, const RowScale& r) {
+    if (above_code(x, bits, r) >= kDoubt) return bits;
+    const float n = fabsf(__uint_as_float(bits) - kMagic), m = fabsf(x);
+    const float w = 254.0f / 256.0f, h = fmaf(n, 2.0f / 256.0f, -1.0f / 256.0f);
+    const float p = w * m, q = h * r.den;
+    const float s = (p - q) + (fmaf(w, m, -p) - fmaf(h, r.den, -q));
+    if (s > 0.0f || (s == 0.0f && (bits & 1) == 0)) return bits;
+    return x < 0.0f ? bits + 1 : bits - 1;
+}
 template <typename T>
 __device__ __forceinline__ uint8_t code1(float x, const RowScale& r) {
-    return r.dead ? 0 : static_cast<uint8_t>(code_bits<T>(r.tiny ? x * 0x1p64f : x, r) & 0xFFu);
+    if (r.dead) return 0;
+    if (r.tiny) x *= 0x1p64f;
+    uint32_t q = code_bits<T>(x, r);
+    if constexpr (std::is_same<T, float>::value) q = settle(x, q, r);
+    return static_cast<uint8_t>(q & 0xFFu);
 }
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// Four at a time: few registers are held over the look at values in doubt.
+template <typename T>
+__device__ __forceinline__ uint32_t code4(const float* f, const RowScale& r) {
+    uint32_t q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = code_bits<T>(f[j], r);
+    if constexpr (std::is_same<T, float>::value) {
+        float least = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) least = fminf(least, above_code(f[j], q[j], r));
+        if (least < kDoubt) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[j] = settle(f[j], q[j], r);
+        }
+    }
+    return pack4(q[0], q[1], q[2], q[3]);
 }
 template <typename T>
 __device__ __forceinline__ uint2 code8(float (&f)[8], const RowScale& r) {
@@ -212,10 +256,8 @@ __device__ __forceinline__ uint2 code8(float (&f)[8], const RowScale& r) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] *= 0x1p64f;
     }
-    uint32_t q[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = code_bits<T>(f[j], r);
-    return make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+    const uint32_t low = code4<T>(f, r);
+    return make_uint2(low, code4<T>(f + 4, r));
 }
 
 #endif  // __CUDACC__

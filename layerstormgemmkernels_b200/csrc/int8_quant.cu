@@ -95,7 +95,7 @@ quant_short_rows_kernel(const RowQuantArgs a, long long rows) {
 
 // V pieces of eight values per thread.
 template <typename T, bool SILU, int V>
-__global__ void __launch_bounds__(V <= 2 ? 1024 : 512)
+__global__ void __launch_bounds__(V <= 2 ? 1024 : 512, SILU ? 2 : 1)
 quant_rows_kernel(const RowQuantArgs a) {
     // in this order: what starts after this kernel may rely on everything in front of it having ended
     pdl_wait_prior();
@@ -222,7 +222,8 @@ int launch_rows(const RowQuantArgs& a, long long rows, cudaStream_t s) {
     }
     // Four pieces a thread make small CTAs, so that loads of one row cover the arithmetic of others:
     // 4096 x 4096 bf16 7.6 us (10.0 with two pieces), 4096 x 14336 27.1 (38.9).  SiLU holds twice the
-    // inputs and its results in registers: two pieces, 8192 x 14336 f32 222 us (265 with four).
+    // inputs and its results in registers: two pieces, and few enough of them that two rows are resident
+    // (8192 x 14336 bf16 160 us, 188 with one row at a time).
     const int v = nvec <= 128 ? 1 : (SILU ? 2 : 4);
     const dim3 block(static_cast<unsigned>(((nvec + v - 1) / v + 31) / 32 * 32));
     if (v == 1) LSG_CUDA_TRY(launch_kernel(quant_rows_kernel<T, SILU, 1>, grid, block, 0, s, true, a));
