@@ -752,6 +752,12 @@ int launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const MmaArgs& a, int
     return LSG_OK;
 }
 
+// Clusters of CTAs that take an SM each (all forms do) that the device holds at a time.
+template <int CTAS>
+int resident(ClusterSlots& seen) {
+    return cluster_slots(int8_mma_kernel<1, false, CTAS, true>, CTAS, kThreads, 227 * 1024, seen);
+}
+
 int round_up(int v, int step) { return (v + step - 1) / step * step; }
 
 struct Plan {
@@ -769,10 +775,11 @@ struct Plan {
 // Against one rule per row count (even tiles of up to 256 tokens, cut when fewer than half the SMs have one):
 // 1001 x 1024 x 4096 12.9 -> 9.7 us, 512 x 4096 x 4096 15.2 -> 11.5, 600 x 2000 x 1024 9.0 -> 5.5, 1500 x 4096 x
 // 4096 25.6 -> 22.3.
-Plan plan_dense(int M, int N, int kblocks, int sms) {
+// slots: clusters of 1, 2, 4, 8 CTAs that are resident at a time.
+Plan plan_dense(int M, int N, int kblocks, const int (&slots)[4]) {
+    const int sms = slots[0];
     const long long ctas = (N + kRows - 1) / kRows;
     const long long bytes = static_cast<long long>(N) * kblocks * kKB;
-    static const int slots[4] = {0, 74, 33, 15};            // clusters of 2, 4, 8 CTAs that are resident on a B200
     Plan best = {256, false, 1};
     long long least = -1;
     const auto consider = [&](int tile, bool pair, int split, long long units, long long active, long long rounds) {
@@ -799,7 +806,7 @@ Plan plan_dense(int M, int N, int kblocks, int sms) {
             if (n * ctas <= slots[c] && kblocks >= (2 << c)) consider(tile, false, 1 << c, n, n * ctas << c, 1);
         const int even = round_up(tile, 32);
         const long long m = (M + even - 1) / even, pairs = m * ((ctas + 1) / 2);
-        if (tile >= 32) consider(even, true, 1, m, 2 * pairs, (pairs + sms / 2 - 1) / (sms / 2));
+        if (tile >= 32 && slots[1] > 0) consider(even, true, 1, m, 2 * pairs, (pairs + slots[1] - 1) / slots[1]);
         if (tile <= 32) break;
     }
     return best;
@@ -820,7 +827,9 @@ int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
     a.early = early ? 1 : 0;
     a.status = device_status_word();
     a.limit = wait_limit_cycles();
-    const int sms = sm_count();
+    static ClusterSlots seen;
+    const int slots[4] = {sm_count(), resident<2>(seen), resident<4>(seen), resident<8>(seen)};
+    const int sms = slots[0];
     const int per_cta = swiglu ? kRows / 2 : kRows;             // output columns of a CTA
     const int cta_tiles = (g.N + per_cta - 1) / per_cta;
     Plan plan;
@@ -831,9 +840,9 @@ int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
         const long long share = (static_cast<long long>(g.M) + g.E - 1) / g.E, most = share + share * 2 / 5;
         plan.tile = most >= 256 ? 256 : (most > 64 ? round_up(static_cast<int>(most), 32) : round_up(static_cast<int>(most), 16));
         plan.split = 1;
-        plan.pair = plan.tile > 64 && (g.M / plan.tile + static_cast<long long>(std::min(g.E, g.M))) * cta_tiles >= sms / 2;
+        plan.pair = slots[1] > 0 && plan.tile > 64 && (g.M / plan.tile + static_cast<long long>(std::min(g.E, g.M))) * cta_tiles >= sms / 2;
     } else {
-        plan = plan_dense(g.M, g.N, a.kblocks, sms);
+        plan = plan_dense(g.M, g.N, a.kblocks, slots);
     }
     const int tile = plan.tile, split = plan.split;
     const bool pair = plan.pair;
@@ -864,7 +873,7 @@ int int8_mma(const Int8Gemm& g, bool swiglu, bool early, cudaStream_t s) {
     const auto go = [&](auto w) {
         constexpr bool W = decltype(w)::value;
         if (pair) {
-            const int grid = 2 * std::min(count, sms / 2);
+            const int grid = 2 * std::min(count, slots[1]);
             return swiglu ? launch<2, true, 1, W>(tmW, tmX, a, grid, 2, s) : launch<2, false, 1, W>(tmW, tmX, a, grid, 2, s);
         }
         if (split == 8) return launch<1, false, 8, W>(tmW, tmX, a, count * 8, 8, s);
