@@ -761,8 +761,10 @@ LSG_API int lsg_moe_permute(const void* hidden_bf16, const int32_t* perm, int ro
 LSG_API int lsg_moe_unpermute(const void* y_bf16, const int32_t* inv_perm, const float* topk_weights,
                               int num_tokens, int top_k, int H, void* out_bf16, void* stream);
 
-/* The same two in bf16, fp16 or f32 (lsg_dtype), for any H; rows outside [0, rows) are pairs without
- * a row (unpermute: they add nothing), perm entries outside the pairs leave their row as it is. */
+/* The same two in bf16, fp16 or f32 (lsg_dtype), for any H and any rows aligned to their type; rows
+ * outside [0, rows) are pairs without a row (unpermute: they add nothing), perm entries outside the
+ * pairs leave their row as it is.  unpermute: top_k <= 16, but for bf16 rows of even H on 4-byte
+ * boundaries, which have any number of slots. */
 LSG_API int lsg_moe_permute_dtype(const void* hidden, int dtype, const int32_t* perm, int rows, int num_tokens, int top_k,
                                   int H, void* out, void* stream);
 LSG_API int lsg_moe_unpermute_dtype(const void* y, int dtype, const int32_t* inv_perm, const float* topk_weights, int rows,

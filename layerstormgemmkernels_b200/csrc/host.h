@@ -24,6 +24,14 @@ bool fused_quant_ok(int M, int K, const void* A);
 int dequant_gemm(int type, int M, int N, int K, const void* A, const void* W, void* C, int ldc,
                  int out_f32, cudaStream_t stream);
 
+// bf16 rows to the experts (whole 16-byte pieces, any number of slots) and back (pairs of values).  Entries of perm
+// outside the tokens' pairs leave their row as it is, entries of inv outside [0, rows) are pairs without a row.
+bool moe_gather_bf16_takes(const void* hidden, const void* out, int H);
+int moe_gather_bf16(const void* hidden, const int32_t* perm, int rows, int tokens, int top_k, int H, void* out, cudaStream_t s);
+bool moe_combine_bf16_takes(const void* y, const void* out, int H);
+int moe_combine_bf16(const void* y, const int32_t* inv, const float* w, int rows, int tokens, int top_k, int H, void* out,
+                     cudaStream_t s);
+
 int build_active_expert_list(const int32_t* offs, int E, int cap, int* active, cudaStream_t s);
 // `rows` bounds every offset read from the device: offsets that run past the caller's row
 // count (an expert-parallel receive buffer that overflowed) can then never index past it.

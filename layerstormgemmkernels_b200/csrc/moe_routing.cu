@@ -272,23 +272,25 @@ moe_permutation_small_kernel(const int32_t* __restrict__ idx, int P, int E, int3
     if (tid < P && tid >= placed) perm[tid] = 0;
 }
 
-// out[row, :] = hidden[perm[row] / k, :]   (bf16 rows, 16-byte vectors)
+// out[row, :] = hidden[perm[row] / k, :]   (bf16 rows, 16-byte vectors); an entry that names no token's pair
+// leaves its row as it is
 __global__ void __launch_bounds__(256)
-moe_gather_kernel(const uint4* __restrict__ hidden, const int32_t* __restrict__ perm, int k, int rows,
+moe_gather_kernel(const uint4* __restrict__ hidden, const int32_t* __restrict__ perm, int k, int rows, int tokens,
                   int vec_per_row, uint4* __restrict__ out) {
     pdl_launch_dependents();
     pdl_wait_prior();
     const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= static_cast<long long>(rows) * vec_per_row) return;
     const int row = static_cast<int>(i / vec_per_row), c = static_cast<int>(i - static_cast<long long>(row) * vec_per_row);
-    out[i] = __ldg(hidden + static_cast<size_t>(perm[row] / k) * vec_per_row + c);
+    const int pair = perm[row], token = pair / k;
+    if (pair >= 0 && token < tokens) out[i] = __ldg(hidden + static_cast<size_t>(token) * vec_per_row + c);
 }
 
 // out[t, :] = sum_s w[t, s] * y[inv[t * k + s], :], slots in order, fp32 accumulate; a pair without a
-// row (inv < 0) adds nothing.
+// row (inv outside [0, rows)) adds nothing.
 __global__ void __launch_bounds__(256)
 moe_combine_kernel(const __nv_bfloat16* __restrict__ y, const int32_t* __restrict__ inv,
-                   const float* __restrict__ w, int T, int k, int H, __nv_bfloat16* __restrict__ out) {
+                   const float* __restrict__ w, int rows, int T, int k, int H, __nv_bfloat16* __restrict__ out) {
     pdl_launch_dependents();
     pdl_wait_prior();
     const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -298,7 +300,7 @@ moe_combine_kernel(const __nv_bfloat16* __restrict__ y, const int32_t* __restric
     float a0 = 0.0f, a1 = 0.0f;
     for (int s = 0; s < k; ++s) {
         const int row = inv[static_cast<size_t>(t) * k + s];
-        if (row < 0) continue;
+        if (row < 0 || row >= rows) continue;
         const float ws = w[static_cast<size_t>(t) * k + s];
         const __nv_bfloat162 v = reinterpret_cast<const __nv_bfloat162*>(y + static_cast<size_t>(row) * H)[c];
         a0 = fmaf(ws, __bfloat162float(v.x), a0);
@@ -313,7 +315,7 @@ moe_combine_kernel(const __nv_bfloat16* __restrict__ y, const int32_t* __restric
 template <int KMAX>
 __global__ void __launch_bounds__(256)
 moe_combine_vec_kernel(const uint4* __restrict__ y, const int32_t* __restrict__ inv, const float* __restrict__ w,
-                       int k, int vpr, uint4* __restrict__ out) {
+                       int rows, int k, int vpr, uint4* __restrict__ out) {
     pdl_launch_dependents();
     pdl_wait_prior();
     const int t = blockIdx.x;
@@ -324,8 +326,9 @@ moe_combine_vec_kernel(const uint4* __restrict__ y, const int32_t* __restrict__ 
         for (int s = 0; s < KMAX; ++s) {
             if (s < k) {
                 const int row = __ldg(inv + static_cast<size_t>(t) * k + s);
-                ws[s] = row >= 0 ? __ldg(w + static_cast<size_t>(t) * k + s) : 0.0f;
-                r[s] = row >= 0 ? __ldg(y + static_cast<size_t>(row) * vpr + v) : make_uint4(0, 0, 0, 0);
+                const bool has = row >= 0 && row < rows;
+                ws[s] = has ? __ldg(w + static_cast<size_t>(t) * k + s) : 0.0f;
+                r[s] = has ? __ldg(y + static_cast<size_t>(row) * vpr + v) : make_uint4(0, 0, 0, 0);
             }
         }
         float acc[8];
@@ -487,19 +490,50 @@ extern "C" int lsg_moe_permutation(const int32_t* topk_idx, int num_tokens, int 
     return LSG_OK;
 }
 
+namespace lsg {
+
+bool moe_gather_bf16_takes(const void* hidden, const void* out, int H) {
+    return H % 8 == 0 && ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+}
+
+int moe_gather_bf16(const void* hidden, const int32_t* perm, int rows, int tokens, int top_k, int H, void* out, cudaStream_t s) {
+    const int vpr = H / 8;
+    const long long total = static_cast<long long>(rows) * vpr;
+    LSG_CUDA_TRY(launch_kernel(moe_gather_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0, s, true,
+                               static_cast<const uint4*>(hidden), perm, top_k, rows, tokens, vpr, static_cast<uint4*>(out)));
+    return LSG_OK;
+}
+
+bool moe_combine_bf16_takes(const void* y, const void* out, int H) {
+    return H % 2 == 0 && ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) & 3) == 0;
+}
+
+int moe_combine_bf16(const void* y, const int32_t* inv, const float* w, int rows, int tokens, int top_k, int H, void* out,
+                     cudaStream_t s) {
+    if (H % 8 == 0 && top_k <= 8 && ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) & 15) == 0) {
+        const int vpr = H / 8;
+        const int threads = vpr >= 256 ? 256 : ((vpr + 31) / 32) * 32;
+        LSG_CUDA_TRY(launch_kernel(moe_combine_vec_kernel<8>, dim3(static_cast<unsigned>(tokens)), dim3(threads), 0, s, true,
+                                   static_cast<const uint4*>(y), inv, w, rows, top_k, vpr, static_cast<uint4*>(out)));
+        return LSG_OK;
+    }
+    const long long total = static_cast<long long>(tokens) * (H / 2);
+    LSG_CUDA_TRY(launch_kernel(moe_combine_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0, s, true,
+                               static_cast<const __nv_bfloat16*>(y), inv, w, rows, tokens, top_k, H, static_cast<__nv_bfloat16*>(out)));
+    return LSG_OK;
+}
+
+}  // namespace lsg
+
+// These two know neither the tokens nor the rows: indices are bounded from below only.
 extern "C" int lsg_moe_permute(const void* hidden_bf16, const int32_t* perm, int rows, int top_k, int H,
                                void* out_bf16, void* stream) {
     if (H < 0) return fail(LSG_ERR_INVALID, "moe_permute: negative shape");
     if (rows <= 0 || H == 0) return LSG_OK;
     if (!hidden_bf16 || !perm || !out_bf16) return fail(LSG_ERR_INVALID, "moe_permute: null pointer");
-    if (H % 8 != 0 || (reinterpret_cast<uintptr_t>(hidden_bf16) & 15) || (reinterpret_cast<uintptr_t>(out_bf16) & 15))
+    if (!moe_gather_bf16_takes(hidden_bf16, out_bf16, H))
         return fail(LSG_ERR_ALIGNMENT, "moe_permute: H must be a multiple of 8 and buffers 16-byte aligned");
-    const int vpr = H / 8;
-    const long long total = static_cast<long long>(rows) * vpr;
-    LSG_CUDA_TRY(launch_kernel(moe_gather_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0,
-                               static_cast<cudaStream_t>(stream), true, static_cast<const uint4*>(hidden_bf16),
-                               perm, top_k, rows, vpr, static_cast<uint4*>(out_bf16)));
-    return LSG_OK;
+    return moe_gather_bf16(hidden_bf16, perm, rows, 0x7fffffff, top_k, H, out_bf16, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int lsg_moe_unpermute(const void* y_bf16, const int32_t* inv_perm, const float* topk_weights,
@@ -508,21 +542,10 @@ extern "C" int lsg_moe_unpermute(const void* y_bf16, const int32_t* inv_perm, co
     if (num_tokens <= 0 || H == 0) return LSG_OK;
     if (!y_bf16 || !inv_perm || !topk_weights || !out_bf16) return fail(LSG_ERR_INVALID, "moe_unpermute: null pointer");
     if (H % 2 != 0) return fail(LSG_ERR_INVALID, "moe_unpermute: H must be even");
-    if ((reinterpret_cast<uintptr_t>(y_bf16) | reinterpret_cast<uintptr_t>(out_bf16)) & 3)
+    if (!moe_combine_bf16_takes(y_bf16, out_bf16, H))
         return fail(LSG_ERR_ALIGNMENT, "moe_unpermute: rows are read in pairs of bf16, on 4-byte boundaries");
-    if (H % 8 == 0 && top_k <= 8 && ((reinterpret_cast<uintptr_t>(y_bf16) | reinterpret_cast<uintptr_t>(out_bf16)) & 15) == 0) {
-        const int vpr = H / 8;
-        const int threads = vpr >= 256 ? 256 : ((vpr + 31) / 32) * 32;
-        LSG_CUDA_TRY(launch_kernel(moe_combine_vec_kernel<8>, dim3(static_cast<unsigned>(num_tokens)), dim3(threads), 0,
-                                   static_cast<cudaStream_t>(stream), true, static_cast<const uint4*>(y_bf16), inv_perm,
-                                   topk_weights, top_k, vpr, static_cast<uint4*>(out_bf16)));
-        return LSG_OK;
-    }
-    const long long total = static_cast<long long>(num_tokens) * (H / 2);
-    LSG_CUDA_TRY(launch_kernel(moe_combine_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0,
-                               static_cast<cudaStream_t>(stream), true, static_cast<const __nv_bfloat16*>(y_bf16),
-                               inv_perm, topk_weights, num_tokens, top_k, H, static_cast<__nv_bfloat16*>(out_bf16)));
-    return LSG_OK;
+    return moe_combine_bf16(y_bf16, inv_perm, topk_weights, 0x7fffffff, num_tokens, top_k, H, out_bf16,
+                            static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int lsg_ep_expert_order(const int32_t* recv_counts, int world, int experts_per_rank, int rows,

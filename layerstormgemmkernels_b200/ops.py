@@ -831,13 +831,14 @@ def ep_expert_order(recv_counts, world, experts_per_rank, rows):
 
 
 def moe_permute(hidden, perm, top_k):
-    """out[row] = hidden[perm[row] // top_k], bf16, fp16 or fp32 [T,H] -> [rows,H]."""
+    """out[row] = hidden[perm[row] // top_k], bf16, fp16 or fp32 [T,H] -> [rows,H]; rows whose entry of
+    perm lies outside the T*k pairs are uninitialised."""
     return _host.moe_permute(hidden, perm, top_k)
 
 
 def moe_unpermute(y, inv_perm, topk_weights, output_dtype=None):
     """out[t] = sum over slots of topk_weights[t,s] * y[inv_perm[t*k+s]], bf16, fp16 or fp32; pairs
-    without a row (inv_perm < 0) add nothing.
+    without a row (inv_perm outside [0, rows)) add nothing.
 
     The sum is rounded once to the rows' type; fp32 rows also go to output_dtype 'bf16' or 'fp16', so
     that experts' rows kept in fp32 leave with one rounding (bf16 rows make it two)."""

@@ -68,7 +68,6 @@ void need_pairs(const char* op, const char* name, const Tensor& t, at::ScalarTyp
     if (t.scalar_type() != type || t.device() != like.device() || !t.is_contiguous() || t.numel() != n)
         refuse(op, std::string(name) + " must be " + std::to_string(n) + " contiguous values of " + c10::toString(type) + " on the rows' device");
 }
-bool lies_on(const Tensor& t, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
 // Sizes that the C ABI takes as int.
 int as_int(const char* op, int64_t v) {
     if (v < 0 || v > 0x7fffffff) refuse(op, "a size is outside 0 .. 2^31 - 1");
@@ -247,13 +246,8 @@ Tensor moe_permute(const Tensor& hidden, const Tensor& perm, int64_t top_k) {
     if (top_k < 1) refuse(op, "top_k must be positive");
     On on(hidden);
     Tensor out = empty({rows, H}, hidden.scalar_type(), hidden);
-    const int32_t* p = static_cast<const int32_t*>(perm.data_ptr());
-    // bf16 in whole 16-byte pieces: a thread a piece (4096 x 8 rows of 768 13.9 us, 34.7 with a CTA a row)
-    if (hidden.scalar_type() == at::kBFloat16 && H % 8 == 0 && lies_on(hidden, 16))
-        check(lsg_moe_permute(hidden.data_ptr(), p, as_int(op, rows), as_int(op, top_k), as_int(op, H), out.data_ptr(), on.stream));
-    else
-        check(lsg_moe_permute_dtype(hidden.data_ptr(), code_of(hidden.scalar_type()), p, as_int(op, rows), as_int(op, T),
-                                    as_int(op, top_k), as_int(op, H), out.data_ptr(), on.stream));
+    check(lsg_moe_permute_dtype(hidden.data_ptr(), code_of(hidden.scalar_type()), static_cast<const int32_t*>(perm.data_ptr()),
+                                as_int(op, rows), as_int(op, T), as_int(op, top_k), as_int(op, H), out.data_ptr(), on.stream));
     return out;
 }
 
@@ -267,14 +261,9 @@ Tensor moe_unpermute(const Tensor& y, const Tensor& inv_perm, const Tensor& topk
     const at::ScalarType from = y.scalar_type(), to = output_dtype.has_value() ? out_type(*output_dtype) : from;
     On on(y);
     Tensor out = empty({T, H}, to, y);
-    const int32_t* inv = static_cast<const int32_t*>(inv_perm.data_ptr());
-    const float* w = static_cast<const float*>(topk_weights.data_ptr());
-    // bf16 in pairs has any number of slots, and 512 x 6 rows of 2048 take 2.7 us (3.8 by slots)
-    if (from == at::kBFloat16 && to == from && H % 2 == 0 && lies_on(y, 4))
-        check(lsg_moe_unpermute(y.data_ptr(), inv, w, as_int(op, T), as_int(op, k), as_int(op, H), out.data_ptr(), on.stream));
-    else
-        check(lsg_moe_unpermute_to(y.data_ptr(), code_of(from), inv, w, as_int(op, rows), as_int(op, T), as_int(op, k), as_int(op, H),
-                                   out.data_ptr(), code_of(to), on.stream));
+    check(lsg_moe_unpermute_to(y.data_ptr(), code_of(from), static_cast<const int32_t*>(inv_perm.data_ptr()),
+                               static_cast<const float*>(topk_weights.data_ptr()), as_int(op, rows), as_int(op, T), as_int(op, k),
+                               as_int(op, H), out.data_ptr(), code_of(to), on.stream));
     return out;
 }
 

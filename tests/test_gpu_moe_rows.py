@@ -121,3 +121,40 @@ def test_rows_refused(ops, dtype):
                 lambda: ops.moe_unpermute(y, inv, w.cpu())):
         with pytest.raises(RuntimeError, match="must be"):
             bad()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("T,k,H", [(1, 1, 2), (6, 4, 34), (9, 8, 2048), (40, 12, 264), (5, 3, 33)])
+def test_indices_outside_the_rows(ops, T, k, H, dtype):
+    """An index that names no row, or no token's pair, on either side: such a pair adds nothing, such a row
+    is not written."""
+    g = torch.Generator().manual_seed(T * k + H)
+    rows = T * k - (1 if T > 1 else 0)                      # y one row short of the pairs
+    inv = torch.randperm(T * k, generator=g).int()
+    far = torch.tensor([rows, rows + 1, 2 ** 31 - 1, 2 ** 30, -1, -2 ** 31], dtype=torch.int64).int()
+    inv[::3] = far[torch.arange(len(inv[::3])) % 6]
+    w = torch.rand(T, k, generator=g) + 0.1
+    y = torch.randn(rows, H, generator=g).to(dtype)
+    out = ops.moe_unpermute(y.cuda(), inv.cuda(), w.cuda())
+    check_sum(out, y, torch.where((inv >= 0) & (inv < rows), inv, torch.full_like(inv, -1)), w)
+    x = torch.randn(T, H, generator=g).to(dtype)
+    perm = torch.arange(T * k, dtype=torch.int32)
+    perm[::2] = torch.tensor([T * k, T * k + 7, 2 ** 31 - 1, -1, -k, -2 ** 31], dtype=torch.int64).int()[torch.arange(len(perm[::2])) % 6]
+    good = (perm >= 0) & (perm < T * k)
+    got = ops.moe_permute(x.cuda(), perm.cuda(), k).cpu()
+    assert torch.equal(got[good], x[(perm[good] // k).long()])
+
+
+def test_more_than_sixteen_slots(ops):
+    """bf16 rows in pairs have any number of slots; other rows at most 16 on the way back."""
+    g = torch.Generator().manual_seed(1)
+    T, k, H = 7, 20, 66
+    inv, w = torch.randperm(T * k, generator=g).int().cuda(), torch.rand(T, k, generator=g).cuda()
+    y = torch.randn(T * k, H, generator=g)
+    check_sum(ops.moe_unpermute(y.to(BF16).cuda(), inv, w), y.to(BF16), inv, w)
+    x = torch.randn(T, H, generator=g).cuda()
+    for dtype in (BF16, FP16, FP32):
+        assert torch.equal(ops.moe_permute(x.to(dtype), inv, k), x.to(dtype)[(inv // k).long()])
+    for bad in (y.cuda(), y.half().cuda(), y[:, 1:].to(BF16).contiguous().cuda()):
+        with pytest.raises(ValueError, match="top_k"):
+            ops.moe_unpermute(bad, inv, w)
