@@ -232,20 +232,18 @@ __device__ __forceinline__ uint8_t code1(float x, const RowScale& r) {
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-// Four at a time: few registers are held over the look at values in doubt.
-template <typename T>
-__device__ __forceinline__ uint32_t code4(const float* f, const RowScale& r) {
+// Four fp32 values: few registers are held over the look at what is in doubt.
+__device__ __forceinline__ uint32_t code4(const float (&f)[8], int at, const RowScale& r) {
     uint32_t q[4];
+    float least = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = code_bits<T>(f[j], r);
-    if constexpr (std::is_same<T, float>::value) {
-        float least = 0.0f;
+    for (int j = 0; j < 4; ++j) {
+        q[j] = code_bits<float>(f[at + j], r);
+        least = fminf(least, above_code(f[at + j], q[j], r));
+    }
+    if (least < kDoubt) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) least = fminf(least, above_code(f[j], q[j], r));
-        if (least < kDoubt) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] = settle(f[j], q[j], r);
-        }
+        for (int j = 0; j < 4; ++j) q[j] = settle(f[at + j], q[j], r);
     }
     return pack4(q[0], q[1], q[2], q[3]);
 }
@@ -256,8 +254,14 @@ __device__ __forceinline__ uint2 code8(float (&f)[8], const RowScale& r) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] *= 0x1p64f;
     }
-    const uint32_t low = code4<T>(f, r);
-    return make_uint2(low, code4<T>(f + 4, r));
+    if constexpr (std::is_same<T, float>::value) {
+        const uint32_t low = code4(f, 0, r);
+        return make_uint2(low, code4(f, 4, r));
+    }
+    uint32_t q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = code_bits<T>(f[j], r);
+    return make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
 }
 
 #endif  // __CUDACC__

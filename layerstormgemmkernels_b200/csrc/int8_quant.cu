@@ -95,7 +95,7 @@ quant_short_rows_kernel(const RowQuantArgs a, long long rows) {
 
 // V pieces of eight values per thread.
 template <typename T, bool SILU, int V>
-__global__ void __launch_bounds__(V <= 2 ? 1024 : 512, SILU ? 2 : 1)
+__global__ void __launch_bounds__(V <= 2 ? 1024 : 512, SILU ? 2 : 0)
 quant_rows_kernel(const RowQuantArgs a) {
     // in this order: what starts after this kernel may rely on everything in front of it having ended
     pdl_wait_prior();
