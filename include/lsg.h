@@ -782,7 +782,8 @@ LSG_API int lsg_moe_unpermute_to(const void* y, int dtype, const int32_t* inv_pe
  *   route      grad_logits[t,topk_idx[t,s]] = w[t,s] (grad_weights[t,s] - sum_r w[t,r] grad_weights[t,r]),
  *              0 for the experts not chosen (w = topk_weights, the softmax over the chosen logits)
  * A pair whose entry of inv_perm lies outside [0, rows) has no row: it adds nothing and its weight's
- * gradient is 0.  Rows of grad_y that no pair names are left as they are, except that with
+ * gradient is 0.  A row belongs to one pair at most (lsg_moe_permutation's do): of several pairs that
+ * name it, grad_y keeps one's gradient and not their sum.  Rows of grad_y that no pair names are left as they are, except that with
  * expert_offsets (int32 [num_experts + 1], may be null) the rows from expert_offsets[num_experts] on
  * are cleared; rows <= num_tokens * top_k.  No counterpart in the reference (it has no routing). */
 LSG_API int lsg_moe_permute_backward(const void* grad_rows, int dtype, const int32_t* inv_perm, int rows, int num_tokens,

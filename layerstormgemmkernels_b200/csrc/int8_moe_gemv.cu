@@ -9,8 +9,9 @@
 // Every CTA quantizes the activations for itself while its first weights arrive: two launches instead of four.
 // CTAs of the second product start beside those of the first one and have up to 14 MB of their weights in shared
 // memory when h is there.
-// One token, with routing and combining, 2 experts of 2048 / 2048: 11.3 us (four launches 17.4), 8 of 1024 / 512: 10.5
-// (14.5), 8 of 2048 / 768: 16.6 (19.5), 8 of 4096 / 1536: 37 (41); 4 tokens, 2 experts of 1024 / 1024 each: 12.4 (15.0).
+// One token, with the combination, 2 experts of 2048 / 2048: 13.7 us (four launches 19.5), 8 of 1024 / 512: 12.4
+// (15.7), 8 of 2048 / 768: 17.9 (20.1), 8 of 4096 / 1536: 38.6 (42); 4 tokens, 2 of 8 of 1024 / 1024 each: 14.4 (17.7).
+// The look at h values in doubt (settle) is 0.3 to 1 us of these.
 // Tried: copies of 512 bytes (18.6 for the third), one weight row a job (20), the jobs of a CTA side by side, which
 // needs the codes of fewer rows (19.0; 2 experts of 4096 / 8192 52 instead of 42), a scale loaded for each job (17.9).
 #include "common.cuh"
@@ -32,8 +33,10 @@ constexpr int kPiece = 1024;               // bytes of a weight row in a slot at
 constexpr int kSlots = 3;
 constexpr int kSlotBytes = kBlock * kPiece;
 constexpr int kRing = kSlots * kSlotBytes; // of a warp
-// Shared memory of a CTA of the second product: over half of an SM's, under what a CTA of the first leaves.  So every SM
-// takes one of them while the first product runs; where two fit, SMs that are done early take two.  48 registers for
+// Shared memory of a CTA of the second product: over half of an SM's, and under what a CTA of the first leaves while its
+// tokens are up to 13000 values (96 KB of ring and the codes, of 228 KB that hold both CTAs' 1.6 KB of their own too).
+// So every SM takes one of them while the first product runs (behind it, with more values); where two fit, SMs that are
+// done early take two.  48 registers for
 // the same reason: one token, 2 experts of 4096 / 8192 42 us, with up to 64 registers 48, and 54 where two fit as well.
 constexpr int kAlone = 116 * 1024;
 constexpr int kCodes = 16384;              // bytes of codes at most
@@ -307,8 +310,8 @@ int launch(Args a, cudaStream_t s) {
 
 // Rows that share an expert read its weights once each, and every CTA quantizes all tokens: with several tokens, only
 // while at most a quarter of the weights (or 25 MB) is expected to be read again and the tokens are up to 8192 values.
-// 4 tokens, 2 of 16 experts of 2048 / 2048 26.5 us here, 28.4 in four launches, 2 of 4 experts 25.7 and 22.1;
-// 8 tokens of 2048, 1 of 64 experts of 2048 / 1024 22.8 and 20.7.
+// 4 tokens, 2 of 16 experts of 2048 / 2048 27.3 us here, 29.6 in four launches, 2 of 4 experts 26.3 and 23.5;
+// 8 tokens of 2048, 1 of 64 experts of 2048 / 1024 23.1 and 21.9.
 bool int8_moe_gemv_takes(int tokens, int top_k, int E, int H, int I) {
     const long long rows = static_cast<long long>(tokens) * top_k;
     if (rows > kRows || static_cast<long long>(tokens) * H > kCodes || rows * I > kCodes) return false;

@@ -13,8 +13,10 @@
 // moves one code in eighty).
 //
 // Memory bound: one CTA per row, the row held in registers between the maximum and the codes, so
-// that every input byte is read once.  Rows that are not whole 16-byte pieces, or longer than
-// 16384 values, are read twice, value by value.
+// that every input byte is read once (4096 x 4096 bf16 6.5 us).  Rows that are not whole 16-byte
+// pieces, or longer than 16384 values, are read twice, value by value, and bound by the instructions
+// of that: 4096 x 4100 35 us, 2048 x 20000 90.  silu(g) * u is bound by its arithmetic: 8192 x 14336
+// bf16 161 us and f32 218, for 587 MB and 1.06 GB.
 #include "common.cuh"
 #include "host.h"
 #include "int8.cuh"

@@ -169,7 +169,9 @@ moe_copy_rows_kernel(const Piece<T, P>* __restrict__ x, const int32_t* __restric
 // One CTA per token: grad_out[t] is read once for all its slots.  Bound by bytes (y read, grad_y
 // written); small CTAs keep loads of other tokens under way while one sums its products: 16384 tokens
 // of 2048 bf16 values, eight slots, 5.0 TB/s with 256 threads, 6.1 with 64.  Few tokens take 256
-// threads (100 tokens: 64 would make the whole backward pass 12.0 us instead of 7.7).
+// threads (100 tokens: 64 would make the whole backward pass 12.0 us instead of 7.7).  Nine to sixteen
+// slots do not fit the 80 registers of three CTAs: their pieces spill (240 bytes a thread), 4096 tokens of
+// 2048 bf16 values, 16 slots 4.4 TB/s.
 template <typename T, int P, int K>
 __global__ void __launch_bounds__(256, 3)
 moe_unpermute_backward_kernel(const Piece<T, P>* __restrict__ grad_out, const Piece<T, P>* __restrict__ y,

@@ -783,7 +783,11 @@ def int8_moe_ffn(hidden, expert_offsets, inv_perm, top_k, gate_up, gate_up_scale
 
     hidden bf16 or fp16 [T,H]; gate_up int8 [E,2I,H] (gate rows, then up rows) with scales fp32
     [E,2I]; down int8 [E,H,I] with scales fp32 [E,H]; H and I multiples of 16.  Rows behind the
-    last expert's are uninitialised.  moe_unpermute takes the result back to the tokens."""
+    last expert's are uninitialised.  moe_unpermute takes the result back to the tokens.
+
+    Rows in 'bf16' are rounded a first time here and their sum a second time by moe_unpermute (2.35e-3
+    off for normal values); 'fp32' rows with moe_unpermute(..., 'bf16') leave one rounding (1.66e-3), for
+    1 us more at one token, 9 % at 4096 tokens of 8 experts of 4096 / 14336."""
     return _host.int8_moe_ffn(hidden, expert_offsets, inv_perm, top_k, gate_up, gate_up_scales, down, down_scales,
                               output_dtype)
 
@@ -846,7 +850,8 @@ def moe_unpermute(y, inv_perm, topk_weights, output_dtype=None):
 
 
 # ---------------------------------------------------------------------------
-# Gradients of the MoE routing steps
+# Gradients of the MoE routing steps: calls of their own, like the steps, which record nothing for
+# torch.autograd (the experts' products have no backward pass here)
 # ---------------------------------------------------------------------------
 def moe_permute_backward(grad_rows, inv_perm, top_k):
     """Gradient of moe_permute: grad_hidden[t] = sum over slots of grad_rows[inv_perm[t*k+s]], in
@@ -862,7 +867,8 @@ def moe_unpermute_backward(grad_out, y, inv_perm, topk_weights, expert_offsets=N
 
     grad_out [T,H] and y [rows,H] bf16, fp16 or fp32, alike; grad_weights fp32 [T,k].  With
     expert_offsets (int32, as moe_permutation returns them) the rows behind the last expert's are
-    cleared in grad_y; without them, rows that no pair names are uninitialised."""
+    cleared in grad_y; without them, rows that no pair names are uninitialised.  A row belongs to one
+    pair at most."""
     return _host.moe_unpermute_backward(grad_out, y, inv_perm, topk_weights, expert_offsets)
 
 
