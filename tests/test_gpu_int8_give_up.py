@@ -2,8 +2,8 @@
 under way and returns, and the next call gives the bits of the one before.
 
 The longest K makes it happen without a fault: the 1024 K blocks of a tile take 340 cycles each at least (16 KB of
-weights at 48 bytes a cycle), 0.17 ms, and 0.05 ms where four CTAs share them; a limit of one cycle gives a wait up
-after its first 17 looks of at most 2 us each."""
+weights at 48 bytes a cycle), 0.17 ms, and 0.1 ms for tiles of 256 tokens that four CTAs share; a limit of one cycle
+gives a wait up after its first 17 looks of at most 2 us each."""
 import pytest
 import torch
 
@@ -51,7 +51,7 @@ def test_rows_of_experts(ops, rows, N):
     gives_up_and_goes_on(call)
 
 
-@pytest.mark.parametrize("M,N", [(100, 2000), (300, 1000), (1000, 4000)])      # K cut among clusters of four; pairs
+@pytest.mark.parametrize("M,N", [(500, 2000), (300, 4000), (1000, 4000)])      # K cut among four and two CTAs; pairs
 def test_dense_behind_the_quantizer(ops, M, N):
     """Weights are under way before the quantizer has ended."""
     x = torch.randn(M, K, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(BF16)
